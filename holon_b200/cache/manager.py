@@ -47,7 +47,8 @@ class CacheGroup:
         self.first = np.zeros(max_seqs + 1, dtype=np.int64)       # first logical page still held behind the kept ones
         self.count = np.zeros(max_seqs + 1, dtype=np.int64)       # logical pages reserved so far
         self.dirty: set[int] = set()
-        self.kv = torch.zeros((len(entries), pages + 1, *decl.page_shape(page_size)), dtype=dtype, device=device)
+        self.kv = torch.zeros((len(entries), pages + 1, *decl.page_shape(page_size)), dtype=getattr(decl, "dtype", None) or dtype,
+                              device=device)
         self.table_device = torch.from_numpy(self.table).to(device)
 
     @staticmethod
@@ -134,8 +135,8 @@ class CacheManager:
         for e in entries:
             if e.decl is not None:
                 by_decl.setdefault(e.decl, []).append(e.entry)
-        itemsize = torch.empty((), dtype=dtype).element_size()
-        per_page = sum(CacheGroup.page_bytes(d, len(es), page_size, itemsize) for d, es in by_decl.items())
+        itemsize = lambda d: (getattr(d, "dtype", None) or dtype).itemsize        # noqa: E731
+        per_page = sum(CacheGroup.page_bytes(d, len(es), page_size, itemsize(d)) for d, es in by_decl.items())
         least = math.ceil(max_model_len / page_size)
         if pages is None:
             if state_memory is None:

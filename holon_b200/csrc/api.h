@@ -52,6 +52,24 @@ int hb_qk_norm_rope_kv_write(void* q_out, const void* qkv, int dtype, const int3
                              int pages, int page_size, int tokens, int heads, int kv_heads, int head_dim,
                              const void* bias, hb_stream stream);
 
+// The same into a cache of 8-bit codes (csrc/cache8.cuh): kv [pages, 2, kv_heads, page_size, head_dim + 1] bytes, where the
+// block of a (page, part, kv head) holds page_size rows of head_dim codes and then page_size scale bytes. bfloat16 qkv; nothing is
+// rounded on the way to the codes. head_dim a multiple of 16 up to 1024, page_size a multiple of 16.
+int hb_qk_norm_rope_kv_write8(void* q_out, const void* qkv, const int32_t* positions, const float* table, int rotary_dim,
+                              int max_positions, const void* q_weight, const void* k_weight, int weight_dtype, float eps,
+                              float offset, void* kv, const int32_t* write_index, int pages, int page_size, int tokens, int heads,
+                              int kv_heads, int head_dim, const void* bias, hb_stream stream);
+// Such pages read back: out [count, 2, kv_heads, page_size, head_dim] (`dtype`) = the values of pages index[0 .. count - 1]; an
+// index that names no page gives zeros.
+int hb_kv_read(void* out, int dtype, const void* kv, const int32_t* index, int count, int pages, int kv_heads, int page_size,
+               int head_dim, hb_stream stream);
+// The pages that the new tokens of rows row0 .. rows - 1 see, in bfloat16 for an attention kernel: page i of row b to page
+// (b - row0) * stride + i of out, rows behind a row's last key as zeros, pages before its window not at all. Also makes the
+// tables that go with it: table [rows - row0, stride], slots [rows] (from row0 on). stride: at least the pages of the longest row.
+int hb_kv_read_rows(void* out, int32_t* table, int32_t* slots, const void* kv, const int32_t* block_table, int table_stride,
+                    const int32_t* row_slot, const int32_t* query_start, const int32_t* kv_len, int row0, int rows, int stride,
+                    int pages, int kv_heads, int page_size, int head_dim, int window, hb_stream stream);
+
 // Attention of the step's new rows over the paged cache, any sizes, on CUDA cores with 32-bit arithmetic.
 // Row b owns query rows query_start[b] .. query_start[b+1], the last ones of its kv_len[b] tokens; a query at position
 // p sees keys j <= p, with window > 0 only p - j < window. `sinks` (float [heads], or null): each head's softmax
@@ -88,6 +106,28 @@ int hb_attention_decode_bf16_cluster(void* out, const void* q, const void* kv, c
                                      const int32_t* kv_len, int rows, int heads, int kv_heads, int head_dim, int pages,
                                      int page_size, float scale, int window, int splits, const float* sinks,
                                      hb_stream stream);
+
+// One-token rows 0 .. rows - 1 over a cache of 8-bit codes (`kv8`) or of bfloat16, 1 to 16 splits that merge inside the kernel as a
+// cluster (csrc/attention_rows.cu). `skip` (or null): tokens at a row's start that it shares with other rows; it attends to those
+// behind them, and the partial results of hb_attention_prefix (part_o, part_ml, part_at, part_rows = hb_attention_prefix_rows()) are
+// joined with that. hb_attention_rows_capacity: clusters of that many CTAs that run at once (splits 1: CTAs an SM), -1 for
+// sizes that are refused.
+int hb_attention_rows_capacity(int kv8, int head_dim, int group, int splits);
+int hb_attention_rows(void* out, const void* q, const void* kv, int kv8, const int32_t* block_table, int table_stride,
+                      const int32_t* row_slot, const int32_t* query_start, const int32_t* kv_len, int rows, int heads, int kv_heads,
+                      int head_dim, int pages, int page_size, float scale, int window, int splits, const float* sinks,
+                      const int32_t* skip, const float* part_o, const float* part_ml, const int32_t* part_at, int part_rows,
+                      hb_stream stream);
+// Groups of one-token rows that hold the same first tokens in the same pages, over the keys of those (csrc/attention_prefix.cu):
+// groups [n_groups][3] = (start in `members`, rows, tokens), rows 0 for a group that is not there; `members` names rows of the
+// step. Leaves unnormalised results of `units` pieces of work, at most max(ctas, kv_heads * tiles) for tiles of
+// hb_attention_prefix_rows() / (heads / kv_heads) rows: part_o [units, hb_attention_prefix_rows(), head_dim], part_ml [units, ..., 2] and
+// per row of the step part_at int32 [rows, 4].
+int hb_attention_prefix_rows(void);
+int hb_attention_prefix(float* part_o, float* part_ml, int32_t* part_at, const void* q, const void* kv, int kv8,
+                        const int32_t* block_table, int table_stride, const int32_t* row_slot, const int32_t* query_start,
+                        const int32_t* members, const int32_t* groups, int n_groups, int heads, int kv_heads, int head_dim, int pages,
+                        int page_size, float scale, int ctas, hb_stream stream);
 
 // The same rows with the keys of all of them shared out evenly over `ctas` CTAs (one wave that fills the GPU): each
 // takes the same number of 64-key tiles, across rows and heads where its stretch crosses them, so rows of any lengths

@@ -43,13 +43,85 @@ class Rows:
         self.plan: dict = {}                           # what the kernel table worked out for these rows, for the next layer
 
 
+class SharedPrefix:
+    """Which one-token rows of a step hold the same first pages, so that attention reads the keys there once for all of them.
+
+    A group is two or more rows and the tokens that all of them share (whole pages, and fewer than any of them holds); a
+    row is in one group at most. Device, int32: `skip` [rows] (tokens that the row shares, 0 outside the groups), `members`
+    [rows] (the groups' rows, one group after the other; what follows is not read) and `groups` [3 · (rows // 2)] ((start in `members`,
+    rows, tokens) a group, zeros behind the last). Host: `rows`, and `longest_own`, the most tokens any row has beside those it shares."""
+
+    __slots__ = ("skip", "members", "groups", "rows", "longest_own")
+
+    LEAST = 256                # tokens that are read once in place of again (over a group's rows but one) from which a group pays
+
+    def __init__(self, skip, members, groups, rows: int, longest_own: int) -> None:
+        self.skip, self.members, self.groups, self.rows, self.longest_own = skip, members, groups, rows, longest_own
+
+    @classmethod
+    def find(cls, table: np.ndarray, kv_len: np.ndarray, page_size: int) -> dict | None:
+        """The arrays (host) and `longest_own` for rows that hold `kv_len` tokens in the pages `table` [rows, pages]; None where
+        no group is worth it. Rows that share more with some than with others go with the cut that saves most."""
+        n = len(kv_len)
+        limit = np.maximum((np.asarray(kv_len, dtype=np.int64) - 1) // page_size, 0)      # (a row's last token stays its own)
+        first = table[:, 0] if n > 1 and table.shape[1] else np.zeros(0, dtype=np.int32)
+        if len(np.unique(first)) == len(first):                       # (no two rows begin alike)
+            return None
+        found: list[tuple[list[int], int]] = []
+        for rows in cls._alike(range(n), table, limit, 0):
+            found += cls._cut(rows, table, limit, 0, page_size)[1]
+        if not found:
+            return None
+        skip, members, groups = np.zeros(n, dtype=np.int32), np.zeros(n, dtype=np.int32), np.zeros(3 * (n // 2), dtype=np.int32)
+        at = 0
+        for i, (rows, pages) in enumerate(found):
+            skip[rows] = pages * page_size
+            members[at:at + len(rows)] = rows
+            groups[3 * i:3 * i + 3] = at, len(rows), pages * page_size
+            at += len(rows)
+        return {"skip": skip, "members": members, "groups": groups, "longest_own": int((np.asarray(kv_len) - skip).max())}
+
+    @staticmethod
+    def _alike(rows, table, limit, page: int) -> list[list[int]]:
+        """The rows that still share at page number `page`, two or more with the same page, in their order."""
+        by: dict[int, list[int]] = {}
+        for r in rows:
+            if limit[r] > page:
+                by.setdefault(int(table[r, page]), []).append(r)
+        return [same for same in by.values() if len(same) > 1]
+
+    @classmethod
+    def _cut(cls, rows: list[int], table, limit, page: int, page_size: int) -> tuple[int, list]:
+        """(tokens saved, groups as (rows, pages)) for rows that share all pages up to number `page`, and that one."""
+        most = int(limit[rows].min())
+        cells = table[rows, page:most]
+        same = (cells == cells[0]).all(0)
+        pages = most if same.all() else page + int(np.argmin(same))
+        saved = pages * page_size * (len(rows) - 1)
+        whole = (saved, [(rows, pages)]) if saved >= cls.LEAST else (0, [])
+        parts = [cls._cut(more, table, limit, pages, page_size) for more in cls._alike(rows, table, limit, pages)]
+        apart = sum(p[0] for p in parts), [g for p in parts for g in p[1]]
+        return apart if apart[0] > whole[0] else whole
+
+    @classmethod
+    def of(cls, table: np.ndarray, kv_len: np.ndarray, page_size: int, device) -> "SharedPrefix | None":
+        """`find`, its arrays on the device."""
+        found = cls.find(table, kv_len, page_size)
+        if found is None:
+            return None
+        on = [torch.from_numpy(found[name]).to(device) for name in ("skip", "members", "groups")]
+        return cls(*on, len(kv_len), found["longest_own"])
+
+
 class GroupStep:
-    """One cache group's part of a step: the device block table and, per token, page · page_size + offset."""
+    """One cache group's part of a step: the device block table and, per token, page · page_size + offset; `shared`: which of
+    the one-token rows hold the same first pages of this group (None: none, or nobody asked)."""
 
-    __slots__ = ("block_table", "write_index", "page_size")
+    __slots__ = ("block_table", "write_index", "page_size", "decl", "shared")
 
-    def __init__(self, block_table, write_index, page_size) -> None:
+    def __init__(self, block_table, write_index, page_size, decl=None, shared: SharedPrefix | None = None) -> None:
         self.block_table, self.write_index, self.page_size = block_table, write_index, page_size
+        self.decl, self.shared = decl, shared
 
 
 class StepContext:

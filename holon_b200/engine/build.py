@@ -9,12 +9,14 @@ import numpy as np
 import torch
 
 from ..cache import CacheManager
+from ..config.engine import CACHE_DTYPES
 from ..config.registry import resolve_architecture
 from ..parts import BuildContext, Model
 from ..weights import load_weights
 from .batch import StepEntry
 from .runner import Runner
 
+GRAPH_PORTIONS = 2                            # prompt portions beside the decode rows of a step that runs as a graph
 TORCH_DTYPES = {"bfloat16": torch.bfloat16, "float32": torch.float32}
 
 
@@ -117,6 +119,7 @@ def _measure(model, ctx, entries, *, page_size: int, max_seqs: int, max_model_le
     largest = max(_peak_of(device, lambda counts=counts: step(counts)) for counts in cuts)
     largest += model.context_scratch(tokens, rows, max_model_len)
     graphed = _peak_of(device, lambda: step(ones + [n for n in portion if n > 0], graph=True)) + 4 * max_seqs * model.spec.vocab
+    graphed += model.graph_scratch(max_seqs, GRAPH_PORTIONS if chunk_with_decode else 0, max_model_len, page_size)
     del runner, cache
     torch.cuda.empty_cache()
     return largest, graphed
@@ -125,11 +128,17 @@ def _measure(model, ctx, entries, *, page_size: int, max_seqs: int, max_model_le
 def build(source, *, dtype: str, device, kernels=None, page_size: int, max_seqs: int, max_model_len: int,
           max_step_tokens: int, state_memory: int | None = None, pages: int | None = None,
           memory_fraction: float = 0.9, prefix_cache: bool = False, chunk_with_decode: int = 0,
-          cuda_graphs: bool = True) -> Built:
+          cuda_graphs: bool = True, cache_dtype: str = "auto", shared_prefix: bool = False) -> Built:
     """`kernels=None` loads the compiled CUDA kernels and fails if they cannot be had. With neither `state_memory`
     nor `pages` the cache pools take `memory_fraction` of the device memory that is free after the weights, less the
     measured activation peak of the largest step and (with `cuda_graphs`) of the largest step that graphs replay,
-    whose pool stays reserved."""
+    whose pool stays reserved. `cache_dtype`, `shared_prefix`: as in `EngineConfig`."""
+    if cache_dtype not in CACHE_DTYPES:
+        raise ValueError(f"cache_dtype must be one of {CACHE_DTYPES}, not {cache_dtype!r}")
+    if cache_dtype == "fp8" and (dtype != "bfloat16" or page_size % 16):
+        raise ValueError("an fp8 cache goes with dtype bfloat16 and a page_size that is a multiple of 16")
+    if shared_prefix and dtype != "bfloat16":
+        raise ValueError("shared_prefix goes with dtype bfloat16")
     device = torch.device(device)
     if kernels is None:
         from ..kernels import load_kernels
@@ -141,8 +150,11 @@ def build(source, *, dtype: str, device, kernels=None, page_size: int, max_seqs:
         raw = arch.complete(raw, source.shapes())
     config = arch.parse(raw)
     spec = arch.recipe(config)
-    ctx = BuildContext(device, tdtype, kernels, max_positions=max_model_len, max_step_tokens=max_step_tokens)
+    ctx = BuildContext(device, tdtype, kernels, max_positions=max_model_len, max_step_tokens=max_step_tokens, cache_dtype=cache_dtype,
+                       shared_prefix=shared_prefix, page_size=page_size)
     model = Model(spec, ctx)
+    if cache_dtype == "fp8" and not any(getattr(e.decl, "fp8", False) for e in model.entries):
+        raise ValueError("cache_dtype fp8 is for the cache of grouped-query attention, and this model has none")
     weight_bytes = load_weights(model, spec, source.tensors(), tdtype, device)
     activations = graphs = free_before = None
     if state_memory is None and pages is None:

@@ -18,11 +18,10 @@ from ..config.engine import EngineConfig
 from ..sampling import Sampler, SamplingParams, sampling_arrays, sequence_seed
 from ..weights import SafetensorsSource
 from .batch import StepEntry
-from .build import build
+from .build import GRAPH_PORTIONS, build
 from .scheduler import Request, Row, Scheduler, Status
 
 GRAPH_BUCKETS = (1, 2, 4, 8, 16, 24, 32, 48, 64, 96, 128, 192, 256)
-GRAPH_PORTIONS = 2                            # prompt portions beside the decode rows of a step that runs as a graph
 
 
 @dataclasses.dataclass
@@ -77,7 +76,8 @@ class Engine:
                            page_size=config.page_size, max_seqs=config.max_seqs, max_model_len=config.max_model_len,
                            max_step_tokens=config.max_step_tokens, state_memory=config.state_memory,
                            memory_fraction=config.memory_fraction, prefix_cache=config.prefix_cache,
-                           chunk_with_decode=config.chunk_with_decode, cuda_graphs=config.cuda_graphs)
+                           chunk_with_decode=config.chunk_with_decode, cuda_graphs=config.cuda_graphs,
+                           cache_dtype=config.cache_dtype, shared_prefix=config.shared_prefix)
         b = self.built
         self.device = b.ctx.device
         self.eos = frozenset(source.eos_token_ids())

@@ -13,7 +13,8 @@ import numpy as np
 import torch
 from torch.utils._device import DeviceContext
 
-from .batch import GroupStep, Rows, StepContext, StepEntry, Uploader
+from ..parts.base import PagedKV
+from .batch import GroupStep, Rows, SharedPrefix, StepContext, StepEntry, Uploader
 from .recorded import Reads
 
 
@@ -52,7 +53,9 @@ class Runner:
         self.device, self.max_step_tokens = build_ctx.device, max_step_tokens
         s, t, g = cache.max_seqs + 1, max_step_tokens, len(cache.groups)
         tables = sum(s * (group.max_pages + 1) + 8 for group in cache.groups)     # every block-table row changed at once
-        self.uploader = Uploader(t * (3 + g) + 16 * s + 64 + tables, self.device)
+        self._sharing = [group.index for group in cache.groups if build_ctx.shared_prefix and isinstance(group.decl, PagedKV)
+                         and group.decl.window <= 0]              # groups whose rows are looked over for pages that they share
+        self.uploader = Uploader(t * (3 + g) + 16 * s + 64 + tables + len(self._sharing) * (4 * s + 16), self.device)
         self.vocab = model.spec.vocab
         self._reads = None                                        # what recorded steps read (None: not looked at)
         self._use_graphs = self._graphs and Reads.declared(model) # whether steps may be recorded, as far as known
@@ -135,6 +138,14 @@ class Runner:
         up.put("from_last", from_last)
         for g in c.groups:
             up.put(f"write_index.{g.index}", g.write_index(token_slot, positions).astype(np.int32))
+        one = n_decode + pad_rows
+        sharing = {}
+        for i in self._sharing if n_decode > 1 else ():
+            found = SharedPrefix.find(c.groups[i].table[row_slot[:one]], kv_len[:one], c.groups[i].page_size)
+            if found is not None:
+                sharing[i] = found
+                for name in ("skip", "members", "groups"):
+                    up.put(f"shared.{name}.{i}", found[name])
         for name, array in (extra or {}).items():
             up.put(name, array)
         changed = []
@@ -151,7 +162,9 @@ class Runner:
                      max(counts), int(kv_len.max()), query_start, kv_len)
         if bucket:
             rows_.plan["any cut"] = True              # (a graph's launches serve every cut of its tokens into its rows)
-        groups = [GroupStep(g.table_device, dev[f"write_index.{g.index}"], g.page_size) for g in c.groups]
+        shared = {i: SharedPrefix(*(dev[f"shared.{name}.{i}"] for name in ("skip", "members", "groups")), one, found["longest_own"])
+                  for i, found in sharing.items()}
+        groups = [GroupStep(g.table_device, dev[f"write_index.{g.index}"], g.page_size, g.decl, shared.get(g.index)) for g in c.groups]
         step = StepContext(dev["token_ids"], dev["positions"], dev["logits_index"], rows_, groups, c)
         step.extra = {name: dev[name] for name in (extra or {})}
         step.from_last = dev["from_last"]

@@ -9,6 +9,7 @@ of up to 16 rows, SwiGLU's product with its activation, and float32 products run
 from __future__ import annotations
 
 import ctypes
+import math
 import os
 
 import torch
@@ -395,7 +396,11 @@ class CudaKernels:
 
     def qk_norm_rope_kv_write(self, q_out, qkv, positions, table, rotary_dim, q_weight, k_weight, eps, offset, kv,
                               write_index, heads, kv_heads, head_dim, bias=None) -> None:
-        """`bias` (qkv's dtype, [(heads + 2 kv_heads) head_dim], or None) is added to q, k and v first."""
+        """`bias` (qkv's dtype, [(heads + 2 kv_heads) head_dim], or None) is added to q, k and v first. A `kv` of bytes [pages, 2,
+        kv_heads, page_size, head_dim + 1] takes keys and values as 8-bit codes with a scale per row (csrc/cache8.cuh)."""
+        if kv is not None and kv.dtype == torch.uint8:
+            return self._kv_write8(q_out, qkv, positions, table, rotary_dim, q_weight, k_weight, eps, offset, kv, write_index, heads,
+                                   kv_heads, head_dim, bias)
         self._check(q_out, qkv, positions, table, q_weight, k_weight, kv, write_index, bias)
         t = qkv.shape[0]
         if bias is not None and (bias.shape != (qkv.shape[1],) or bias.dtype != qkv.dtype):
@@ -415,6 +420,48 @@ class CudaKernels:
                    self._p(kv), self._i32(write_index, "write_index"), kv.shape[0] if kv is not None else 0,
                    kv.shape[3] if kv is not None else 1, t, heads, kv_heads, head_dim, self._p(bias))
 
+    def _kv_write8(self, q_out, qkv, positions, table, rotary_dim, q_weight, k_weight, eps, offset, kv, write_index, heads,
+                   kv_heads, head_dim, bias) -> None:
+        self._check(q_out, qkv, positions, table, q_weight, k_weight, kv, write_index, bias)
+        t, width = qkv.shape[0], (heads + 2 * kv_heads) * head_dim
+        if qkv.dtype != torch.bfloat16 or q_out.dtype != torch.bfloat16 or qkv.shape != (t, width) or q_out.shape != (t, heads, head_dim):
+            raise KernelError("qk_norm_rope_kv_write: an 8-bit cache takes bfloat16 qkv [tokens, (heads + 2 kv_heads) head_dim] and q_out "
+                              "[tokens, heads, head_dim]")
+        if bias is not None and (bias.shape != (width,) or bias.dtype != qkv.dtype):
+            raise KernelError("qk_norm_rope_kv_write: bias must be one row of qkv's width and dtype")
+        if table is not None and (table.dtype != torch.float32 or table.shape[1] != rotary_dim):
+            raise KernelError("qk_norm_rope_kv_write: the rotation table must be float32 [positions, rotary_dim]")
+        if positions.shape != (t,) or write_index is None or write_index.shape != (t,):
+            raise KernelError("qk_norm_rope_kv_write: positions and write_index are int32 [tokens]")
+        gains = [w for w in (q_weight, k_weight) if w is not None]
+        if any(w.shape != (head_dim,) or w.dtype != gains[0].dtype for w in gains):
+            raise KernelError("qk_norm_rope_kv_write: the two norm weights are [head_dim], of one dtype")
+        pages, page_size = self._pages8(kv, kv_heads, head_dim)
+        self._call("hb_qk_norm_rope_kv_write8", self._p(q_out), self._p(qkv), self._i32(positions, "positions"), self._p(table),
+                   rotary_dim, table.shape[0] if table is not None else 0, self._p(q_weight), self._p(k_weight),
+                   _code(q_weight) if q_weight is not None else 0, ctypes.c_float(eps), ctypes.c_float(offset), self._p(kv),
+                   self._i32(write_index, "write_index"), pages, page_size, t, heads, kv_heads, head_dim, self._p(bias))
+
+    @staticmethod
+    def _pages8(kv, kv_heads: int, head_dim: int) -> tuple[int, int]:
+        """(pages, page size) of an 8-bit cache whose heads are these."""
+        if kv.dim() != 5 or kv.dtype != torch.uint8 or kv.shape[1:3] != (2, kv_heads) or kv.shape[4] != head_dim + 1:
+            raise KernelError(f"an 8-bit cache is uint8 [pages, 2, kv_heads, page_size, head_dim + 1]; got {kv.dtype} {tuple(kv.shape)} for "
+                              f"{kv_heads} kv heads of {head_dim}")
+        if head_dim % 16 or kv.shape[3] % 16:
+            raise KernelError(f"an 8-bit cache has head sizes and page sizes that are multiples of 16, not {head_dim} and {kv.shape[3]}")
+        return kv.shape[0], kv.shape[3]
+
+    def kv_read(self, out, kv, pages) -> None:
+        """out [n, 2, kv_heads, page_size, head_dim] (bfloat16 or float32) = the values that pages `pages` (int32 [n]) of the
+        8-bit cache `kv` stand for; exact in both types. A number that names no page gives zeros."""
+        self._check(out, kv, pages)
+        count, page_size = self._pages8(kv, kv.shape[2] if kv.dim() == 5 else 0, kv.shape[-1] - 1)
+        if pages.dim() != 1 or out.shape != (pages.shape[0], 2, kv.shape[2], page_size, kv.shape[4] - 1):
+            raise KernelError("kv_read: out must be [n, 2, kv_heads, page_size, head_dim] for int32 pages [n]")
+        self._call("hb_kv_read", self._p(out), _code(out), self._p(kv), self._i32(pages, "pages"), pages.shape[0], count, kv.shape[2],
+                   page_size, kv.shape[4] - 1)
+
     def qkv_rope(self, q_out, x, weight, positions, table, rotary_dim, q_weight, k_weight, eps, offset, kv,
                  write_index, heads, kv_heads, head_dim) -> bool:
         """The product x · weightᵀ with qk_norm_rope_kv_write folded into its epilogue, for the few rows of a decode
@@ -423,6 +470,8 @@ class CudaKernels:
         scaled, x = (x, x.y) if hasattr(x, "ss") else (None, x)      # rows that lack their norm's scale (parts.base.Scaled)
         t, k = x.shape
         wide = x.dtype == torch.bfloat16 and self._wide_takes(t, weight, scaled.ss.shape[1] if scaled else None)
+        if kv is not None and kv.dtype == torch.uint8:               # (the product's epilogue writes bfloat16 pages only)
+            return False
         if not self.fused_qkv or x.dtype != torch.bfloat16 or (t > (self.MID_ROWS if self.mid else self.SKINNY_ROWS) and not wide) or k % 8 or table is None \
                 or head_dim not in (32, 64, 128) or rotary_dim != head_dim or (q_weight is None) != (k_weight is None):
             return False
@@ -473,14 +522,20 @@ class CudaKernels:
                    ctypes.c_float(scaled.eps if scaled else 0.0), scaled.dim if scaled else 0)
         return True
 
-    def paged_attention(self, out, q, kv, block_table, rows, scale, window, sinks=None) -> None:
+    def paged_attention(self, out, q, kv, block_table, rows, scale, window, sinks=None, shared=None) -> None:
         """`sinks` (float32 [heads], or None): a weight exp(sinks[h]) in each head's softmax denominator that has
         neither key nor value. Every kernel takes them but the balanced form for one-token rows (such rows then run
-        with equal cuts, merged in a cluster or by the merge kernel)."""
+        with equal cuts, merged in a cluster or by the merge kernel). `kv` of bytes: a cache of 8-bit codes
+        (qk_norm_rope_kv_write). `shared` (engine.batch.SharedPrefix, or None): which one-token rows hold the same first
+        pages; their keys there are read once for all of them."""
         self._check(out, q, kv, block_table, rows.row_slot, rows.query_start, rows.kv_len, sinks)
         t, heads, head_dim = q.shape
         if sinks is not None and (sinks.dtype != torch.float32 or sinks.shape != (heads,)):
             raise KernelError("paged_attention: sinks must be float32 [heads]")
+        if shared is not None and (window > 0 or q.dtype != torch.bfloat16 or shared.rows != rows.n_decode):
+            raise KernelError("paged_attention: shared beginnings go with bfloat16, without a window, and are those of the step's one-token rows")
+        if kv.dtype == torch.uint8:
+            return self._attention8(out, q, kv, block_table, rows, scale, int(window), sinks, shared)
         if out.shape != q.shape or kv.dtype != q.dtype or out.dtype != q.dtype or kv.shape[4] != head_dim:
             raise KernelError("paged_attention: out and q [tokens, heads, head_dim], kv [pages, 2, kv_heads, page_size, "
                               "head_dim], one dtype")
@@ -501,7 +556,9 @@ class CudaKernels:
                     else rows.n_tokens // 64 + rows.n_rows
             return self._call("hb_attention_f32", self._p(out), self._p(q), self._p(kv), *common, rows.n_decode,
                               rows.n_rows, tiles, *sizes, self._p(sinks))
-        if rows.n_decode:
+        if shared is not None and rows.n_decode and self._shares(heads, kv_heads, head_dim, kv, q, out):
+            self._attention_rows(out, q, kv, common, rows, kv_heads, kv.shape[3], scale, 0, sinks, shared)
+        elif rows.n_decode:
             splits = self.decode_splits(rows.n_decode, heads, kv_heads, rows.max_kv)
             mode = self._decode_mode_of(rows)
             if sinks is None and splits > 1 and mode == "balanced" and rows.n_decode <= self.BALANCED_ROWS:
@@ -526,19 +583,139 @@ class CudaKernels:
                 self._call("hb_attention_decode_bf16", self._p(out), self._p(scratch), self._p(q), self._p(kv), *common,
                            rows.n_decode, *sizes, splits, self._p(sinks))
         if rows.n_rows > rows.n_decode:
-            if self.prefill_attention == "tcgen05" and head_dim == 128 and kv.shape[3] % 64 == 0:
-                tile_q, tiles = 256, self._query_tiles(rows, 256)
-                if self.prefill_tile == 128 or (self.prefill_tile is None and 4 * heads * tiles < 3 * self.sms):              # tiles of 256 queries would leave SMs idle: one group of
-                    tile_q, tiles = 128, self._query_tiles(rows, 128)   # 128 a CTA, twice the CTAs
-                self._call("hb_attention_prefill_tcgen05", self._p(out), self._p(q), self._p(kv), *common,
-                           rows.n_decode, rows.n_rows, tiles, t, *sizes, tile_q, self._p(sinks))
-            else:
-                self._call("hb_attention_prefill_bf16", self._p(out), self._p(q), self._p(kv), *common, rows.n_decode,
-                           rows.n_rows, self._query_tiles(rows, 64), *sizes, self._p(sinks))
+            self._attention_prompts(out, q, kv, common, rows, rows.n_decode, rows.n_rows, sizes, sinks)
+
+    def _attention_prompts(self, out, q, kv, common, rows, first: int, last: int, sizes, sinks) -> None:
+        """Rows `first` .. `last` - 1, which bring several tokens each, over bfloat16 pages. `common`, `sizes`: the arguments that
+        the kernels share."""
+        heads, head_dim = sizes[0], sizes[2]
+        if self.prefill_attention == "tcgen05" and head_dim == 128 and kv.shape[3] % 64 == 0:
+            tile_q, tiles = 256, self._query_tiles(rows, 256, first, last)
+            if self.prefill_tile == 128 or (self.prefill_tile is None and 4 * heads * tiles < 3 * self.sms):              # tiles of 256 queries would leave SMs idle: one group of
+                tile_q, tiles = 128, self._query_tiles(rows, 128, first, last)   # 128 a CTA, twice the CTAs
+            self._call("hb_attention_prefill_tcgen05", self._p(out), self._p(q), self._p(kv), *common,
+                       first, last, tiles, q.shape[0], *sizes, tile_q, self._p(sinks))
+        else:
+            self._call("hb_attention_prefill_bf16", self._p(out), self._p(q), self._p(kv), *common, first,
+                       last, self._query_tiles(rows, 64, first, last), *sizes, self._p(sinks))
+
+    # ---- 8-bit pages, shared beginnings
+    READ_BACK_TOKENS = 65536                  # tokens of scratch that rows of several tokens read an 8-bit cache back into at once
+
+    def _attention8(self, out, q, kv, block_table, rows, scale, window: int, sinks, shared) -> None:
+        t, heads, head_dim = q.shape
+        kv_heads = kv.shape[2] if kv.dim() == 5 else 0
+        pages, page_size = self._pages8(kv, kv_heads, head_dim)
+        if q.dtype != torch.bfloat16 or out.dtype != q.dtype or out.shape != q.shape or heads % kv_heads or head_dim > 256:
+            raise KernelError("paged_attention: an 8-bit cache takes bfloat16 q and out [tokens, heads, head_dim] with head sizes up to 256")
+        common = (self._i32(block_table, "block_table"), block_table.shape[1], self._i32(rows.row_slot, "row_slot"),
+                  self._i32(rows.query_start, "query_start"), self._i32(rows.kv_len, "kv_len"))
+        if rows.n_decode:
+            if shared is not None and not self._shares(heads, kv_heads, head_dim, kv, q, out):
+                shared = None
+            self._attention_rows(out, q, kv, common, rows, kv_heads, page_size, scale, window, sinks, shared)
+        for first, last, stride in self._read_back_portions(rows, page_size, block_table.shape[1]):
+            count = last - first
+            back = torch.empty((count * stride, 2, kv_heads, page_size, head_dim), dtype=torch.bfloat16, device=self.device)
+            tables = torch.empty(count * stride + last, dtype=torch.int32, device=self.device)
+            table, slots = tables[:count * stride], tables[count * stride:]
+            self._call("hb_kv_read_rows", self._p(back), self._p(table), self._p(slots), self._p(kv), *common, first, last, stride, pages,
+                       kv_heads, page_size, head_dim, window)
+            self._attention_prompts(out, q, back, (self._p(table), stride, self._p(slots), *common[3:]), rows, first, last,
+                                    (heads, kv_heads, head_dim, count * stride, page_size, ctypes.c_float(scale), window), sinks)
+
+    def _read_back_portions(self, rows, page_size: int, most: int):
+        """The rows of several tokens in runs (first, last, pages a row) whose keys are read back at once: as many rows as
+        READ_BACK_TOKENS of scratch hold at the length of the longest, one at least. Where the rows' lengths are not known on the
+        host, or are not those that the launch will meet (a captured step), all at once at the longest there may be."""
+        if rows.n_rows <= rows.n_decode:
+            return
+        pages_of = lambda tokens: min(most, max(1, -(-int(tokens) // page_size)))             # noqa: E731
+        if rows.host_kv_len is None or "any cut" in rows.plan:
+            yield rows.n_decode, rows.n_rows, pages_of(rows.max_kv)
+            return
+        first, stride = rows.n_decode, 0
+        for b in range(rows.n_decode, rows.n_rows):
+            mine = max(stride, pages_of(rows.host_kv_len[b]))
+            if b > first and (b + 1 - first) * mine * page_size > self.READ_BACK_TOKENS:
+                yield first, b, stride
+                first, mine = b, pages_of(rows.host_kv_len[b])
+            stride = mine
+        yield first, rows.n_rows, stride
+
+    def read_back_scratch(self, tokens: int, rows: int, longest: int, kv_heads: int, head_dim: int, page_size: int) -> int:
+        """Bytes of scratch that rows of several tokens take at most for reading an 8-bit cache back (`rows` such rows of up to
+        `longest` tokens in a step of `tokens`)."""
+        rows = min(rows, tokens // 2)
+        if rows < 1:
+            return 0
+        whole = -(-longest // page_size) * page_size
+        return max(whole, min(rows * whole, self.READ_BACK_TOKENS)) * 2 * kv_heads * head_dim * 2
+
+    def _shares(self, heads: int, kv_heads: int, head_dim: int, kv, q, out) -> bool:
+        """Whether the kernels for shared beginnings take these sizes (other sizes attend row by row)."""
+        return head_dim % 16 == 0 and head_dim <= 256 and heads // kv_heads <= self._prefix_rows() \
+            and not (kv.data_ptr() | q.data_ptr()) % 16 and out.data_ptr() % 8 == 0
+
+    def _prefix_rows(self) -> int:
+        key = ("prefix rows",)
+        if key not in self._splits:
+            self._splits[key] = int(self.lib.hb_attention_prefix_rows())
+        return self._splits[key]
+
+    def _attention_rows(self, out, q, kv, common, rows, kv_heads: int, page_size: int, scale, window: int, sinks, shared) -> None:
+        """The step's one-token rows over 8-bit pages, or over either kind with the beginnings that some of them share."""
+        heads, head_dim, n, kv8 = q.shape[1], q.shape[2], rows.n_decode, int(kv.dtype == torch.uint8)
+        part = (None, None, None, None, 0)
+        longest = rows.max_kv
+        if shared is not None:
+            tile, ctas = self._prefix_rows(), self.sms * self.PREFIX_CTAS
+            units = self._prefix_units(n, heads, kv_heads)
+            floats = units * tile * (head_dim + 2)
+            scratch = torch.empty(self.shared_scratch(n, heads, kv_heads, head_dim), dtype=torch.float32, device=self.device)
+            at = scratch.data_ptr()
+            part_o, part_ml, part_at = (ctypes.c_void_p(at + 4 * i) for i in (0, units * tile * head_dim, floats))
+            self._call("hb_attention_prefix", part_o, part_ml, part_at, self._p(q), self._p(kv), kv8, *common[:4], self._p(shared.members),
+                       self._p(shared.groups), shared.groups.shape[0] // 3, heads, kv_heads, head_dim, kv.shape[0], page_size,
+                       ctypes.c_float(scale), ctas)
+            part = (self._p(shared.skip), part_o, part_ml, part_at, tile)
+            longest = shared.longest_own
+        if window > 0:
+            longest = min(longest, window)
+        splits = self._row_splits(kv8, n, heads, kv_heads, head_dim, longest)
+        self._call("hb_attention_rows", self._p(out), self._p(q), self._p(kv), kv8, *common, n, heads, kv_heads, head_dim, kv.shape[0],
+                   page_size, ctypes.c_float(scale), window, splits, self._p(sinks), *part)
+
+    PREFIX_CTAS = 2                           # CTAs an SM of the kernel for shared keys
+
+    def _prefix_units(self, rows: int, heads: int, kv_heads: int) -> int:
+        """Partial results that `rows` one-token rows may leave at most for what they share, whatever their groups are: a tile for
+        every so many rows that fill one, and one more for each group."""
+        per_tile = max(1, self._prefix_rows() // (heads // kv_heads))
+        return max(self.sms * self.PREFIX_CTAS, kv_heads * (rows // per_tile + rows // 2))
+
+    def shared_scratch(self, rows: int, heads: int, kv_heads: int, head_dim: int) -> int:
+        """32-bit words of scratch for what `rows` one-token rows share."""
+        return self._prefix_units(rows, heads, kv_heads) * self._prefix_rows() * (head_dim + 2) + 4 * rows
+
+    def _row_splits(self, kv8: int, rows: int, heads: int, kv_heads: int, head_dim: int, longest: int) -> int:
+        """Into how many CTAs (a cluster) the keys of a one-token row are cut: the number with the least waves x (64-key tiles a
+        CTA walks + its start)."""
+        key = ("rows", kv8, rows, heads, kv_heads, head_dim, -(-longest // 64))
+        if key not in self._splits:
+            group, tiles = heads // kv_heads, max(1, -(-longest // 64))
+            pairs = rows * kv_heads * -(-group // 16)
+            best = (math.inf, 1)
+            for s in range(1, min(16, tiles) + 1):
+                room = int(self.lib.hb_attention_rows_capacity(kv8, head_dim, group, s)) * (self.sms if s == 1 else 1)
+                if room > 0:
+                    best = min(best, (-(-pairs // room) * (-(-tiles // s) + 2 + (s > 1)), s))
+            self._splits[key] = best[1]
+        return self._splits[key]
 
     KV_BUCKET_MIN = 512                       # the smallest number of keys a captured decode launch is planned for
 
-    def attention_capture_plan(self, rows, max_model_len: int):
+    def attention_capture_plan(self, rows, max_model_len: int, shared=None):
         """For a step that runs as a CUDA graph: what of the attention's launch plan a captured launch keeps, as a
         hashable key, pinned on `rows` so that every layer's launch is planned with it. The keys of a row are cut for
         a power-of-two bucket of the longest row (a graph of that bucket serves every batch whose longest row fits
@@ -558,7 +735,13 @@ class CudaKernels:
         portions, tokens = rows.n_rows - rows.n_decode, rows.n_tokens - rows.n_decode
         for size in (64, 128, 256):
             rows.plan[size] = tokens // size + portions
-        return mode, bucket
+        if shared is None:
+            return mode, bucket
+        own = 64                                                     # the rows' own keys behind shared ones: a bucket of their own
+        while own < shared.longest_own:
+            own *= 2
+        shared.longest_own = min(own, bucket)
+        return mode, bucket, shared.longest_own
 
     # Every layer of a step asks the same questions about the step's rows: the answers are kept on the rows.
     def _decode_mode_of(self, rows) -> str:
@@ -569,13 +752,15 @@ class CudaKernels:
         return plan["mode"]
 
     @staticmethod
-    def _query_tiles(rows, size: int) -> int:
-        """Tiles of `size` queries over the rows that bring several tokens."""
+    def _query_tiles(rows, size: int, first: int | None = None, last: int | None = None) -> int:
+        """Tiles of `size` queries over the rows that bring several tokens (or over rows `first` .. `last` - 1 of them)."""
         plan = rows.plan
-        if size not in plan:
+        key = size if first is None or (first, last) == (rows.n_decode, rows.n_rows) else (size, first, last)
+        if key not in plan:
             qs = rows.host_query_start
-            plan[size] = sum((int(qs[b + 1]) - int(qs[b]) + size - 1) // size for b in range(rows.n_decode, rows.n_rows))
-        return plan[size]
+            a, b = (rows.n_decode, rows.n_rows) if key == size else (first, last)
+            plan[key] = sum((int(qs[r + 1]) - int(qs[r]) + size - 1) // size for r in range(a, b))
+        return plan[key]
 
     BALANCED_ROWS = 256                       # rows the balanced decode kernel takes (its prefix array)
 

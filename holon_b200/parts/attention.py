@@ -38,6 +38,9 @@ class GQA(Part):
             raise ValueError(f"gqa: {heads} heads are no multiple of {kv_heads} kv heads")
         if qk_norm is not None and unit_norm_eps is not None:
             raise ValueError("gqa: give qk_norm or unit_norm_eps, not both")
+        self.fp8 = ctx.cache_dtype == "fp8"
+        if self.fp8 and (head_dim % 16 or head_dim > 256):
+            raise ValueError(f"gqa: an fp8 cache takes head sizes that are multiples of 16 up to 256, not {head_dim}")
         self.ctx, self.heads, self.kv_heads, self.head_dim, self.window = ctx, heads, kv_heads, head_dim, int(window)
         self.scale = 1.0 / head_dim ** 0.5 if scale is None else float(scale)
         self.unit_norm_eps, self.values_are_keys = unit_norm_eps, bool(values_are_keys)
@@ -84,10 +87,22 @@ class GQA(Part):
     takes_scaled = True                      # x may be base.Scaled: both first products apply the row scale
 
     def cache(self) -> PagedKV:
-        return PagedKV(self.kv_heads, self.head_dim, self.window)
+        return PagedKV(self.kv_heads, self.head_dim, self.window, self.fp8)
 
     def slot_states(self):
         return ()
+
+    def context_scratch(self, tokens: int, rows: int, longest: int) -> int:
+        scratch = getattr(self.ctx.kernels, "read_back_scratch", None) if self.fp8 else None
+        return scratch(tokens, rows, longest, self.kv_heads, self.head_dim, self.ctx.page_size) if scratch is not None else 0
+
+    def graph_scratch(self, rows: int, portions: int, longest: int, page_size: int) -> int:
+        k, bytes_ = self.ctx.kernels, 0
+        if self.fp8:                                                 # (a captured step reads all its portions back at once)
+            bytes_ += portions * -(-longest // page_size) * page_size * 4 * self.kv_heads * self.head_dim
+        if self.ctx.shared_prefix and hasattr(k, "shared_scratch"):
+            bytes_ += 4 * k.shared_scratch(rows, self.heads, self.kv_heads, self.head_dim)
+        return bytes_
 
     @property
     def plan_group(self):
@@ -97,7 +112,10 @@ class GQA(Part):
     def capture_plan(self, step, max_model_len: int):
         """What the attention kernels pin for a step that is captured as a CUDA graph (see base.Part)."""
         plan = getattr(self.ctx.kernels, "attention_capture_plan", None)
-        return plan(step.rows, max_model_len) if plan is not None else None
+        shared = next((g.shared for g in step.groups if g.shared is not None and g.decl == self.cache()), None)
+        if shared is None:
+            return plan(step.rows, max_model_len) if plan is not None else None
+        return plan(step.rows, max_model_len, shared) if plan is not None else "shared"
 
     def forward(self, x: torch.Tensor, step, cache) -> torch.Tensor:
         t, k = x.shape[0], self.ctx.kernels
@@ -115,10 +133,10 @@ class GQA(Part):
         elif fused is None or not fused(q, x, self.qkv.weight.tensor, *after):
             k.qk_norm_rope_kv_write(q, self.qkv.forward(x), *after)
         o = self.ctx.empty(t, self.heads, self.head_dim)
-        if self.sink is not None:
-            k.paged_attention(o, q, cache.kv, cache.group.block_table, step.rows, self.scale, self.window, self.sink.tensor)
-        else:
-            k.paged_attention(o, q, cache.kv, cache.group.block_table, step.rows, self.scale, self.window)
+        more = {} if self.sink is None else {"sinks": self.sink.tensor}
+        if cache.group.shared is not None:
+            more["shared"] = cache.group.shared
+        k.paged_attention(o, q, cache.kv, cache.group.block_table, step.rows, self.scale, self.window, **more)
         return self.o_proj.forward(o.view(t, self.heads * self.head_dim), link=take_link(step))
 
 

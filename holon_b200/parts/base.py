@@ -77,6 +77,11 @@ class Part:
         the cache (a request holds up to `longest` tokens). What the new tokens alone ask for is measured; this is added to it."""
         return max((child.context_scratch(tokens, rows, longest) for child in self._children.values()), default=0)
 
+    def graph_scratch(self, rows: int, portions: int, longest: int, page_size: int) -> int:
+        """The same for a step that is replayed from a graph: `rows` one-token rows beside `portions` rows of several tokens. Such
+        a step takes what the longest requests ask for, whatever its own rows hold."""
+        return max((child.graph_scratch(rows, portions, longest, page_size) for child in self._children.values()), default=0)
+
     def finalize(self) -> None:
         """Called once after every parameter holds its tensor. What needs the tensors, the device or the kernel table
         (derived tensors, a library of the part's own: `ctx.kernels.extension`) is done here, not in the constructor:
@@ -90,15 +95,22 @@ class Part:
 @dataclasses.dataclass(frozen=True)
 class PagedKV:
     """Keys and values of every token, in pages; `window` W > 0: only the last W positions are ever read again, so
-    pages that lie wholly before them are given back."""
+    pages that lie wholly before them are given back. `fp8`: pages hold 8-bit codes and a scale byte per token, kv head and
+    part instead of the engine's dtype."""
 
     kv_heads: int
     head_dim: int
     window: int = 0
+    fp8: bool = False
+
+    @property
+    def dtype(self) -> torch.dtype | None:
+        """What its pages hold (None: the engine's dtype)."""
+        return torch.uint8 if self.fp8 else None
 
     def page_shape(self, page_size: int) -> tuple[int, ...]:
-        """One page of one cache entry: keys, then values, per kv head."""
-        return (2, self.kv_heads, page_size, self.head_dim)
+        """One page of one cache entry: keys, then values, per kv head (codes: page_size rows, then page_size scale bytes)."""
+        return (2, self.kv_heads, page_size, self.head_dim + self.fp8)
 
 
 @dataclasses.dataclass(frozen=True)
@@ -170,9 +182,12 @@ class BuildContext:
 
     recordable = True
 
-    def __init__(self, device, dtype: torch.dtype, kernels, max_positions: int, max_step_tokens: int = 0) -> None:
+    def __init__(self, device, dtype: torch.dtype, kernels, max_positions: int, max_step_tokens: int = 0,
+                 cache_dtype: str = "auto", shared_prefix: bool = False, page_size: int = 0) -> None:
+        """`cache_dtype`, `shared_prefix`: as in `EngineConfig`; `page_size`: of the cache, where it is known."""
         self.device, self.dtype, self.kernels = torch.device(device), dtype, kernels
         self.max_positions, self.max_step_tokens = max_positions, max_step_tokens
+        self.cache_dtype, self.shared_prefix, self.page_size = cache_dtype, shared_prefix, page_size
 
     def part(self, ref: PartRef, **site: Any) -> Part:
         from . import _builtin  # noqa: F401  (registers the built-in parts)

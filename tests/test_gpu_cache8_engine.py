@@ -1,0 +1,144 @@
+"""The step function and the engine with an 8-bit cache and with shared beginnings: against the plain kernel table, recorded and
+replayed steps, mixed steps, several samples of one prompt, the memory account."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import cache8_tools as c8
+from helpers import random_prompt
+from holon_b200.engine import Engine, EngineConfig, SamplingParams, StepEntry, build
+from holon_b200.weights import RandomSource
+
+pytestmark = pytest.mark.gpu
+SMALL = dict(architectures=["Qwen3ForCausalLM"], num_hidden_layers=2, hidden_size=128, num_attention_heads=6, num_key_value_heads=2, head_dim=48,
+             intermediate_size=192, vocab_size=331, rope_theta=10000.0, rms_norm_eps=1e-6, tie_word_embeddings=False)
+WIDE = dict(SMALL, hidden_size=256, num_attention_heads=8, num_key_value_heads=2, head_dim=128)
+CONFIGS = {"48": SMALL, "128": WIDE}
+# Codes from inputs that differ by bfloat16's rounding: one number in 32 falls on the other side of a border and moves by a step of
+# about 2^-3.5, 1.7% of a row's norm; two layers of it beside the 2e-2 that bfloat16 engines are held to elsewhere.
+NEAR = 5e-2
+
+
+def made(config, device="cuda:0", **kw):
+    args = dict(dtype="bfloat16", page_size=16, max_seqs=8, max_model_len=1024, max_step_tokens=1024, pages=200)
+    args.update(kw)
+    kernels = c8.RefKernels8() if device == "cpu" else None
+    with torch.inference_mode():
+        return build(RandomSource(config, seed=5, device=device, dtype=torch.bfloat16), device=device, kernels=kernels, **args)
+
+
+def off(a, b):
+    return (torch.linalg.norm(a.float().cpu() - b.float().cpu()) / torch.linalg.norm(b.float().cpu())).item()
+
+
+def trace(built, lengths, steps, seed=1, shared=0):
+    """Prompts of `lengths` whose first `shared` tokens are the same, then `steps` known tokens each; all logits."""
+    g = torch.Generator().manual_seed(seed)
+    vocab = built.model.spec.vocab
+    same = torch.randint(0, vocab, (shared,), generator=g).tolist()
+    ids = [(same + torch.randint(0, vocab, (n + steps,), generator=g).tolist())[:n + steps] for n in lengths]
+    out, cache, slots, at = [], built.cache, [], []
+    with torch.inference_mode():
+        for i, n in enumerate(lengths):                               # one after the other: later ones start on the first one's pages
+            slot = cache.admit(ids[i][:n])
+            start = int(cache.computed[slot])
+            assert cache.reserve(slot, n)
+            out.append(built.runner.step([StepEntry(slot, ids[i][start:n], start, [n - start - 1])]))
+            cache.publish(slot, ids[i][:n])
+            slots.append(slot)
+        for s in range(steps):
+            entries = []
+            for slot, tokens, n in zip(slots, ids, lengths):
+                assert cache.reserve(slot, n + s + 1)
+                entries.append(StepEntry(slot, tokens[n + s:n + s + 1], n + s, [0]))
+            out.append(built.runner.step(entries))
+        for slot in slots:
+            cache.release(slot)
+    return [x.clone() for x in out]
+
+
+@pytest.mark.parametrize("name", CONFIGS)
+@pytest.mark.parametrize("page", [16, 64])
+def test_steps_against_the_plain_table(name, page):
+    config = CONFIGS[name]
+    source = RandomSource(config, seed=5, device="cpu", dtype=torch.bfloat16)
+    with torch.inference_mode():
+        gpu = build(source, dtype="bfloat16", device="cuda:0", page_size=page, max_seqs=8, max_model_len=512, max_step_tokens=512, pages=100,
+                    cache_dtype="fp8", cuda_graphs=False)
+        cpu = build(source, dtype="bfloat16", device="cpu", kernels=c8.RefKernels8(), page_size=page, max_seqs=8, max_model_len=512,
+                    max_step_tokens=512, pages=100, cache_dtype="fp8")
+    assert gpu.cache.groups[0].kv.dtype == torch.uint8
+    for a, b in zip(trace(gpu, [150, 33, 1], 5), trace(cpu, [150, 33, 1], 5)):
+        assert off(a, b) <= NEAR
+
+
+@pytest.mark.parametrize("fp8", [True, False])
+@pytest.mark.parametrize("name", CONFIGS)
+def test_shared_beginnings(name, fp8):
+    """Rows on one prompt's pages: the same logits with the keys read once as row by row, in steps that run kernel by kernel and in
+    recorded ones; and the recordings of both kinds live side by side."""
+    kw = dict(cache_dtype="fp8" if fp8 else "auto", prefix_cache=True)
+    plain, once, graphs = made(CONFIGS[name], cuda_graphs=False, **kw), made(CONFIGS[name], cuda_graphs=False, shared_prefix=True, **kw), \
+        made(CONFIGS[name], shared_prefix=True, **kw)
+    seen = []
+    context = once.runner.context
+    once.runner.context = lambda *a, **k: (step := context(*a, **k), seen.append(step.groups[0].shared is not None))[0]
+    near = NEAR if fp8 else 2e-2
+    for lengths, shared in (([300, 290, 310, 305], 288), ([300, 40, 500], 0), ([300, 290, 310, 305], 288), ([400, 390, 310, 305, 60], 300)):
+        want = trace(plain, lengths, 6, seed=shared + 1, shared=shared)
+        seen.clear()
+        for a, b in zip(trace(once, lengths, 6, seed=shared + 1, shared=shared), want):
+            assert off(a, b) <= near
+        assert any(seen) == bool(shared)
+        for a, b in zip(trace(graphs, lengths, 6, seed=shared + 1, shared=shared), want):
+            assert off(a, b) <= near
+    assert sum(r is not None for r in graphs.runner._recorded.values()) >= 3
+    for b in (plain, once, graphs):
+        b.cache.check()
+
+
+@pytest.mark.parametrize("graphs", [True, False])
+@pytest.mark.parametrize("fp8,shared", [(True, False), (True, True), (False, True)])
+def test_generation(fp8, shared, graphs):
+    """Mixed steps, graphs, several samples of a prompt beside other requests: greedy samples of one prompt are the same tokens, whatever
+    they run beside, and the engine ends with everything given back."""
+    engine = Engine(EngineConfig(model="", page_size=16, max_seqs=9, max_model_len=512, max_step_tokens=256, chunk_with_decode=32,
+                                 state_memory=16 << 20, cuda_graphs=graphs, cache_dtype="fp8" if fp8 else "auto", shared_prefix=shared),
+                    source=RandomSource(WIDE, seed=5, device="cuda:0", dtype=torch.bfloat16))
+    greedy = SamplingParams(temperature=0.0, max_tokens=12, n=5, ignore_eos=True)
+    with torch.inference_mode():
+        engine.add(random_prompt(331, 200, 7), greedy, rid="a")
+        engine.add(random_prompt(331, 90, 8), SamplingParams(temperature=0.8, seed=3, max_tokens=20, n=2, ignore_eos=True), rid="b")
+        got, late = {}, False
+        while engine.has_work():
+            for d in engine.step():
+                got.setdefault((d.rid, d.index), []).extend(d.token_ids)
+            if not late and len(got.get(("a", 0), [])) > 3:
+                late = True
+                engine.add(random_prompt(331, 160, 9), SamplingParams(temperature=0.0, max_tokens=8, ignore_eos=True), rid="c")
+    assert sorted(map(len, got.values())) == [8] + [12] * 5 + [20] * 2
+    assert len({tuple(got["a", i]) for i in range(1, 5)}) == 1                          # (0 starts a step before the others)
+    stats = engine.stats()
+    assert (stats["graph_steps"] > 0) == graphs and stats["prefix_hit_tokens"] > 0
+    engine.built.cache.check()
+    engine.close()
+    assert not engine.built.cache.live
+
+
+def test_memory_of_the_largest_steps():
+    """With pools sized by what is left, the account holds the scratch that portions are read back into, and an 8-bit cache holds about
+    twice the tokens in the same bytes."""
+    def engine(**kw):
+        return Engine(EngineConfig(model="", page_size=64, max_seqs=8, max_model_len=4096, max_step_tokens=512, chunk_with_decode=64, **kw),
+                      source=RandomSource(WIDE, seed=5, device="cuda:0", dtype=torch.bfloat16))
+    fixed = {kw: engine(state_memory=64 << 20, cache_dtype=kw).stats()["free_tokens"] for kw in ("auto", "fp8")}
+    assert 1.9 < fixed["fp8"] / fixed["auto"] < 2.0
+    e = engine(memory_fraction=0.05, cache_dtype="fp8", shared_prefix=True)
+    k, m = e.built.ctx.kernels, e.built.memory
+    assert m.activations >= k.read_back_scratch(512, 8, 4096, 2, 128, 64) > 0
+    assert m.graphs >= 2 * 4096 * 4 * 2 * 128 + 4 * k.shared_scratch(8, 8, 2, 128)
+    with torch.inference_mode():
+        out = e.generate([random_prompt(331, 3000, i) for i in range(3)], SamplingParams(temperature=0.0, max_tokens=4, ignore_eos=True))
+    assert all(len(t) == 4 for t in out)
+    e.close()
