@@ -1,32 +1,49 @@
 // Attention of rows that bring one token each, over pages of 8-bit codes, and over the keys that rows which share their
-// first pages hold behind those (pages of either kind). mma.sync m16n8k16, 32-bit accumulation and softmax.
+// first pages hold behind those (pages of either kind).
 //
-// A CTA owns (row, kv head, split of the row's keys); the kv head's group of query heads is the 16-row M tile, so keys and
-// values are read once per group. Its four warps take 16 keys each of every 64-key tile, keep their own running softmax and
-// are merged in shared memory; the splits of a (row, kv head) are one thread-block cluster and are merged through
-// distributed shared memory, in the order of the splits. With `skip` (tokens a row shares with others) the walk starts
-// behind them, and the partial results that attention_prefix.cu left for the shared keys are added in the same merge.
+// A CTA owns (row, kv head, split of the row's keys, up to eight of the kv head's query heads). A fifth warp brings tiles of keys by
+// TMA; four warps take 32 keys each of every tile, keep their own running softmax and are merged in shared memory; the splits of a
+// (row, kv head) are one thread-block cluster and are merged through distributed shared memory, in the order of the splits. With
+// `skip` (tokens a row shares with others) the walk starts behind them, and the partial results that attention_prefix.cu left
+// for the shared keys are added in the same merge.
 //
-// 8-bit pages: codes go to the matrix instructions as halves, which hold every code exactly. With k_j = 2^a_j K_j and
+// Both products have the heads as their eight columns: S^T = K Q^T (16 keys a product) and O^T = V^T P^T (16 numbers of the head), so
+// that eight heads fill the shape and a lane's maxima and sums belong to the columns of its outputs; the weights pass from one
+// product's result to the other's operand by a transposition of 8 x 8 blocks.
+// 8-bit pages: codes become halves, which hold every code exactly (mma.sync on codes themselves is the same conversion and more
+// instructions on this GPU: 8 to 12 where the two conversions and the product are 5, counted). With k_j = 2^a_j K_j and
 // v_j = 2^b_j V_j (K, V codes) and the head's query scaled into the halves' range by a power of two 2^-c,
-//     u_j = (q 2^-c · K_j) 2^(a_j + c) scale log2(e) + b_j,   w_j = 2^(u_j - M),   O = sum w_j V_j,   l = sum w_j 2^-b_j
+//     u_j = (q 2^-c . K_j) 2^(a_j + c) scale log2(e) + b_j,   w_j = 2^(u_j - M),   O = sum w_j V_j,   l = sum w_j 2^-b_j
 // with M the running maximum of u, not of the scores: the weights that meet the codes stay at most 2^14 whatever the values' scales
 // are (14 is taken off M so that small weights are no subnormal halves), and l sums the softmax's own weights in the same units.
-// ldmatrix moves pairs of codes as it moves bfloat16: a lane gets codes 4 c .. 4 c + 3 of a key where the fragment wants
-// columns 2 c, 2 c + 1, 2 c + 8, 2 c + 9, so queries are laid out in that order; of values it gets two neighbouring codes of two keys,
-// one byte permutation pairs the keys, and the even and the odd columns are two products.
+// ldmatrix moves pairs of codes as it moves bfloat16: of a key a lane gets codes 4 c .. 4 c + 3 where the fragment wants columns 2 c,
+// 2 c + 1, 2 c + 8, 2 c + 9, so queries are laid out in that order; of values it gets two neighbouring codes of two keys, one byte
+// permutation pairs the keys, and the even numbers of the head are the product's rows 0 - 7, the odd ones its rows 8 - 15.
 #include <cuda_fp16.h>
 
 #include "attention_mma.cuh"
 #include "cache8.cuh"
+#include "tcgen05.cuh"
 
-#define AR_THREADS 128
+#define AR_WARPS 4                    // that compute; one more loads
+#define AR_THREADS (32 * AR_WARPS + 32)
+#define AR_HEADS 8
 #define AR_BIAS 14.f
+#ifndef AR_NK
+#define AR_NK(D_PAD, KV8) ((KV8) || (D_PAD) <= 64 ? 2 : 1)
+#define AR_STAGES(BYTES) ((BYTES) <= 16384 ? 4 : (BYTES) <= 32768 ? 3 : 2)
+#endif
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// An 8 x 8 block of 16-bit numbers, transposed within the warp.
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(r) : "r"(x));
+    return r;
 }
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
     __half2 v = __floats2half2_rn(lo, hi);
@@ -36,6 +53,11 @@ __device__ __forceinline__ void st_cluster_f32(const float* local, uint32_t rank
     uint32_t remote;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(remote) : "r"(smem_u32(local)), "r"(rank));
     asm volatile("st.shared::cluster.f32 [%0], %1;\n" ::"r"(remote), "f"(v) : "memory");
+}
+// An untiled copy of a few bytes (16-byte boundaries and size), counted on `bar`.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 
 struct RowsArgs {
@@ -47,305 +69,265 @@ struct RowsArgs {
     const int32_t* skip;           // tokens a row shares (their partial results are in part_*), or null
     const float *part_o, *part_ml; // [units, part_rows, head_dim] and [units, part_rows, 2]
     const int4* part_at;           // per row: the first unit of kv head 0, units a kv head, the row's place among its tile's rows
-    int part_rows, table_stride, heads, kv_heads, head_dim, pages, page_size, window, splits;
+    int part_rows, table_stride, heads, kv_heads, head_dim, pages, page_size, box, window, splits;
     float scale_log2;
 };
 
-// Byte offset of (row, 16-byte chunk) in a tile whose rows are ROW bytes: eight rows at one chunk lie in eight bank groups.
-template <int ROW> __device__ __forceinline__ uint32_t row_off(int row, int chunk) {
-    return (uint32_t)(row * ROW + ((ROW == 64 ? chunk ^ ((row >> 1) & 3) : chunk ^ (row & 7)) << 4));
-}
-// Bytes of a tile's row: bfloat16 heads padded to 64, 128 or 256, codes to 64, 128 or 256.
+// A stage's tile of KEYS keys: keys, then values, each as column blocks [KEYS rows][SUB bytes] that TMA swizzles over SUB bytes.
 template <int D_PAD, bool KV8> struct Tile {
-    static constexpr int ROW = KV8 ? D_PAD : 2 * D_PAD;
-    static constexpr int PART = TILE_N * ROW;                    // keys or values
-    static constexpr int STAGE = 2 * PART + (KV8 ? 128 : 0);     // and 64 + 64 scale bytes
-    static constexpr int Q = D_PAD > 128 ? D_PAD / 16 * 512 : 0; // fragments of the queries, where they do not stay in registers
-    static constexpr int SUMS = (4 * 16 * D_PAD + 4 * 16 * 2 + 16 * D_PAD + 16 * 2) * 4;
-    static constexpr int BYTES(int stages) { return Q + (stages * STAGE > SUMS ? stages * STAGE : SUMS); }
+    static constexpr int ROW = KV8 ? D_PAD : 2 * D_PAD;              // bytes of a key
+    static constexpr int NK = AR_NK(D_PAD, KV8), KEYS = 16 * AR_WARPS * NK;   // a warp takes NK times 16 keys of a tile
+    static constexpr int SUB = ROW < 128 ? ROW : 128, NSUB = ROW / SUB, BLOCK = KEYS * SUB;
+    static constexpr int PART = NSUB * BLOCK, STAGE = 2 * PART;
+    static constexpr int STAGES = AR_STAGES(STAGE);
+    static constexpr int SUMS = (AR_WARPS * AR_HEADS * (D_PAD + 2)) * 4;      // what the warps leave, over the tiles
+    static constexpr int BODY = STAGES * STAGE > SUMS ? STAGES * STAGE : SUMS;
+    static constexpr int BARS = BODY + STAGES * 2 * KEYS;            // behind the tiles: a stage's scale bytes, then the barriers
+    static constexpr int RECV = BARS + 16 * STAGES;                  // then what the other CTAs of a cluster send
 };
-
-// Keys and values [tile * 64, tile * 64 + 64) of a kv head; keys outside [lo, hi) become zeros. `page`: the tile's page where
-// a tile lies in one (page_size a multiple of 64), else every row looks its own up.
-template <int D_PAD, bool KV8>
-__device__ __forceinline__ void load_tile(uint32_t dst, const RowsArgs& a, const int32_t* table, int hk, int tile, int lo, int hi, bool in_page,
-                                          int page) {
+// Byte offset of (row, 16-byte chunk) in a part of a tile: eight rows at one chunk lie in eight bank groups.
+template <int D_PAD, bool KV8> __device__ __forceinline__ uint32_t tile_at(int row, int chunk) {
     using T = Tile<D_PAD, KV8>;
-    constexpr int CPR = T::ROW / 16, STEP = AR_THREADS / CPR;
-    const int bytes = KV8 ? a.head_dim : 2 * a.head_dim;            // of a row in memory
-    const size_t block = (size_t)a.page_size * (KV8 ? a.head_dim + 1 : 2 * a.head_dim), part = (size_t)a.kv_heads * block;
-    const int ch = threadIdx.x % CPR, r0 = threadIdx.x / CPR, j0 = tile * TILE_N;
-    if (KV8 && threadIdx.x < 8) {                                   // the scales: 16 keys a thread (pages are multiples of 16 keys)
-        const int j = j0 + (threadIdx.x & 3) * 16, v = threadIdx.x >> 2;
-        bool valid = j + 16 > lo && j < hi;
-        const int pi = j / a.page_size;
-        const int p = !valid ? 0 : in_page ? page : table[pi];
-        valid = valid && p >= 0 && p < a.pages;
-        const size_t off = ((size_t)(valid ? p : 0) * 2 + v) * part + (size_t)hk * block + (size_t)a.page_size * a.head_dim + (valid ? j - pi * a.page_size : 0);
-        cp_async16(dst + 2 * T::PART + v * 64 + (threadIdx.x & 3) * 16, a.kv + off, valid);
-    }
-    if (ch * 16 >= bytes) return;                                   // columns past head_dim are never read
-    if (in_page) {
-        const bool page_ok = page >= 0 && page < a.pages;
-        const unsigned char* base = a.kv + (size_t)(page_ok ? page : 0) * 2 * part + (size_t)hk * block + ch * 16
-                                    + (size_t)(j0 % a.page_size) * bytes;
-#pragma unroll
-        for (int r = r0; r < TILE_N; r += STEP) {
-            const bool valid = page_ok && j0 + r >= lo && j0 + r < hi;
-            const unsigned char* src = base + (valid ? (size_t)r * bytes : 0);
-            const uint32_t d = dst + row_off<T::ROW>(r, ch);
-            cp_async16(d, src, valid);
-            cp_async16(d + T::PART, src + part, valid);
-        }
-        return;
-    }
-#pragma unroll
-    for (int r = r0; r < TILE_N; r += STEP) {
-        const int j = j0 + r;
-        bool valid = j >= lo && j < hi;
-        size_t off = 0;
-        if (valid) {
-            const int pi = j / a.page_size, p = table[pi];
-            valid = p >= 0 && p < a.pages;
-            off = (size_t)(valid ? p : 0) * 2 * part + (size_t)hk * block + (size_t)(j - pi * a.page_size) * bytes + ch * 16;
-        }
-        const uint32_t d = dst + row_off<T::ROW>(r, ch);
-        cp_async16(d, a.kv + off, valid);
-        cp_async16(d + T::PART, a.kv + off + part, valid);
-    }
+    if (T::SUB == 64) return (uint32_t)(row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4));
+    return (uint32_t)((chunk >> 3) * T::BLOCK + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
 }
 
-// The A fragments of up to 16 heads' queries at `q` (head_dim apart); for codes as halves, each head divided by a power of two
-// that brings its largest number near 2^6, which `up0` and `up1` (lane/4, lane/4 + 8) undo.
+// The loading warp: tiles [first, last) of (row, kv head). A tile is KEYS / box boxes of `box` keys that lie in one page each. Keys in
+// pages that do not exist, and boxes behind the row's last key, are zeros (their scales: those of the first page).
 template <int D_PAD, bool KV8>
-__device__ __forceinline__ void load_q(uint32_t (&qf)[D_PAD > 128 ? 1 : D_PAD / 16][4], uint32_t q_s, const bf16* q, int g, int head_dim,
-                                       float& up0, float& up1) {
-    const int lane = threadIdx.x & 31, r0 = lane >> 2, c = lane & 3;
-    float down[2] = {1.f, 1.f};
-    up0 = up1 = 1.f;
-    if (KV8) {
-        float m[2] = {0.f, 0.f};
-        for (int ks = 0; ks < head_dim >> 4; ++ks)
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-                if (r0 + 8 * h < g) {
-                    const uint2 w = *(const uint2*)(q + (size_t)(r0 + 8 * h) * head_dim + ks * 16 + 4 * c);
-                    const float2 x = __bfloat1622float2(*(const __nv_bfloat162*)&w.x), y = __bfloat1622float2(*(const __nv_bfloat162*)&w.y);
-                    m[h] = fmaxf(fmaxf(m[h], fmaxf(c8_magnitude(x.x), c8_magnitude(x.y))), fmaxf(c8_magnitude(y.x), c8_magnitude(y.y)));
-                }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            m[h] = fmaxf(m[h], __shfl_xor_sync(0xffffffffu, m[h], 1));
-            m[h] = fmaxf(m[h], __shfl_xor_sync(0xffffffffu, m[h], 2));
-            const int e = min(max((int)(__float_as_uint(m[h]) >> 23) - 127 - 6, -100), 121);
-            down[h] = c8_power(-e);
-            (h ? up1 : up0) = c8_power(e);
-        }
-    }
-    auto pair = [&](int r, int d, float f) -> uint32_t {             // numbers d, d + 1 of head r
-        if (r >= g) return 0u;
-        const uint32_t w = *(const uint32_t*)(q + (size_t)r * head_dim + d);
-        if (!KV8) return w;
-        const float2 x = __bfloat1622float2(*(const __nv_bfloat162*)&w);
-        return pack_f16(x.x * f, x.y * f);
-    };
-    constexpr bool IN_REGS = D_PAD <= 128;
-#pragma unroll
-    for (int ks = 0; ks < D_PAD / 16; ++ks) {
-        if (ks * 16 >= head_dim) break;
-        const int lo = ks * 16 + (KV8 ? 4 * c : 2 * c), hi = lo + (KV8 ? 2 : 8);
-        const uint32_t f[4] = {pair(r0, lo, down[0]), pair(r0 + 8, lo, down[1]), pair(r0, hi, down[0]), pair(r0 + 8, hi, down[1])};
-        if (IN_REGS) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) qf[IN_REGS ? ks : 0][i] = f[i];
-        } else if (threadIdx.x < 32) {                               // (every warp makes the same ones: the first stores them)
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(q_s + (ks * 32 + lane) * 16), "r"(f[0]), "r"(f[1]), "r"(f[2]), "r"(f[3]) : "memory");
-        }
-    }
-}
-
-// One walk of the four warps over tiles [first, last) of (row, kv head); leaves each warp's sums in shared memory:
-// [warp][16][D_PAD] floats and [warp][16][2] (maximum in log2 units, sum) at `smem` + Q.
-template <int D_PAD, int STAGES, bool KV8>
-__device__ __forceinline__ void walk(unsigned char* smem, const RowsArgs& a, const int32_t* table, const bf16* q, int hk, int g, int first, int last,
-                                     int lo, int n) {
+__device__ __forceinline__ void load_tiles(const CUtensorMap* map, const RowsArgs& a, uint32_t base, const int32_t* table, int hk, int first, int last,
+                                           int n) {
     using T = Tile<D_PAD, KV8>;
-    const uint32_t q_s = smem_u32(smem), kv_s = q_s + T::Q;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const bool in_page = a.page_size % TILE_N == 0;
-    const int per_page = in_page ? a.page_size / TILE_N : 1;
-    auto page_of = [&](int tile) { return in_page && tile < last ? table[tile / per_page] : 0; };
+    const int lane = threadIdx.x & 31, boxes = T::KEYS / a.box, batch = 32 / boxes;
+    const uint32_t full = base + T::BARS, empty = full + 8 * T::STAGES;
+    const uint32_t bytes = T::STAGE + (KV8 ? 2 * T::KEYS : 0);
+    const size_t block = (size_t)a.page_size * (a.head_dim + 1);
+    for (int t0 = first; t0 < last; t0 += batch) {
+        const int key = t0 * T::KEYS + lane * a.box, pi = key / a.page_size, in = key - pi * a.page_size;     // this lane's box
+        const int page = lane < batch * boxes && key < n ? table[pi] : -1;
+        const bool there = page >= 0 && page < a.pages;
+        const int k_block = there ? page * 2 * a.kv_heads + hk : 2 * a.pages * a.kv_heads, v_block = there ? k_block + a.kv_heads : k_block;
+        const unsigned char* k_scale = a.kv + (size_t)(there ? k_block : hk) * block + (size_t)a.page_size * a.head_dim + in;
+        const unsigned char* v_scale = k_scale + (size_t)a.kv_heads * block;
+        for (int i = 0; i < batch && t0 + i < last; ++i) {
+            const int j = t0 + i - first, s = j % T::STAGES;
+            if (!__all_sync(0xffffffffu, mbar_wait(empty + 8 * s, ((j / T::STAGES) & 1) ^ 1, 1))) return;
+            if (lane == 0) mbar_expect_tx(full + 8 * s, bytes);
+            __syncwarp();
+            if (lane / boxes != i) continue;
+            const uint32_t row = (lane % boxes) * a.box, dst = base + s * T::STAGE + row * T::SUB;
 #pragma unroll
-    for (int s = 0; s < STAGES - 1; ++s) {
-        if (first + s < last) load_tile<D_PAD, KV8>(kv_s + s * T::STAGE, a, table, hk, first + s, lo, n, in_page, page_of(first + s));
-        cp_async_commit();
-    }
-    int page_ahead = page_of(first + STAGES - 1);
-    constexpr bool Q_IN_REGS = D_PAD <= 128;
-    uint32_t qf[Q_IN_REGS ? D_PAD / 16 : 1][4];
-    float up0, up1;
-    load_q<D_PAD, KV8>(qf, q_s, q, g, a.head_dim, up0, up1);
-    up0 *= a.scale_log2; up1 *= a.scale_log2;
-
-    float o[D_PAD / 8][4];
-#pragma unroll
-    for (int i = 0; i < D_PAD / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;      // rows lane/4 and lane/4 + 8
-    const int ksteps = a.head_dim >> 4;
-    // ldmatrix addresses. Keys: matrices (keys 0-7, chunk), (keys 8-15, chunk), (keys 0-7, next), (keys 8-15, next) for codes;
-    // for bfloat16 (keys 0-7, chunk), (keys 0-7, next), (keys 8-15, chunk), (keys 8-15, next). Values, transposed: as codes' keys.
-    const int key_row = warp * 16 + (lane & 7) + (KV8 ? (lane & 8) : (lane & 16) >> 1), key_ch = KV8 ? lane >> 4 : (lane >> 3) & 1;
-    const int val_row = warp * 16 + (lane & 7) + (lane & 8), val_ch = lane >> 4;
-
-    for (int tile = first; tile < last; ++tile) {
-        const int stage = (tile - first) % STAGES;
-        cp_async_wait<STAGES - 2>();
-        __syncthreads();
-        if (tile + STAGES - 1 < last)
-            load_tile<D_PAD, KV8>(kv_s + ((tile - first + STAGES - 1) % STAGES) * T::STAGE, a, table, hk, tile + STAGES - 1, lo, n, in_page, page_ahead);
-        cp_async_commit();
-        page_ahead = page_of(tile + STAGES);
-        const int key0 = tile * TILE_N + warp * 16;                 // this warp's 16 keys
-        if (key0 >= n || key0 + 16 <= lo) continue;                 // (uniform per warp; the barrier is above)
-        const uint32_t kt = kv_s + stage * T::STAGE, vt = kt + T::PART;
-        float s[2][4] = {};
-        if constexpr (KV8) {
-#pragma unroll
-            for (int p = 0; p < D_PAD / 32; ++p) {                  // 32 numbers of the head
-                if (2 * p < ksteps) {
-                    uint32_t x[4];
-                    ldmatrix_x4(x, kt + row_off<T::ROW>(key_row, 2 * p + key_ch));   // (past head_dim: whatever lies there, not used)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int ks = 2 * p + h;
-                        if (ks < ksteps) {
-                            uint32_t f[4];
-                            if (!Q_IN_REGS) asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n" : "=r"(f[0]), "=r"(f[1]), "=r"(f[2]), "=r"(f[3]) : "r"(q_s + (ks * 32 + lane) * 16));
-                            mma_f16(s[0], Q_IN_REGS ? qf[Q_IN_REGS ? ks : 0] : f, c8_halves(x[2 * h]), c8_halves(x[2 * h] >> 16));
-                            mma_f16(s[1], Q_IN_REGS ? qf[Q_IN_REGS ? ks : 0] : f, c8_halves(x[2 * h + 1]), c8_halves(x[2 * h + 1] >> 16));
-                        }
-                    }
-                }
+            for (int c = 0; c < T::NSUB; ++c) {                      // (columns past head_dim: zeros)
+                tma_load_3d(dst + c * T::BLOCK, map, full + 8 * s, c * (KV8 ? T::SUB : T::SUB / 2), in, k_block);
+                tma_load_3d(dst + T::PART + c * T::BLOCK, map, full + 8 * s, c * (KV8 ? T::SUB : T::SUB / 2), in, v_block);
             }
+            if (KV8) {
+                const uint32_t at = base + T::BODY + s * 2 * T::KEYS + row;
+                bulk_load(at, k_scale, a.box, full + 8 * s);
+                bulk_load(at + T::KEYS, v_scale, a.box, full + 8 * s);
+            }
+        }
+    }
+}
+
+// The B fragments of up to eight heads' queries at `q` (head_dim apart), head lane / 4; for codes as halves, each head divided by a
+// power of two that brings its largest number near 2^6, which `up` undoes.
+template <int D_PAD, bool KV8> struct Query {
+    uint32_t f[D_PAD / 16][2];
+    float up = 1.f;
+    __device__ __forceinline__ void load(const bf16* q, int g, int head_dim) {
+        const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+        const bf16* row = q + (size_t)(r < g ? r : 0) * head_dim;
+        if constexpr (!KV8) {
+#pragma unroll
+            for (int ks = 0; ks < D_PAD / 16; ++ks)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    f[ks][h] = r < g && ks * 16 < head_dim ? *(const uint32_t*)(row + ks * 16 + 8 * h + 2 * c) : 0u;
         } else {
+            float m = 0.f;
 #pragma unroll
             for (int ks = 0; ks < D_PAD / 16; ++ks) {
-                if (ks < ksteps) {
-                    uint32_t x[4], f[4];
-                    if (!Q_IN_REGS) asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n" : "=r"(f[0]), "=r"(f[1]), "=r"(f[2]), "=r"(f[3]) : "r"(q_s + (ks * 32 + lane) * 16));
-                    ldmatrix_x4(x, kt + row_off<T::ROW>(key_row, 2 * ks + key_ch));
-                    mma_bf16(s[0], Q_IN_REGS ? qf[Q_IN_REGS ? ks : 0] : f, x[0], x[1]);
-                    mma_bf16(s[1], Q_IN_REGS ? qf[Q_IN_REGS ? ks : 0] : f, x[2], x[3]);
+                const uint2 w = r < g && ks * 16 < head_dim ? *(const uint2*)(row + ks * 16 + 4 * c) : make_uint2(0u, 0u);
+                const float2 x = __bfloat1622float2(*(const __nv_bfloat162*)&w.x), y = __bfloat1622float2(*(const __nv_bfloat162*)&w.y);
+                m = fmaxf(fmaxf(m, fmaxf(c8_magnitude(x.x), c8_magnitude(x.y))), fmaxf(c8_magnitude(y.x), c8_magnitude(y.y)));
+                f[ks][0] = w.x; f[ks][1] = w.y;
+            }
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+            const int e = min(max((int)(__float_as_uint(m) >> 23) - 127 - 6, -100), 121);
+            const float down = c8_power(-e);
+            up = c8_power(e);
+#pragma unroll
+            for (int ks = 0; ks < D_PAD / 16; ++ks)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float2 x = __bfloat1622float2(*(const __nv_bfloat162*)&f[ks][h]);
+                    f[ks][h] = pack_f16(x.x * down, x.y * down);
                 }
-            }
         }
-        float drop[2][2] = {{1.f, 1.f}, {1.f, 1.f}};                // 2^-b of this lane's keys
-        float mx0 = -INFINITY, mx1 = -INFINITY;
+    }
+};
+
+__device__ __forceinline__ float column_max(float v) {              // over the eight lanes that hold a column
+    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+    return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+}
+__device__ __forceinline__ float column_sum(float v) {
+    v += __shfl_xor_sync(0xffffffffu, v, 4);
+    v += __shfl_xor_sync(0xffffffffu, v, 8);
+    return v + __shfl_xor_sync(0xffffffffu, v, 16);
+}
+
+// A computing warp's walk over tiles [first, last); leaves its sums over the tiles' memory: [warp][8][D_PAD] floats and
+// [warp][8][2] (maximum in log2 units, sum), once every warp is done with the tiles.
+template <int D_PAD, bool KV8>
+__device__ __forceinline__ void walk(unsigned char* smem, uint32_t base, const RowsArgs& a, const bf16* q, int g, int first, int last, int lo, int n) {
+    using T = Tile<D_PAD, KV8>;
+    constexpr int NK = T::NK;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+    const uint32_t full = base + T::BARS, empty = full + 8 * T::STAGES;
+    Query<D_PAD, KV8> query;
+    query.load(q, g, a.head_dim);
+    float up[2];                                                     // of heads 2 c, 2 c + 1
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt) {
-            float ka[2] = {1.f, 1.f}, vb[2] = {0.f, 0.f};
-            if (KV8) {                                              // (a byte below any that is written: a page that is not there, codes of 0)
-                uint16_t kw, vw;
-                const uint32_t at = vt + T::PART + warp * 16 + nt * 8 + (lane & 3) * 2;
-                asm volatile("ld.shared.u16 %0, [%1];\n" : "=h"(kw) : "r"(at));
-                asm volatile("ld.shared.u16 %0, [%1];\n" : "=h"(vw) : "r"(at + 64));
+    for (int h = 0; h < 2; ++h) up[h] = __shfl_sync(0xffffffffu, query.up, 8 * c + 4 * h) * a.scale_log2;
+    float o[D_PAD / 16][4];                                          // 16 numbers of the head x heads 2 c, 2 c + 1
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const uint32_t kb = e ? kw >> 8 : kw & 255, b = min(max(e ? vw >> 8 : vw & 255, C8_LOW + 127), 254);
-                    ka[e] = __uint_as_float(kb << 23);
-                    vb[e] = (float)((int)b - 127);
-                    drop[nt][e] = __uint_as_float((254u - b) << 23);
-                }
-            }
+    for (int i = 0; i < D_PAD / 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    const int row = warp * 16 * NK + (lane & 15), ch = lane >> 4;   // ldmatrix: (rows 0-7, chunk), (8-15, chunk), (0-7, next), (8-15, next)
+
+    for (int tile = first; tile < last; ++tile) {
+        const int j = tile - first, stage = j % T::STAGES;
+        if (!__all_sync(0xffffffffu, mbar_wait(full + 8 * stage, (j / T::STAGES) & 1, 2))) break;
+        const int key0 = tile * T::KEYS + warp * 16 * NK;            // this warp's keys
+        const uint32_t kt = base + stage * T::STAGE, vt = kt + T::PART;
+        if (key0 < n && key0 + 16 * NK > lo) {
+            float u[NK][4];                                          // keys r, r + 8 of each 16 x heads 2 c, 2 c + 1
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int j = key0 + nt * 8 + (lane & 3) * 2 + (e & 1);
-                const float u = fmaf(s[nt][e], ka[e & 1] * (e < 2 ? up0 : up1), vb[e & 1]);
-                s[nt][e] = j >= lo && j < n ? u : -INFINITY;
-            }
-            mx0 = fmaxf(mx0, fmaxf(s[nt][0], s[nt][1]));
-            mx1 = fmaxf(mx1, fmaxf(s[nt][2], s[nt][3]));
-        }
-        mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1)); mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
-        mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1)); mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
-        const float n0 = fmaxf(m0, mx0 - (KV8 ? AR_BIAS : 0.f)), n1 = fmaxf(m1, mx1 - (KV8 ? AR_BIAS : 0.f));
-        const float b0 = n0 == -INFINITY ? 0.f : n0, b1 = n1 == -INFINITY ? 0.f : n1;      // a row with nothing yet: 2^(-inf) = 0 below
-        const float c0 = ex2(m0 - b0), c1 = ex2(m1 - b1);
-        m0 = n0; m1 = n1;
-        float sum0 = 0.f, sum1 = 0.f;
+            for (int kk = 0; kk < NK; ++kk) {
+                u[kk][0] = u[kk][1] = u[kk][2] = u[kk][3] = 0.f;
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[nt][e] = ex2(s[nt][e] - (e < 2 ? b0 : b1));
-            sum0 += s[nt][0] * drop[nt][0] + s[nt][1] * drop[nt][1];
-            sum1 += s[nt][2] * drop[nt][0] + s[nt][3] * drop[nt][1];
-        }
-        l0 = l0 * c0 + sum0; l1 = l1 * c1 + sum1;                   // per-lane partial sums; quads are joined at the end
-        if (__any_sync(0xffffffffu, c0 != 1.f || c1 != 1.f)) {      // the running maximum moved: rescale what is summed
-#pragma unroll
-            for (int i = 0; i < D_PAD / 8; ++i) { o[i][0] *= c0; o[i][1] *= c0; o[i][2] *= c1; o[i][3] *= c1; }
-        }
-        uint32_t p[4];
-        if constexpr (KV8) {
-            p[0] = pack_f16(s[0][0], s[0][1]); p[1] = pack_f16(s[0][2], s[0][3]);
-            p[2] = pack_f16(s[1][0], s[1][1]); p[3] = pack_f16(s[1][2], s[1][3]);
-#pragma unroll
-            for (int d = 0; d < D_PAD / 32; ++d) {                  // 32 columns: chunks 2 d and 2 d + 1
-                if (2 * d < ksteps) {
+                for (int ks = 0; ks < D_PAD / 16; ks += KV8 ? 2 : 1) {
                     uint32_t x[4];
-                    ldmatrix_x4_trans(x, vt + row_off<T::ROW>(val_row, 2 * d + val_ch));
+                    ldmatrix_x4(x, kt + tile_at<D_PAD, KV8>(row + 16 * kk, (KV8 ? ks : 2 * ks) + ch));
+                    if constexpr (KV8) {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        if (2 * d + h < ksteps) {
-                            const uint32_t y0 = __byte_perm(x[2 * h], 0, 0x3120), y1 = __byte_perm(x[2 * h + 1], 0, 0x3120);
-                            mma_f16(o[4 * d + 2 * h], p, c8_halves(y0), c8_halves(y1));                    // even columns of the chunk
-                            mma_f16(o[4 * d + 2 * h + 1], p, c8_halves(y0 >> 16), c8_halves(y1 >> 16));    // odd ones
+                        for (int h = 0; h < 2; ++h) {
+                            const uint32_t k[4] = {c8_halves(x[2 * h]), c8_halves(x[2 * h + 1]), c8_halves(x[2 * h] >> 16), c8_halves(x[2 * h + 1] >> 16)};
+                            mma_f16(u[kk], k, query.f[ks + h][0], query.f[ks + h][1]);
                         }
+                    } else {
+                        mma_bf16(u[kk], x, query.f[ks][0], query.f[ks][1]);
                     }
                 }
             }
-        } else {
-            p[0] = pack_bf16(s[0][0], s[0][1]); p[1] = pack_bf16(s[0][2], s[0][3]);
-            p[2] = pack_bf16(s[1][0], s[1][1]); p[3] = pack_bf16(s[1][2], s[1][3]);
+            float drop[NK][2];                                       // 2^-b of this lane's keys
 #pragma unroll
-            for (int d = 0; d < D_PAD / 16; ++d) {
-                if (d < ksteps) {
-                    uint32_t x[4];
-                    ldmatrix_x4_trans(x, vt + row_off<T::ROW>(val_row, 2 * d + val_ch));
-                    mma_bf16(o[2 * d], p, x[0], x[1]);
-                    mma_bf16(o[2 * d + 1], p, x[2], x[3]);
+            for (int kk = 0; kk < NK; ++kk)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    drop[kk][i] = 1.f;
+                    if (KV8) {                                       // (a byte that is never written, in a page that is not there: codes of 0)
+                        uint32_t kb, b;
+                        const uint32_t at = base + T::BODY + stage * 2 * T::KEYS + warp * 16 * NK + kk * 16 + i * 8 + r;
+                        asm volatile("ld.shared.u8 %0, [%1];\n" : "=r"(kb) : "r"(at));
+                        asm volatile("ld.shared.u8 %0, [%1];\n" : "=r"(b) : "r"(at + T::KEYS));
+                        kb = min(kb, 254u); b = min(max(b, (uint32_t)(C8_LOW + 127)), 254u);
+                        const float ka = __uint_as_float(kb << 23), vb = (float)((int)b - 127);
+                        drop[kk][i] = __uint_as_float((254u - b) << 23);
+                        u[kk][2 * i] = fmaf(u[kk][2 * i], ka * up[0], vb);
+                        u[kk][2 * i + 1] = fmaf(u[kk][2 * i + 1], ka * up[1], vb);
+                    } else {
+                        u[kk][2 * i] *= up[0];
+                        u[kk][2 * i + 1] *= up[1];
+                    }
                 }
-            }
-        }
-    }
-    cp_async_wait<0>();
-    l0 += __shfl_xor_sync(0xffffffffu, l0, 1); l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, 1); l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-    __syncthreads();                                                // every warp is done with the tiles: reuse them
-    float* wo = (float*)(smem + T::Q);
-    float* wml = wo + 4 * 16 * D_PAD;
-    const int r0 = lane >> 2, c = lane & 3;
+            if (key0 < lo || key0 + 16 * NK > n) {
+                // Keys before `lo` and from `n` on: no score, and values that are zeros whatever their bytes say (a weight of zero
+                // times no number is none). The next copy into this stage comes behind the fence.
 #pragma unroll
-    for (int i = 0; i < D_PAD / 8; i += 2) {
-        if (i * 8 < a.head_dim) {
+                for (int kk = 0; kk < NK; ++kk)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int key = key0 + kk * 16 + i * 8 + r;
+                        if (key < lo || key >= n) u[kk][2 * i] = u[kk][2 * i + 1] = -INFINITY;
+                    }
+                for (int i = lane; i < 16 * NK * (T::ROW / 16); i += 32) {
+                    const int at = i / (T::ROW / 16), key = key0 + at;
+                    if (key < lo || key >= n)
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};\n" ::"r"(vt + tile_at<D_PAD, KV8>(warp * 16 * NK + at, i % (T::ROW / 16))), "r"(0u) : "memory");
+                }
+                fence_async_smem();
+                __syncwarp();
+            }
+            float f[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                if (r0 + 8 * h >= g) continue;
-                float* row = wo + (warp * 16 + r0 + 8 * h) * D_PAD + i * 8;
-                if (KV8) {
-                    *(float4*)(row + 4 * c) = make_float4(o[i][2 * h], o[i + 1][2 * h], o[i][2 * h + 1], o[i + 1][2 * h + 1]);
-                } else {
-                    *(float2*)(row + 2 * c) = make_float2(o[i][2 * h], o[i][2 * h + 1]);
-                    *(float2*)(row + 8 + 2 * c) = make_float2(o[i + 1][2 * h], o[i + 1][2 * h + 1]);
+                float mx = u[0][h];
+#pragma unroll
+                for (int i = 1; i < 2 * NK; ++i) mx = fmaxf(mx, u[i >> 1][2 * (i & 1) + h]);
+                const float top = fmaxf(m[h], column_max(mx) - (KV8 ? AR_BIAS : 0.f)), off = top == -INFINITY ? 0.f : top;
+                f[h] = ex2(m[h] - off);                              // (nothing yet: 2^(-inf) = 0)
+                m[h] = top;
+                float sum = 0.f;
+#pragma unroll
+                for (int i = 0; i < 2 * NK; ++i) {
+                    float& w = u[i >> 1][2 * (i & 1) + h];
+                    w = ex2(w - off);
+                    sum = KV8 ? fmaf(w, drop[i >> 1][i & 1], sum) : sum + w;
+                }
+                l[h] = fmaf(l[h], f[h], sum);                        // this lane's keys; the column is joined at the end
+            }
+            if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f)) {   // a running maximum moved: rescale what is summed
+#pragma unroll
+                for (int i = 0; i < D_PAD / 16; ++i) { o[i][0] *= f[0]; o[i][1] *= f[1]; o[i][2] *= f[0]; o[i][3] *= f[1]; }
+            }
+#pragma unroll
+            for (int kk = 0; kk < NK; ++kk) {
+                uint32_t p[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    p[i] = transposed(KV8 ? pack_f16(u[kk][2 * i], u[kk][2 * i + 1]) : pack_bf16(u[kk][2 * i], u[kk][2 * i + 1]));
+#pragma unroll
+                for (int d = 0; d < D_PAD / 16; d += KV8 ? 2 : 1) {
+                    uint32_t x[4];
+                    ldmatrix_x4_trans(x, vt + tile_at<D_PAD, KV8>(row + 16 * kk, (KV8 ? d : 2 * d) + ch));
+                    if constexpr (KV8) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {                // two neighbouring codes of two keys -> pairs of keys: even numbers, odd ones
+                            const uint32_t y0 = __byte_perm(x[2 * h], 0, 0x3120), y1 = __byte_perm(x[2 * h + 1], 0, 0x3120);
+                            const uint32_t v[4] = {c8_halves(y0), c8_halves(y0 >> 16), c8_halves(y1), c8_halves(y1 >> 16)};
+                            mma_f16(o[d + h], v, p[0], p[1]);
+                        }
+                    } else {
+                        const uint32_t v[4] = {x[0], x[2], x[1], x[3]};
+                        mma_bf16(o[d], v, p[0], p[1]);
+                    }
                 }
             }
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(empty + 8 * stage);
     }
-    if (c == 0) {
-        wml[(warp * 16 + r0) * 2] = m0; wml[(warp * 16 + r0) * 2 + 1] = l0;
-        wml[(warp * 16 + r0 + 8) * 2] = m1; wml[(warp * 16 + r0 + 8) * 2 + 1] = l1;
+    l[0] = column_sum(l[0]); l[1] = column_sum(l[1]);
+    asm volatile("bar.sync 1, %0;\n" ::"n"(32 * AR_WARPS) : "memory");   // every warp is done with the tiles: reuse them
+    float* wo = (float*)smem;
+#pragma unroll
+    for (int i = 0; i < D_PAD / 16; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (2 * c + h >= g) continue;
+            float* to = wo + (warp * AR_HEADS + 2 * c + h) * D_PAD + i * 16;
+            if (KV8) *(float2*)(to + 2 * r) = make_float2(o[i][h], o[i][2 + h]);
+            else { to[r] = o[i][h]; to[8 + r] = o[i][2 + h]; }
+        }
+    if (r == 0) {
+        float* ml = wo + AR_WARPS * AR_HEADS * D_PAD + (warp * AR_HEADS + 2 * c) * 2;
+        *(float4*)ml = make_float4(m[0], l[0], m[1], l[1]);
     }
-    __syncthreads();
 }
 
 // A running merge of partial results (maximum in log2 units, sum, weighted sum of one column), in the order of the calls.
@@ -358,63 +340,73 @@ struct Merge {
     }
 };
 
-// The result of one column of head `h`: what the splits left, the shared keys' partial results, the sink.
-__device__ __forceinline__ float finished(Merge x, const RowsArgs& a, int b, int h, int hk, int in_group, int d, bool shares) {
+// The result of one column of a head: what the splits left, the shared keys' partial results, the sink.
+__device__ __forceinline__ float finished(Merge x, const RowsArgs& a, int b, int hk, int in_group, int d, bool shares) {
+    const int group = a.heads / a.kv_heads;
     if (shares) {
         const int4 at = a.part_at[b];
-        const int group = a.heads / a.kv_heads;
         for (int s = 0; s < at.y; ++s) {
             const size_t slot = (size_t)(at.x + hk * at.y + s) * a.part_rows + at.z * group + in_group;
             x.add(a.part_ml[slot * 2], a.part_ml[slot * 2 + 1], a.part_o[slot * a.head_dim + d]);
         }
     }
-    if (a.sinks && x.l > 0.f) x.l += ex2(fmaf(a.sinks[h], 1.4426950408889634f, -x.m));   // the sink: a weight without a value
+    if (a.sinks && x.l > 0.f) x.l += ex2(fmaf(a.sinks[hk * group + in_group], 1.4426950408889634f, -x.m));   // the sink: a weight without a value
     return x.l > 0.f || x.l != x.l ? x.o / x.l : 0.f;               // (a sum that is no number gives none)
 }
 
-// grid (rows, kv_heads * m_tiles, splits), a cluster along z, 128 threads. m_tiles = ceil(group / 16).
-template <int D_PAD, int STAGES, bool KV8>
-__global__ void __launch_bounds__(AR_THREADS) rows_kernel(const RowsArgs a) {
-    extern __shared__ __align__(128) unsigned char smem[];
+// grid (rows, kv_heads * ceil(group / 8), splits), a cluster along z.
+template <int D_PAD, bool KV8>
+__global__ void __launch_bounds__(AR_THREADS, D_PAD > 128 ? 1 : 3) rows_kernel(const __grid_constant__ CUtensorMap map, const RowsArgs a) {
+    extern __shared__ unsigned char smem_raw[];
     using T = Tile<D_PAD, KV8>;
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    unsigned char* smem = smem_raw + (base - smem_u32(smem_raw));
     const bool cluster = a.splits > 1;
     if (cluster) asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");   // (this CTA runs: waited for before anybody writes here)
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < T::STAGES; ++s) {
+            mbar_init(base + T::BARS + 8 * s, 1);
+            mbar_init(base + T::BARS + 8 * (T::STAGES + s), AR_WARPS);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    }
     const int b = blockIdx.x, split = blockIdx.z, splits = a.splits;
-    const int group = a.heads / a.kv_heads, m_tiles = (group + 15) / 16;
-    const int hk = blockIdx.y / m_tiles, g0 = blockIdx.y % m_tiles * 16, g = min(16, group - g0);
+    const int group = a.heads / a.kv_heads, m_tiles = (group + AR_HEADS - 1) / AR_HEADS;
+    const int hk = blockIdx.y / m_tiles, g0 = blockIdx.y % m_tiles * AR_HEADS, g = min(AR_HEADS, group - g0);
     const int n = a.kv_len[b], t = a.query_start[b];
     const int shared = a.skip ? a.skip[b] : 0;
     const int lo = max(shared, a.window > 0 ? max(0, n - a.window) : 0);          // the one query sits at position n - 1
-    const int tile_lo = lo / TILE_N, tile_hi = (n + TILE_N - 1) / TILE_N;
+    const int tile_lo = lo / T::KEYS, tile_hi = (n + T::KEYS - 1) / T::KEYS;
     const int per = max(0, tile_hi - tile_lo + splits - 1) / splits;
     const int first = tile_lo + split * per, last = min(tile_hi, first + per);
-    walk<D_PAD, STAGES, KV8>(smem, a, a.block_table + (size_t)a.row_slot[b] * a.table_stride,
-                             a.q + ((size_t)t * a.heads + hk * group + g0) * a.head_dim, hk, g, first, last, lo, n);
-    const float* wo = (const float*)(smem + T::Q);
-    const float* wml = wo + 4 * 16 * D_PAD;
+    __syncthreads();
+    if (threadIdx.x >= 32 * AR_WARPS)
+        load_tiles<D_PAD, KV8>(&map, a, base, a.block_table + (size_t)a.row_slot[b] * a.table_stride, hk, first, last, n);
+    else
+        walk<D_PAD, KV8>(smem, base, a, a.q + ((size_t)t * a.heads + hk * group + g0) * a.head_dim, g, first, last, lo, n);
+    __syncthreads();
+    const float* wo = (const float*)smem;
+    const float* wml = wo + AR_WARPS * AR_HEADS * D_PAD;
     const int total = g * a.head_dim, share = (total + splits - 1) / splits;
     bf16* out = a.out + ((size_t)t * a.heads + hk * group + g0) * a.head_dim;
-    float* recv_o = (float*)(smem + T::BYTES(STAGES));              // [splits][share], then [splits][g][2]: what the others send
+    float* recv_o = (float*)(smem + T::RECV);                       // [splits][share], then [splits][g][2]: what the others send
     float* recv_ml = recv_o + splits * share;
-    if (cluster) {
-        __syncwarp();
-        asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");   // every CTA of the cluster runs
-    }
+    if (cluster) asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");   // every CTA of the cluster runs
     for (int i = threadIdx.x; i < total; i += AR_THREADS) {
         const int r = i / a.head_dim, d = i - r * a.head_dim;
         Merge x;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) x.add(wml[(w * 16 + r) * 2], wml[(w * 16 + r) * 2 + 1], wo[(w * 16 + r) * D_PAD + d]);
+        for (int w = 0; w < AR_WARPS; ++w) x.add(wml[(w * AR_HEADS + r) * 2], wml[(w * AR_HEADS + r) * 2 + 1], wo[(w * AR_HEADS + r) * D_PAD + d]);
         if (!cluster) {
-            out[i] = __float2bfloat16_rn(finished(x, a, b, hk * group + g0 + r, hk, g0 + r, d, shared > 0));
+            out[i] = __float2bfloat16_rn(finished(x, a, b, hk, g0 + r, d, shared > 0));
             continue;
         }
         const int peer = i / share;                                 // the CTA that combines this number
         st_cluster_f32(recv_o + split * share + (i - peer * share), peer, x.o);
         if (d == 0)
-            for (int q = 0; q < splits; ++q) {
-                st_cluster_f32(recv_ml + (split * g + r) * 2, q, x.m);
-                st_cluster_f32(recv_ml + (split * g + r) * 2 + 1, q, x.l);
+            for (int p = 0; p < splits; ++p) {
+                st_cluster_f32(recv_ml + (split * g + r) * 2, p, x.m);
+                st_cluster_f32(recv_ml + (split * g + r) * 2 + 1, p, x.l);
             }
     }
     if (!cluster) return;
@@ -425,25 +417,32 @@ __global__ void __launch_bounds__(AR_THREADS) rows_kernel(const RowsArgs a) {
         if (e >= total) break;
         const int r = e / a.head_dim, d = e - r * a.head_dim;
         Merge x;
-        for (int q = 0; q < splits; ++q) x.add(recv_ml[(q * g + r) * 2], recv_ml[(q * g + r) * 2 + 1], recv_o[q * share + i]);
-        out[e] = __float2bfloat16_rn(finished(x, a, b, hk * group + g0 + r, hk, g0 + r, d, shared > 0));
+        for (int p = 0; p < splits; ++p) x.add(recv_ml[(p * g + r) * 2], recv_ml[(p * g + r) * 2 + 1], recv_o[p * share + i]);
+        out[e] = __float2bfloat16_rn(finished(x, a, b, hk, g0 + r, d, shared > 0));
     }
 }
 
-template <int D_PAD, int STAGES, bool KV8> static size_t rows_smem(int splits, int group, int head_dim) {
-    const int g = group < 16 ? group : 16;
+template <int D_PAD, bool KV8> static size_t rows_smem(int splits, int group, int head_dim) {
+    const int g = group < AR_HEADS ? group : AR_HEADS;
     const size_t recv = splits > 1 ? (size_t)(g * head_dim + splits + splits * g * 2) * 4 : 0;      // (a share is rounded up)
-    return Tile<D_PAD, KV8>::BYTES(STAGES) + recv;
+    return Tile<D_PAD, KV8>::RECV + recv + 1024;                    // (and the way to a boundary of 1,024 bytes)
 }
 
-template <int D_PAD, int STAGES, bool KV8>
-static int launch_rows(const RowsArgs* a, int rows, int splits, int group, int head_dim, int* capacity, cudaStream_t s) {
-    auto kernel = rows_kernel<D_PAD, STAGES, KV8>;
-    const size_t smem = rows_smem<D_PAD, STAGES, KV8>(splits, group, head_dim);
-    HB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)rows_smem<D_PAD, STAGES, KV8>(16, 16, D_PAD)));
-    if (splits > 8) HB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+template <int D_PAD, bool KV8>
+static int launch_rows(RowsArgs* a, int rows, int splits, int group, int head_dim, int* capacity, cudaStream_t s) {
+    using T = Tile<D_PAD, KV8>;
+    auto kernel = rows_kernel<D_PAD, KV8>;
+    const size_t smem = rows_smem<D_PAD, KV8>(splits, group, head_dim);
+    static unsigned long long prepared = 0;                         // devices that the kernel's limits are set on
+    int device = 0;
+    HB_CUDA(cudaGetDevice(&device));
+    if (device >= 64 || !(prepared >> device & 1)) {
+        HB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)rows_smem<D_PAD, KV8>(16, AR_HEADS, D_PAD)));
+        HB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        if (device < 64) prepared |= 1ull << device;
+    }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = capacity ? dim3(1, 1, splits) : dim3(rows, a->kv_heads * ((group + 15) / 16), splits);
+    cfg.gridDim = capacity ? dim3(1, 1, splits) : dim3(rows, a->kv_heads * ((group + AR_HEADS - 1) / AR_HEADS), splits);
     cfg.blockDim = dim3(AR_THREADS);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
@@ -457,14 +456,27 @@ static int launch_rows(const RowsArgs* a, int rows, int splits, int group, int h
         else HB_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(capacity, kernel, AR_THREADS, smem));
         return 0;
     }
-    HB_CUDA(cudaLaunchKernelEx(&cfg, kernel, *a));
+    a->box = a->page_size % 64 == 0 ? 64 : a->page_size % 32 == 0 ? 32 : 16;
+    const uint64_t bytes = KV8 ? 1 : 2;
+    CUtensorMap map;
+    const cuuint64_t dims[3] = {(cuuint64_t)head_dim, (cuuint64_t)a->page_size, (cuuint64_t)a->pages * 2 * a->kv_heads};
+    const cuuint64_t strides[2] = {head_dim * bytes, a->page_size * (uint64_t)(head_dim + (KV8 ? 1 : 0)) * bytes};
+    const cuuint32_t box[3] = {(cuuint32_t)(T::SUB / bytes), (cuuint32_t)a->box, 1}, elem[3] = {1, 1, 1};
+    const CUresult r = cuTensorMapEncodeTiled(&map, KV8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+                                              const_cast<unsigned char*>(a->kv), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                              T::SUB == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) HB_REFUSE("attention_rows: cuTensorMapEncodeTiled failed with %d", (int)r);
+    HB_CUDA(cudaLaunchKernelEx(&cfg, kernel, (const CUtensorMap)map, (const RowsArgs)*a));
     return 0;
 }
-template <bool KV8> static int any_rows(const RowsArgs* a, int rows, int splits, int group, int head_dim, int* capacity, cudaStream_t s) {
-    if (head_dim <= 64) return launch_rows<64, 4, KV8>(a, rows, splits, group, head_dim, capacity, s);
-    if (head_dim <= 128) return launch_rows<128, KV8 ? 4 : 2, KV8>(a, rows, splits, group, head_dim, capacity, s);
-    return launch_rows<256, KV8 ? 3 : 2, KV8>(a, rows, splits, group, head_dim, capacity, s);
+template <bool KV8> static int any_rows(RowsArgs* a, int rows, int splits, int group, int head_dim, int* capacity, cudaStream_t s) {
+    if (head_dim <= 64) return launch_rows<64, KV8>(a, rows, splits, group, head_dim, capacity, s);
+    if (head_dim <= 128) return launch_rows<128, KV8>(a, rows, splits, group, head_dim, capacity, s);
+    return launch_rows<256, KV8>(a, rows, splits, group, head_dim, capacity, s);
 }
+
+HB_DEFINE_STATUS_MIRROR(hb_attention_rows_status_mirror)
 
 // Clusters of `splits` CTAs that run at once (splits 1: CTAs an SM); -1 where the sizes are refused.
 extern "C" int hb_attention_rows_capacity(int kv8, int head_dim, int group, int splits) {
@@ -485,16 +497,17 @@ extern "C" int hb_attention_rows(void* out, const void* q, const void* kv, int k
     if (rows == 0) return 0;
     if (head_dim % 16 || head_dim > 256 || head_dim < 16) HB_REFUSE("attention_rows: head_dim %d is no multiple of 16 up to 256", head_dim);
     if (kv_heads < 1 || heads < 1 || heads % kv_heads) HB_REFUSE("attention_rows: %d heads, %d kv heads", heads, kv_heads);
-    if (page_size < 1 || (kv8 && page_size % 16)) HB_REFUSE("attention_rows: page size %d is no multiple of 16", page_size);
+    if (page_size < 16 || page_size % 16) HB_REFUSE("attention_rows: page size %d is no multiple of 16", page_size);
     if (splits < 1 || splits > 16) HB_REFUSE("attention_rows: %d splits (1 to 16, a cluster's size)", splits);
     if (!(scale > 0.f)) HB_REFUSE("attention_rows: the score scale must be positive");
     const int group = heads / kv_heads;
-    if ((long)kv_heads * ((group + 15) / 16) > 65535) HB_REFUSE("attention_rows: %d heads", heads);
-    if (((uintptr_t)kv % 16) || (((uintptr_t)q | (uintptr_t)out) % 8)) HB_REFUSE("attention_rows: the cache must start on 16 bytes, q and out on 8");
+    if ((long)kv_heads * ((group + AR_HEADS - 1) / AR_HEADS) > 65535) HB_REFUSE("attention_rows: %d heads", heads);
+    if (pages < 1 || (long)pages * 2 * kv_heads > 0x7ffffffel) HB_REFUSE("attention_rows: %d pages of %d kv heads", pages, kv_heads);
+    if (((uintptr_t)kv % 16) || ((uintptr_t)q % 8)) HB_REFUSE("attention_rows: the cache must start on 16 bytes, q on 8");
     if (skip && (!part_o || !part_ml || !part_at || window > 0)) HB_REFUSE("attention_rows: shared keys need their partial results, and no window");
-    const RowsArgs a = {(bf16*)out, (const bf16*)q, (const unsigned char*)kv, block_table, row_slot, query_start, kv_len, sinks, skip, part_o,
-                        part_ml, (const int4*)part_at, part_rows, table_stride, heads, kv_heads, head_dim, pages, page_size, window, splits,
-                        scale * 1.4426950408889634f};
+    RowsArgs a = {(bf16*)out, (const bf16*)q, (const unsigned char*)kv, block_table, row_slot, query_start, kv_len, sinks, skip, part_o,
+                  part_ml, (const int4*)part_at, part_rows, table_stride, heads, kv_heads, head_dim, pages, page_size, 0, window, splits,
+                  scale * 1.4426950408889634f};
     return kv8 ? any_rows<true>(&a, rows, splits, group, head_dim, nullptr, (cudaStream_t)stream)
                : any_rows<false>(&a, rows, splits, group, head_dim, nullptr, (cudaStream_t)stream);
 }

@@ -654,7 +654,7 @@ class CudaKernels:
 
     def _shares(self, heads: int, kv_heads: int, head_dim: int, kv, q, out) -> bool:
         """Whether the kernels for shared beginnings take these sizes (other sizes attend row by row)."""
-        return head_dim % 16 == 0 and head_dim <= 256 and heads // kv_heads <= self._prefix_rows() \
+        return head_dim % 16 == 0 and head_dim <= 256 and kv.shape[3] % 16 == 0 and heads // kv_heads <= self._prefix_rows() \
             and not (kv.data_ptr() | q.data_ptr()) % 16 and out.data_ptr() % 8 == 0
 
     def _prefix_rows(self) -> int:
@@ -704,7 +704,7 @@ class CudaKernels:
         key = ("rows", kv8, rows, heads, kv_heads, head_dim, -(-longest // 64))
         if key not in self._splits:
             group, tiles = heads // kv_heads, max(1, -(-longest // 64))
-            pairs = rows * kv_heads * -(-group // 16)
+            pairs = rows * kv_heads * -(-group // 8)
             best = (math.inf, 1)
             for s in range(1, min(16, tiles) + 1):
                 room = int(self.lib.hb_attention_rows_capacity(kv8, head_dim, group, s)) * (self.sms if s == 1 else 1)
