@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(PX_THREADS) prefix_kernel(const PrefixArgs a) 
         const PrefixUnit u = prefix_unit(a.groups, a.n_groups, per_tile, a.kv_heads, all.chunk, w);
         const int mrows = u.count * group;
         if (u.hk == 0 && u.split == 0 && threadIdx.x < u.count)
-            a.part_at[a.members[u.start + threadIdx.x]] = make_int4(u.first, u.splits, (int)threadIdx.x, 0);
+            a.part_at[a.members[u.start + threadIdx.x]] = make_int4(u.first, u.splits, (int)threadIdx.x * group, 0);
         __syncthreads();                                            // (the tiles are no longer read by the unit before)
         for (int i = threadIdx.x; i < PX_ROWS * (D_PAD / 8); i += PX_THREADS) {
             const int r = i / (D_PAD / 8), ch = i % (D_PAD / 8);
@@ -181,19 +181,38 @@ template <int D_PAD, bool KV8> static int launch_prefix(const PrefixArgs& a, int
     return 0;
 }
 
-// Query rows a tile holds: the partial results of unit u lie at rows u * hb_attention_prefix_rows() of part_o and part_ml.
-extern "C" int hb_attention_prefix_rows(void) { return PX_ROWS; }
+int hb_attention_prefix_tcgen05(float* part_o, float* part_ml, int32_t* part_at, const void* q, const void* kv, int kv8, const int32_t* block_table,
+                                int table_stride, const int32_t* row_slot, const int32_t* query_start, const int32_t* members, const int32_t* groups,
+                                int n_groups, int heads, int kv_heads, int pages, int page_size, float scale, int ctas, cudaStream_t s);
+static bool on_tcgen05(int head_dim, int page_size, int group) { return head_dim == 128 && page_size % 64 == 0 && group <= 128; }
+
+extern "C" int hb_attention_prefix_plan(int head_dim, int page_size, int group, int* part_rows, int* tile_rows) {
+    if (head_dim % 16 || head_dim > 256 || head_dim < 16 || group < 1 || page_size < 1) return 0;
+    if (on_tcgen05(head_dim, page_size, group)) {
+        *part_rows = 256;
+        *tile_rows = 2 * (128 / group);
+        return 1;
+    }
+    *part_rows = PX_ROWS;
+    *tile_rows = PX_ROWS / group;
+    return group <= PX_ROWS ? 2 : 0;
+}
 
 extern "C" int hb_attention_prefix(float* part_o, float* part_ml, int32_t* part_at, const void* q, const void* kv, int kv8,
                                    const int32_t* block_table, int table_stride, const int32_t* row_slot, const int32_t* query_start,
                                    const int32_t* members, const int32_t* groups, int n_groups, int heads, int kv_heads, int head_dim, int pages,
                                    int page_size, float scale, int ctas, hb_stream stream) {
     if (n_groups < 1 || ctas < 1) return 0;
-    if (head_dim % 16 || head_dim > 256 || head_dim < 16) HB_REFUSE("attention_prefix: head_dim %d is no multiple of 16 up to 256", head_dim);
-    if (kv_heads < 1 || heads < 1 || heads % kv_heads || heads / kv_heads > PX_ROWS) HB_REFUSE("attention_prefix: %d heads, %d kv heads", heads, kv_heads);
-    if (page_size < 1 || (kv8 && page_size % 16)) HB_REFUSE("attention_prefix: page size %d is no multiple of 16", page_size);
+    int part_rows, tile_rows;
+    if (kv_heads < 1 || heads < 1 || heads % kv_heads || !hb_attention_prefix_plan(head_dim, page_size, heads / kv_heads, &part_rows, &tile_rows))
+        HB_REFUSE("attention_prefix: %d heads, %d kv heads of %d", heads, kv_heads, head_dim);
+    if (page_size < 16 || page_size % 16) HB_REFUSE("attention_prefix: page size %d is no multiple of 16", page_size);
     if (!(scale > 0.f)) HB_REFUSE("attention_prefix: the score scale must be positive");
+    if (pages < 1 || (long)pages * 2 * kv_heads > 0x7ffffffel) HB_REFUSE("attention_prefix: %d pages of %d kv heads", pages, kv_heads);
     if (((uintptr_t)kv | (uintptr_t)q | (uintptr_t)part_at | (uintptr_t)part_o) % 16 || (uintptr_t)part_ml % 8) HB_REFUSE("attention_prefix: tensors must start on 16 bytes");
+    if (on_tcgen05(head_dim, page_size, heads / kv_heads))
+        return hb_attention_prefix_tcgen05(part_o, part_ml, part_at, q, kv, kv8, block_table, table_stride, row_slot, query_start, members, groups,
+                                           n_groups, heads, kv_heads, pages, page_size, scale, ctas, (cudaStream_t)stream);
     const PrefixArgs a = {part_o, part_ml, (int4*)part_at, (const bf16*)q, (const unsigned char*)kv, block_table, row_slot, query_start, members,
                           groups, n_groups, table_stride, heads, kv_heads, head_dim, pages, page_size, scale * 1.4426950408889634f};
     cudaStream_t s = (cudaStream_t)stream;

@@ -1,0 +1,444 @@
+// Attention of rows that share their first pages over those pages' keys, head size 128 and pages of a multiple of 64 tokens:
+// attention_prefix.cu's work on tcgen05 tensor cores.
+//
+// A tile is up to two groups of 128 query rows (rows of the step x query heads of the kv head); a persistent CTA, one an SM, takes
+// units of it (prefix_units.cuh). Per group and 64 keys, as in the kernel for prompts: S = Q K^T (128 x 64 x 16, eight products,
+// operands in shared memory, S in one of two 64-column buffers of tensor memory); softmax with a query row a thread, the weights go back
+// over the S they came from; O += P V (128 x 128 x 16, four products, P from tensor memory). The running maximum may lag by 2^8
+// before O is rescaled. No key is masked: shared pages are whole, and whole numbers of 64 keys.
+// bfloat16 pages: keys and values come by TMA as the products want them. 8-bit pages: TMA brings the codes, two warps turn them
+// into halves (exactly) in the same layout, and the softmax applies the rows' scales as attention_rows.cu does: u = s 2^(a + c) scale
+// log2(e) + b, weights 2^(u - M) times 2^7 so that with the lag they stay below a half's largest, sums with 2^-b.
+// Barriers keep their phases from unit to unit; every role counts the tiles that it has seen.
+#include <cuda_fp16.h>
+
+#include "cache8.cuh"
+#include "prefix_units.cuh"
+#include "tcgen05.cuh"
+
+#define PT_D 128
+#define PT_BM 128                                 // query rows per group
+#define PT_GROUPS 2
+#define PT_BN 64
+#define PT_Q_BYTES (PT_BM * PT_D * 2)             // 32 KB a group: two [128 x 64] swizzled blocks
+#define PT_KV_BYTES (PT_BN * PT_D * 2)            // 16 KB: two [64 x 64] swizzled blocks
+#define PT_RAW_BYTES (PT_BN * PT_D)               // 8 KB of codes
+#define PT_RAW_STAGE (2 * PT_RAW_BYTES + 1024)    // keys, values, 64 + 64 scale bytes
+#define PT_TMEM_COLS 512                          // per group: S0 [0, 64), S1 [64, 128), O [128, 256)
+#define PT_RESCALE 8.0f
+#define PT_BIAS 7.0f                              // 8-bit pages: what the weights are raised by
+#define PT_MMA_WARP1 10                           // warps 10, 11: the groups' P V; 2 - 9: softmax; 0: loads; 1: Q K^T; 12, 13: codes to halves
+#define PT_CONVERTERS 2
+
+template <bool KV8> struct Shape {
+    static constexpr int THREADS = KV8 ? 448 : 384;
+    static constexpr int STAGES = KV8 ? 2 : 3;    // of keys and values as the products read them
+    static constexpr int RAW = KV8 ? 4 : 1;       // of codes (bfloat16: none, and no barrier of theirs is used)
+    static constexpr int KV = PT_GROUPS * PT_Q_BYTES, RAWS = KV + STAGES * 2 * PT_KV_BYTES, SCALES = RAWS + (KV8 ? RAW * PT_RAW_STAGE : 0);
+    static constexpr int UP = SCALES + (KV8 ? STAGES * 3 * PT_BN * 4 : 0);           // [256] floats: what undoes a query's scale
+    static constexpr int BARS = UP + (KV8 ? PT_GROUPS * PT_BM * 4 : 0);
+    static constexpr int SMEM = BARS + 512 + 1024;
+};
+
+struct PrefixTcArgs {
+    float *part_o, *part_ml;
+    int4* part_at;
+    const bf16* q;
+    const unsigned char* kv;
+    const int32_t *block_table, *row_slot, *query_start, *members, *groups;
+    int n_groups, table_stride, heads, kv_heads, pages, page_size;
+    float scale_log2;
+};
+
+__device__ __forceinline__ void pt_bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ void st_shared16(uint32_t at, const uint4& v) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ uint4 ld_shared16(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+    return v;
+}
+
+// The tile's queries, row by row (eight lanes a row): group g's row r is head r % group of the tile's row g * per_group + r / group.
+// Rows without a query are zeros. 8-bit pages: as halves, each row divided by a power of two that brings its largest number near 2^6.
+template <bool KV8>
+__device__ __forceinline__ void load_queries(unsigned char* smem, uint32_t q_s, const PrefixTcArgs& a, const PrefixUnit& u, int group, int per_group) {
+    const int sub = threadIdx.x & 7;
+    for (int i = threadIdx.x >> 3; i < PT_GROUPS * PT_BM; i += Shape<KV8>::THREADS / 8) {
+        const int g = i / PT_BM, r = i % PT_BM, row = g * per_group + r / group;
+        const bool live = r < per_group * group && row < u.count;
+        uint4 x = make_uint4(0, 0, 0, 0), y = x;
+        if (live) {
+            const bf16* src = a.q + ((size_t)a.query_start[a.members[u.start + row]] * a.heads + u.hk * group + r % group) * PT_D;
+            x = *(const uint4*)(src + sub * 8);
+            y = *(const uint4*)(src + 64 + sub * 8);
+        }
+        if (KV8) {
+            uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+            float m = 0.f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float2 v = __bfloat1622float2(*(const __nv_bfloat162*)&w[k]);
+                m = fmaxf(m, fmaxf(c8_magnitude(v.x), c8_magnitude(v.y)));
+            }
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+            const int e = min(max((int)(__float_as_uint(m) >> 23) - 127 - 6, -100), 121);
+            const float down = c8_power(-e);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float2 v = __bfloat1622float2(*(const __nv_bfloat162*)&w[k]);
+                const __half2 h = __floats2half2_rn(v.x * down, v.y * down);
+                w[k] = *(const uint32_t*)&h;
+            }
+            x = make_uint4(w[0], w[1], w[2], w[3]);
+            y = make_uint4(w[4], w[5], w[6], w[7]);
+            if (sub == 0) ((float*)(smem + Shape<KV8>::UP))[i] = c8_power(e);
+        }
+        const uint32_t at = q_s + g * PT_Q_BYTES + r * 128 + ((sub ^ (r & 7)) << 4);
+        st_shared16(at, x);
+        st_shared16(at + PT_Q_BYTES / 2, y);
+    }
+    fence_async_smem();                                               // (the products read them through the async proxy)
+}
+
+template <bool KV8>
+__global__ void __launch_bounds__(Shape<KV8>::THREADS, 1) prefix_tcgen05_kernel(const __grid_constant__ CUtensorMap map_kv, const PrefixTcArgs a) {
+    extern __shared__ unsigned char smem_raw[];
+    using H = Shape<KV8>;
+    const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
+    unsigned char* smem = smem_raw + (base - smem_addr(smem_raw));
+    const uint32_t q_s = base, kv_s = base + H::KV, bars = base + H::BARS;
+    const uint32_t kv_full0 = bars, kv_empty0 = kv_full0 + 8 * H::STAGES, raw_full0 = kv_empty0 + 8 * H::STAGES, raw_empty0 = raw_full0 + 8 * H::RAW;
+    // per group g and buffer i, at index (g * 2 + i): scores computed; weights written; weights read (O holds the tile)
+    const uint32_t s_full0 = raw_empty0 + 8 * H::RAW, p_full0 = s_full0 + 32, p_empty0 = p_full0 + 32, o_full0 = p_empty0 + 32, slot = o_full0 + 16;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int group = a.heads / a.kv_heads, per_group = PT_BM / group, per_tile = PT_GROUPS * per_group;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < H::STAGES; ++s) { mbar_init(kv_full0 + 8 * s, KV8 ? PT_CONVERTERS : 1); mbar_init(kv_empty0 + 8 * s, 1 + PT_GROUPS); }
+        for (int s = 0; s < H::RAW; ++s) { mbar_init(raw_full0 + 8 * s, 1); mbar_init(raw_empty0 + 8 * s, PT_CONVERTERS); }
+        for (int i = 0; i < 2 * PT_GROUPS; ++i) { mbar_init(s_full0 + 8 * i, 1); mbar_init(p_full0 + 8 * i, 4); mbar_init(p_empty0 + 8 * i, 1); }
+        for (int g = 0; g < PT_GROUPS; ++g) mbar_init(o_full0 + 8 * g, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(slot), "r"(PT_TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+    }
+    const PrefixUnits all = prefix_units(a.groups, a.n_groups, per_tile, a.kv_heads, gridDim.x);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    uint32_t tmem;
+    asm volatile("ld.shared.b32 %0, [%1];\n" : "=r"(tmem) : "r"(slot));
+
+    int seen = 0, g_seen[PT_GROUPS] = {0, 0}, g_units[PT_GROUPS] = {0, 0};       // tiles before this unit: of all, of a group's own; its units
+    bool ok = true;
+    for (int w = blockIdx.x; w < all.units; w += gridDim.x) {
+        const PrefixUnit u = prefix_unit(a.groups, a.n_groups, per_tile, a.kv_heads, all.chunk, w);
+        const int first = u.split * all.chunk, tiles = min(u.tokens / PT_BN, first + all.chunk) - first;
+        int g_rows[PT_GROUPS];                                        // query rows of each group
+#pragma unroll
+        for (int g = 0; g < PT_GROUPS; ++g) g_rows[g] = max(0, min(per_group, u.count - g * per_group)) * group;
+        if (warp == 0 && u.hk == 0 && u.split == 0)
+            for (int i = lane; i < u.count; i += 32)
+                a.part_at[a.members[u.start + i]] = make_int4(u.first, u.splits, i / per_group * PT_BM + i % per_group * group, 0);
+        load_queries<KV8>(smem, q_s, a, u, group, per_group);
+        __syncthreads();
+
+        if (warp == 0) {
+            const int32_t* table = a.block_table + (size_t)a.row_slot[a.members[u.start]] * a.table_stride;
+            for (int t0 = 0; t0 < tiles && ok; t0 += 32) {
+                const int key = (first + t0 + lane) * PT_BN, pi = key / a.page_size, in = key - pi * a.page_size;     // this lane's tile
+                int page = t0 + lane < tiles ? table[pi] : 0;
+                const bool there = page >= 0 && page < a.pages;       // (a page that is not there: zeros)
+                const int k_block = there ? page * 2 * a.kv_heads + u.hk : 2 * a.pages * a.kv_heads;
+                const int v_block = there ? k_block + a.kv_heads : k_block;
+                const size_t bytes = (size_t)a.page_size * (PT_D + 1);
+                const unsigned char* k_scale = a.kv + (size_t)(there ? k_block : u.hk) * bytes + (size_t)a.page_size * PT_D + in;
+                for (int i = 0; i < 32 && t0 + i < tiles; ++i) {
+                    const int n = seen + t0 + i, s = n % (KV8 ? H::RAW : H::STAGES), turn = n / (KV8 ? H::RAW : H::STAGES);
+                    ok = __all_sync(0xffffffffu, mbar_wait((KV8 ? raw_empty0 : kv_empty0) + 8 * s, (turn & 1) ^ 1, 1));
+                    if (!ok) break;
+                    if (lane != i) continue;
+                    if (KV8) {
+                        const uint32_t full = raw_full0 + 8 * s, dst = base + H::RAWS + s * PT_RAW_STAGE;
+                        mbar_expect_tx(full, 2 * PT_RAW_BYTES + 128);
+                        tma_load_3d(dst, &map_kv, full, 0, in, k_block);
+                        tma_load_3d(dst + PT_RAW_BYTES, &map_kv, full, 0, in, v_block);
+                        pt_bulk_load(dst + 2 * PT_RAW_BYTES, k_scale, 64, full);
+                        pt_bulk_load(dst + 2 * PT_RAW_BYTES + 64, k_scale + (size_t)a.kv_heads * bytes, 64, full);
+                    } else {
+                        const uint32_t full = kv_full0 + 8 * s, dst = kv_s + s * 2 * PT_KV_BYTES;
+                        mbar_expect_tx(full, 2 * PT_KV_BYTES);
+                        tma_load_3d(dst, &map_kv, full, 0, in, k_block);
+                        tma_load_3d(dst + PT_KV_BYTES / 2, &map_kv, full, 64, in, k_block);
+                        tma_load_3d(dst + PT_KV_BYTES, &map_kv, full, 0, in, v_block);
+                        tma_load_3d(dst + PT_KV_BYTES + PT_KV_BYTES / 2, &map_kv, full, 64, in, v_block);
+                    }
+                }
+            }
+        } else if (KV8 && warp >= 12) {
+            const int part = warp - 12, sub = lane & 7;
+            for (int j = 0; j < tiles && ok; ++j) {
+                const int n = seen + j, s = n % H::RAW, d = n % H::STAGES;
+                ok = mbar_wait(raw_full0 + 8 * s, (n / H::RAW) & 1, 2) && mbar_wait(kv_empty0 + 8 * d, ((n / H::STAGES) & 1) ^ 1, 3);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                const uint32_t raw = base + H::RAWS + s * PT_RAW_STAGE, dst = kv_s + d * 2 * PT_KV_BYTES;
+                float* scales = (float*)(smem + H::SCALES + d * 3 * PT_BN * 4);
+                {
+                    const int key = part * 32 + lane;
+                    const unsigned char* b = smem + H::RAWS + s * PT_RAW_STAGE + 2 * PT_RAW_BYTES + key;
+                    const int kb = min((int)b[0], 254), vb = min(max((int)b[64], C8_LOW + 127), 254);
+                    scales[key] = __uint_as_float((uint32_t)kb << 23);
+                    scales[PT_BN + key] = (float)(vb - 127);
+                    scales[2 * PT_BN + key] = __uint_as_float((uint32_t)(254 - vb) << 23);
+                }
+                // Eight lanes read four chunks of 16 codes of a row and of row ^ 5, and write them as halves: no two of either in one
+                // group of banks. One warp takes the first halves of all rows, the other the second ones.
+#pragma unroll 4
+                for (int i = 0; i < 16; ++i) {
+                    const int row = (i & 7) * 8 + ((lane >> 3) ^ (sub >> 2) * 5), ch = part * 4 + (sub & 3);
+                    const uint32_t from = raw + (i >> 3) * PT_RAW_BYTES + row * 128 + ((ch ^ (row & 7)) << 4);
+                    const uint4 c = ld_shared16(from);
+                    const uint4 lo = make_uint4(c8_halves(c.x), c8_halves(c.x >> 16), c8_halves(c.y), c8_halves(c.y >> 16));
+                    const uint4 hi = make_uint4(c8_halves(c.z), c8_halves(c.z >> 16), c8_halves(c.w), c8_halves(c.w >> 16));
+                    const uint32_t to = dst + (i >> 3) * PT_KV_BYTES + part * (PT_KV_BYTES / 2) + row * 128;
+                    st_shared16(to + (((2 * (ch & 3)) ^ (row & 7)) << 4), lo);
+                    st_shared16(to + (((2 * (ch & 3) + 1) ^ (row & 7)) << 4), hi);
+                }
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) { mbar_arrive(kv_full0 + 8 * d); mbar_arrive(raw_empty0 + 8 * s); }
+            }
+        } else if (warp == 1 || (warp >= PT_MMA_WARP1 && warp < 12)) {
+            if (lane == 0) {
+                // kind::f16, D float32, A and B bfloat16 or half; N / 8 at bit 17, M / 16 at bit 24; bit 16: B is MN-major
+                const uint32_t types = (1u << 4) | (KV8 ? 0u : (1u << 7) | (1u << 10));
+                const uint32_t idesc_qk = types | ((uint32_t)(PT_BN >> 3) << 17) | ((uint32_t)(PT_BM >> 4) << 24);
+                const uint32_t idesc_pv = types | (1u << 16) | ((uint32_t)(PT_D >> 3) << 17) | ((uint32_t)(PT_BM >> 4) << 24);
+                if (warp == 1) {
+                    for (int j = 0; j < tiles && ok; ++j) {
+                        const int n = seen + j, s = n % H::STAGES;
+                        ok = mbar_wait(kv_full0 + 8 * s, (n / H::STAGES) & 1, 4);
+                        const uint32_t k_src = kv_s + s * 2 * PT_KV_BYTES;
+                        for (int g = 0; g < PT_GROUPS && ok; ++g) {
+                            if (g_rows[g] == 0) continue;
+                            const int k = g_seen[g] + j, gb = g * 2 + (k & 1);
+                            // S overwrites S and P of two tiles ago: wait until their P V has read them
+                            ok = mbar_wait(p_empty0 + 8 * gb, ((k >> 1) & 1) ^ 1, 5);
+                            if (!ok) break;
+                            tc_fence_after();
+                            const uint32_t s_t = tmem + g * 256 + (k & 1) * PT_BN;
+#pragma unroll
+                            for (int kk = 0; kk < PT_D / 16; ++kk) {  // d 0..63 in the first block, 64..127 in the second
+                                const uint32_t blk = kk >> 2, within = (kk & 3) * 2;
+                                tc_mma(s_t, tc_smem_desc(q_s + g * PT_Q_BYTES + blk * (PT_Q_BYTES / 2)) + within,
+                                       tc_smem_desc(k_src + blk * (PT_KV_BYTES / 2)) + within, idesc_qk, kk != 0);
+                            }
+                            tc_commit(s_full0 + 8 * gb);
+                        }
+                        if (ok) tc_commit(kv_empty0 + 8 * s);         // the keys of the stage have been read (all three must arrive)
+                    }
+                } else {
+                    const int g = warp - PT_MMA_WARP1;
+                    const uint32_t o_t = tmem + g * 256 + 2 * PT_BN;
+                    for (int j = 0; j < tiles && ok; ++j) {           // (a group without rows still paces the stages)
+                        const int n = seen + j, s = n % H::STAGES;
+                        ok = mbar_wait(kv_full0 + 8 * s, (n / H::STAGES) & 1, 6);
+                        if (ok && g_rows[g] > 0) {                    // O_g += P_g V
+                            const int k = g_seen[g] + j, gb = g * 2 + (k & 1);
+                            ok = mbar_wait(p_full0 + 8 * gb, (k >> 1) & 1, 7);
+                            if (!ok) break;
+                            tc_fence_after();
+                            const uint32_t v_src = kv_s + s * 2 * PT_KV_BYTES + PT_KV_BYTES;
+                            const uint32_t p_t = tmem + g * 256 + (k & 1) * PT_BN;   // P lies over the first half of its own S
+#pragma unroll
+                            for (int kk = 0; kk < PT_BN / 16; ++kk)   // 16 keys a step: 8 columns along P, 16 rows down V
+                                tc_mma_f16_ts(o_t, p_t + kk * 8, tc_smem_desc_mn(v_src + kk * 16 * 128, PT_KV_BYTES / 2), idesc_pv, (j | kk) != 0);
+                            tc_commit(p_empty0 + 8 * gb);             // P has been read; O_g holds the tile
+                            if (j == tiles - 1) tc_commit(o_full0 + 8 * g);
+                        }
+                        if (ok) tc_commit(kv_empty0 + 8 * s);         // the values of the stage have been read
+                    }
+                }
+            }
+            ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+        } else if (warp >= 2 && warp < PT_MMA_WARP1) {
+            const int g = (warp - 2) >> 2;                            // this warp's group of query rows
+            const int quarter = warp & 3;                             // and its quarter of the TMEM lanes
+            const int r = quarter * 32 + lane;                        // this thread's query row within the group
+            const uint32_t lane_t = tmem + g * 256 + ((uint32_t)(quarter * 32) << 16);
+            const uint32_t o_t = lane_t + 2 * PT_BN;
+            float m_used = -INFINITY, l = 0.f;                        // in log2 units; the maximum may lag by PT_RESCALE
+            const float factor = KV8 ? a.scale_log2 * ((const float*)(smem + H::UP))[g * PT_BM + r] : a.scale_log2;
+            const uint64_t factor2 = pack2(factor, factor);
+            if (g_rows[g] > 0) {
+                for (int j = 0; j < tiles && ok; ++j) {
+                    const int k = g_seen[g] + j, gb = g * 2 + (k & 1);
+                    ok = mbar_wait(s_full0 + 8 * gb, (k >> 1) & 1, 8);
+                    if (KV8 && ok) ok = mbar_wait(kv_full0 + 8 * ((seen + j) % H::STAGES), ((seen + j) / H::STAGES) & 1, 9);   // (the scales)
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    tc_fence_after();
+                    uint32_t sr[2][32];
+                    tc_ld32_nowait(lane_t + (k & 1) * PT_BN, sr[0]);
+                    tc_ld32_nowait(lane_t + (k & 1) * PT_BN + 32, sr[1]);
+                    tc_ld_wait();
+                    const uint32_t scales = base + H::SCALES + ((seen + j) % H::STAGES) * 3 * PT_BN * 4;
+                    if (KV8) {
+#pragma unroll
+                        for (int i = 0; i < PT_BN; i += 4) {
+                            const uint4 ka = ld_shared16(scales + i * 4), vb = ld_shared16(scales + (PT_BN + i) * 4);
+                            uint32_t* x = &sr[i >> 5][i & 31];
+                            float f0, f1;
+                            unpack2(fma2(mul2(pack2(__uint_as_float(x[0]), __uint_as_float(x[1])), pack2(__uint_as_float(ka.x), __uint_as_float(ka.y))),
+                                         factor2, pack2(__uint_as_float(vb.x), __uint_as_float(vb.y))), f0, f1);
+                            x[0] = __float_as_uint(f0); x[1] = __float_as_uint(f1);
+                            unpack2(fma2(mul2(pack2(__uint_as_float(x[2]), __uint_as_float(x[3])), pack2(__uint_as_float(ka.z), __uint_as_float(ka.w))),
+                                         factor2, pack2(__uint_as_float(vb.z), __uint_as_float(vb.w))), f0, f1);
+                            x[2] = __float_as_uint(f0); x[3] = __float_as_uint(f1);
+                        }
+                    }
+                    float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};   // four chains instead of one of 64
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) mx4[i & 3] = fmaxf(mx4[i & 3], __uint_as_float(sr[c][i]));
+                    const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+                    const float mt = KV8 ? mx - PT_BIAS : mx * factor;
+                    const bool grow = mt > m_used + PT_RESCALE || (m_used == -INFINITY && mt > -INFINITY);
+                    if (__any_sync(0xffffffffu, grow)) {              // rescale what is summed (whole warp: the TMEM ops are collective)
+                        const float m_new = grow ? mt : m_used;
+                        const float f = m_used == -INFINITY ? 0.f : at_ex2(m_used - m_new);
+                        if (j > 0) {
+                            ok = mbar_wait(p_empty0 + 8 * (g * 2 + ((k - 1) & 1)), ((k - 1) >> 1) & 1, 10);   // O holds every tile before this one
+                            ok = __all_sync(0xffffffffu, ok);
+                            if (!ok) break;
+                            tc_fence_after();
+#pragma unroll
+                            for (int c = 0; c < PT_D / 32; ++c) {
+                                uint32_t o[32];
+                                tc_ld32(o_t + c * 32, o);
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                                tc_st32(o_t + c * 32, o);
+                            }
+                        }
+                        l *= f;
+                        m_used = m_new;
+                    }
+                    const float off = m_used == -INFINITY ? 0.f : -m_used;
+                    const uint64_t off2 = pack2(off, off);
+                    uint64_t sum2[4] = {0ull, 0ull, 0ull, 0ull};      // four chains of packed sums
+                    uint32_t pk[32];                                  // 64 weights as pairs
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2) {
+                            float x, y;
+                            const uint64_t pair = pack2(__uint_as_float(sr[c][i]), __uint_as_float(sr[c][i + 1]));
+                            unpack2(KV8 ? add2(pair, off2) : fma2(pair, factor2, off2), x, y);
+                            x = at_ex2(x);
+                            y = at_ex2(y);
+                            if (KV8) {
+                                uint64_t drop;
+                                asm volatile("ld.shared.b64 %0, [%1];\n" : "=l"(drop) : "r"(scales + (2 * PT_BN + c * 32 + i) * 4));
+                                sum2[(i >> 1) & 3] = fma2(pack2(x, y), drop, sum2[(i >> 1) & 3]);
+                                const __half2 h = __floats2half2_rn(x, y);
+                                pk[c * 16 + i / 2] = *(const uint32_t*)&h;
+                            } else {
+                                sum2[(i >> 1) & 3] = add2(sum2[(i >> 1) & 3], pack2(x, y));
+                                const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+                                pk[c * 16 + i / 2] = *(const uint32_t*)&h;
+                            }
+                        }
+                    float lo, hi;
+                    unpack2(add2(add2(sum2[0], sum2[1]), add2(sum2[2], sum2[3])), lo, hi);
+                    l += lo + hi;
+                    tc_st32(lane_t + (k & 1) * PT_BN, pk);            // P over the S it came from: 32 columns of pairs
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(p_full0 + 8 * gb);
+                }
+                if (ok) ok = __all_sync(0xffffffffu, mbar_wait(o_full0 + 8 * g, g_units[g] & 1, 11));
+                tc_fence_after();
+                if (ok) {                                             // (the tensor-memory loads are warp-collective: no lane skips them)
+                    const size_t at = (size_t)w * (PT_GROUPS * PT_BM) + g * PT_BM + r;
+                    const bool mine = r < g_rows[g];
+                    if (mine) *(float2*)(a.part_ml + at * 2) = make_float2(m_used, l);
+#pragma unroll
+                    for (int c = 0; c < PT_D / 32; ++c) {
+                        uint32_t o[32];
+                        tc_ld32(o_t + c * 32, o);
+                        if (mine) {
+#pragma unroll
+                            for (int i = 0; i < 32; i += 4)
+                                *(uint4*)(a.part_o + at * PT_D + c * 32 + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                        }
+                    }
+                    tc_fence_before();
+                }
+            }
+        }
+        seen += tiles;
+#pragma unroll
+        for (int g = 0; g < PT_GROUPS; ++g)
+            if (g_rows[g] > 0) { g_seen[g] += tiles; ++g_units[g]; }
+        if (!__syncthreads_and((int)ok)) break;                       // a wait that gave up anywhere ends the walk everywhere
+        tc_fence_after();
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(PT_TMEM_COLS) : "memory");
+    }
+}
+
+HB_DEFINE_STATUS_MIRROR(hb_attention_prefix_status_mirror)
+
+template <bool KV8> static int launch(const PrefixTcArgs& a, int ctas, cudaStream_t s) {
+    using H = Shape<KV8>;
+    const uint64_t bytes = KV8 ? 1 : 2;
+    CUtensorMap map;
+    const cuuint64_t dims[3] = {PT_D, (cuuint64_t)a.page_size, (cuuint64_t)a.pages * 2 * a.kv_heads};
+    const cuuint64_t strides[2] = {PT_D * bytes, a.page_size * (uint64_t)(PT_D + (KV8 ? 1 : 0)) * bytes};
+    const cuuint32_t box[3] = {KV8 ? 128u : 64u, PT_BN, 1}, elem[3] = {1, 1, 1};
+    const CUresult r = cuTensorMapEncodeTiled(&map, KV8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+                                              const_cast<unsigned char*>(a.kv), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) HB_REFUSE("attention_prefix: cuTensorMapEncodeTiled failed with %d", (int)r);
+    auto kernel = prefix_tcgen05_kernel<KV8>;
+    static unsigned long long prepared = 0;                           // devices that the kernel's limit is set on
+    int device = 0;
+    HB_CUDA(cudaGetDevice(&device));
+    if (device >= 64 || !(prepared >> device & 1)) {
+        HB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, H::SMEM));
+        if (device < 64) prepared |= 1ull << device;
+    }
+    kernel<<<ctas, H::THREADS, H::SMEM, s>>>(map, a);
+    HB_LAUNCH_CHECK("attention_prefix");
+    return 0;
+}
+
+// hb_attention_prefix's work where head_dim is 128 and pages are multiples of 64 tokens (its checks are done).
+int hb_attention_prefix_tcgen05(float* part_o, float* part_ml, int32_t* part_at, const void* q, const void* kv, int kv8, const int32_t* block_table,
+                                int table_stride, const int32_t* row_slot, const int32_t* query_start, const int32_t* members, const int32_t* groups,
+                                int n_groups, int heads, int kv_heads, int pages, int page_size, float scale, int ctas, cudaStream_t s) {
+    const PrefixTcArgs a = {part_o, part_ml, (int4*)part_at, (const bf16*)q, (const unsigned char*)kv, block_table, row_slot, query_start, members,
+                            groups, n_groups, table_stride, heads, kv_heads, pages, page_size, scale * 1.4426950408889634f};
+    return kv8 ? launch<true>(a, ctas, s) : launch<false>(a, ctas, s);
+}

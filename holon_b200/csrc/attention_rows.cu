@@ -54,6 +54,11 @@ __device__ __forceinline__ void st_cluster_f32(const float* local, uint32_t rank
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(remote) : "r"(smem_u32(local)), "r"(rank));
     asm volatile("st.shared::cluster.f32 [%0], %1;\n" ::"r"(remote), "f"(v) : "memory");
 }
+__device__ __forceinline__ void st_cluster_f32x4(const float* local, uint32_t rank, const float4& v) {
+    uint32_t remote;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(remote) : "r"(smem_u32(local)), "r"(rank));
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};\n" ::"r"(remote), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+}
 // An untiled copy of a few bytes (16-byte boundaries and size), counted on `bar`.
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n"
@@ -68,7 +73,7 @@ struct RowsArgs {
     const float* sinks;
     const int32_t* skip;           // tokens a row shares (their partial results are in part_*), or null
     const float *part_o, *part_ml; // [units, part_rows, head_dim] and [units, part_rows, 2]
-    const int4* part_at;           // per row: the first unit of kv head 0, units a kv head, the row's place among its tile's rows
+    const int4* part_at;           // per row: the first unit of kv head 0, units a kv head, where the row's heads start among a unit's part_rows
     int part_rows, table_stride, heads, kv_heads, head_dim, pages, page_size, box, window, splits;
     float scale_log2;
 };
@@ -181,7 +186,7 @@ __device__ __forceinline__ float column_sum(float v) {
 }
 
 // A computing warp's walk over tiles [first, last); leaves its sums over the tiles' memory: [warp][8][D_PAD] floats and
-// [warp][8][2] (maximum in log2 units, sum), once every warp is done with the tiles.
+// [warp][g][2] (maximum in log2 units, sum), once every warp is done with the tiles.
 template <int D_PAD, bool KV8>
 __device__ __forceinline__ void walk(unsigned char* smem, uint32_t base, const RowsArgs& a, const bf16* q, int g, int first, int last, int lo, int n) {
     using T = Tile<D_PAD, KV8>;
@@ -324,34 +329,39 @@ __device__ __forceinline__ void walk(unsigned char* smem, uint32_t base, const R
             if (KV8) *(float2*)(to + 2 * r) = make_float2(o[i][h], o[i][2 + h]);
             else { to[r] = o[i][h]; to[8 + r] = o[i][2 + h]; }
         }
-    if (r == 0) {
-        float* ml = wo + AR_WARPS * AR_HEADS * D_PAD + (warp * AR_HEADS + 2 * c) * 2;
-        *(float4*)ml = make_float4(m[0], l[0], m[1], l[1]);
-    }
+    if (r == 0)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            if (2 * c + h < g) *(float2*)(wo + AR_WARPS * AR_HEADS * D_PAD + (warp * g + 2 * c + h) * 2) = make_float2(m[h], l[h]);
 }
 
-// A running merge of partial results (maximum in log2 units, sum, weighted sum of one column), in the order of the calls.
-struct Merge {
-    float m = -INFINITY, l = 0.f, o = 0.f;
-    __device__ __forceinline__ void add(float mi, float li, float oi) {
-        if (mi == -INFINITY && li == 0.f) return;                   // (nothing seen; a sum that is no number stays one)
-        const float top = fmaxf(m, mi), f = m == top ? 1.f : ex2(m - top), w = mi == top ? 1.f : ex2(mi - top);
-        m = top; l = l * f + li * w; o = o * f + oi * w;
-    }
-};
-
-// The result of one column of a head: what the splits left, the shared keys' partial results, the sink.
-__device__ __forceinline__ float finished(Merge x, const RowsArgs& a, int b, int hk, int in_group, int d, bool shares) {
-    const int group = a.heads / a.kv_heads;
-    if (shares) {
-        const int4 at = a.part_at[b];
-        for (int s = 0; s < at.y; ++s) {
-            const size_t slot = (size_t)(at.x + hk * at.y + s) * a.part_rows + at.z * group + in_group;
-            x.add(a.part_ml[slot * 2], a.part_ml[slot * 2 + 1], a.part_o[slot * a.head_dim + d]);
+// How `pieces` partial results [pieces][g][2] (maximum in log2 units, sum) of each of g heads, and the `parts` ones of the shared keys
+// that start at `part` (a head's are `stride` floats apart from split to split, neighbouring heads' lie side by side), are weighed:
+// weights to w [g][pieces + parts], maximum and sum of the whole to whole [g][2]. A warp takes a head; no piece's order matters to
+// the maximum, and the sums' order depends on the numbers alone.
+__device__ __forceinline__ void weigh(float* w, float* whole, const float* ml, int pieces, int g, const float* part, size_t stride, int parts) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, count = pieces + parts;
+    for (int r = warp; r < g; r += AR_THREADS / 32) {
+        float top = -INFINITY;
+        for (int i = lane; i < count; i += 32) {
+            const float m = i < pieces ? ml[(i * g + r) * 2] : part[(i - pieces) * stride + r * 2];
+            w[r * count + i] = m;                                    // (its own lane reads it again)
+            top = fmaxf(top, m);
         }
+        top = warp_max(top);
+        const float off = top == -INFINITY ? 0.f : top;
+        float sum = 0.f;
+        for (int i = lane; i < count; i += 32) {
+            const float l = i < pieces ? ml[(i * g + r) * 2 + 1] : part[(i - pieces) * stride + r * 2 + 1], f = ex2(w[r * count + i] - off);
+            w[r * count + i] = f;
+            sum = fmaf(l, f, sum);                                   // (a sum that is no number stays one)
+        }
+        sum = warp_sum(sum);
+        if (lane == 0) { whole[2 * r] = top; whole[2 * r + 1] = sum; }
     }
-    if (a.sinks && x.l > 0.f) x.l += ex2(fmaf(a.sinks[hk * group + in_group], 1.4426950408889634f, -x.m));   // the sink: a weight without a value
-    return x.l > 0.f || x.l != x.l ? x.o / x.l : 0.f;               // (a sum that is no number gives none)
+}
+__device__ __forceinline__ void add4(float4& x, float w, const float4& y) {
+    x.x = fmaf(w, y.x, x.x); x.y = fmaf(w, y.y, x.y); x.z = fmaf(w, y.z, x.z); x.w = fmaf(w, y.w, x.w);
 }
 
 // grid (rows, kv_heads * ceil(group / 8), splits), a cluster along z.
@@ -385,46 +395,64 @@ __global__ void __launch_bounds__(AR_THREADS, D_PAD > 128 ? 1 : 3) rows_kernel(c
     else
         walk<D_PAD, KV8>(smem, base, a, a.q + ((size_t)t * a.heads + hk * group + g0) * a.head_dim, g, first, last, lo, n);
     __syncthreads();
-    const float* wo = (const float*)smem;
+    // What the four warps left becomes one result a head, or, in a cluster, goes to the CTAs that combine it: each takes a share of
+    // the numbers of all splits. The shared keys' partial results join the last step, and the sink.
+    const float* wo = (const float*)smem;                           // [warp][8][D_PAD], then [warp][g][2]
     const float* wml = wo + AR_WARPS * AR_HEADS * D_PAD;
-    const int total = g * a.head_dim, share = (total + splits - 1) / splits;
-    bf16* out = a.out + ((size_t)t * a.heads + hk * group + g0) * a.head_dim;
+    float* weights = (float*)(smem + T::SUMS);
+    float* whole = (float*)(smem + T::BODY);                        // [8][2], over the scales, which are done
     float* recv_o = (float*)(smem + T::RECV);                       // [splits][share], then [splits][g][2]: what the others send
+    const int total = g * a.head_dim, share = ((total + splits - 1) / splits + 3) & ~3;
     float* recv_ml = recv_o + splits * share;
-    if (cluster) asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");   // every CTA of the cluster runs
-    for (int i = threadIdx.x; i < total; i += AR_THREADS) {
-        const int r = i / a.head_dim, d = i - r * a.head_dim;
-        Merge x;
+    bf16* out = a.out + ((size_t)t * a.heads + hk * group + g0) * a.head_dim;
+    int4 at = make_int4(0, 0, 0, 0);
+    if (shared > 0) at = a.part_at[b];
+    const size_t slot = (size_t)(at.x + hk * at.y) * a.part_rows + at.z + g0;
+    const float* part_ml = shared > 0 ? a.part_ml + slot * 2 : nullptr;
+    const float* part_o = shared > 0 ? a.part_o + slot * a.head_dim : nullptr;
+    const size_t stride = (size_t)a.part_rows * a.head_dim;         // from one split's partial results to the next
+    if (cluster) {
+        weigh(weights, whole, wml, AR_WARPS, g, nullptr, 0, 0);
+        __syncthreads();
+        asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");   // every CTA of the cluster runs
+        for (int i = threadIdx.x * 4; i < total; i += AR_THREADS * 4) {
+            const int r = i / a.head_dim, d = i - r * a.head_dim, peer = i / share;
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int w = 0; w < AR_WARPS; ++w) x.add(wml[(w * AR_HEADS + r) * 2], wml[(w * AR_HEADS + r) * 2 + 1], wo[(w * AR_HEADS + r) * D_PAD + d]);
-        if (!cluster) {
-            out[i] = __float2bfloat16_rn(finished(x, a, b, hk, g0 + r, d, shared > 0));
-            continue;
+            for (int w = 0; w < AR_WARPS; ++w) add4(x, weights[r * AR_WARPS + w], *(const float4*)(wo + (w * AR_HEADS + r) * D_PAD + d));
+            st_cluster_f32x4(recv_o + split * share + (i - peer * share), peer, x);
         }
-        const int peer = i / share;                                 // the CTA that combines this number
-        st_cluster_f32(recv_o + split * share + (i - peer * share), peer, x.o);
-        if (d == 0)
-            for (int p = 0; p < splits; ++p) {
-                st_cluster_f32(recv_ml + (split * g + r) * 2, p, x.m);
-                st_cluster_f32(recv_ml + (split * g + r) * 2 + 1, p, x.l);
-            }
+        for (int i = threadIdx.x; i < splits * g; i += AR_THREADS) {
+            const int peer = i / g, r = i - peer * g;
+            st_cluster_f32(recv_ml + (split * g + r) * 2, peer, whole[2 * r]);
+            st_cluster_f32(recv_ml + (split * g + r) * 2 + 1, peer, whole[2 * r + 1]);
+        }
+        __syncwarp();
+        cluster_barrier();                                          // everything sent has arrived; nobody reads another's memory after it
     }
-    if (!cluster) return;
-    __syncwarp();
-    cluster_barrier();                                              // everything sent has arrived; nobody reads another's memory after it
-    for (int i = threadIdx.x; i < share; i += AR_THREADS) {
-        const int e = split * share + i;
-        if (e >= total) break;
-        const int r = e / a.head_dim, d = e - r * a.head_dim;
-        Merge x;
-        for (int p = 0; p < splits; ++p) x.add(recv_ml[(p * g + r) * 2], recv_ml[(p * g + r) * 2 + 1], recv_o[p * share + i]);
-        out[e] = __float2bfloat16_rn(finished(x, a, b, hk, g0 + r, d, shared > 0));
+    const int pieces = cluster ? splits : AR_WARPS, count = pieces + at.y;
+    weigh(weights, whole, cluster ? recv_ml : wml, pieces, g, part_ml, (size_t)a.part_rows * 2, at.y);
+    __syncthreads();
+    const int from = cluster ? split * share : 0, upto = cluster ? min(total, from + share) : total;
+    for (int i = from + threadIdx.x * 4; i < upto; i += AR_THREADS * 4) {
+        const int r = i / a.head_dim, d = i - r * a.head_dim;
+        const float* w = weights + r * count;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int p = 0; p < pieces; ++p)
+            add4(x, w[p], *(const float4*)(cluster ? recv_o + p * share + (i - from) : wo + (p * AR_HEADS + r) * D_PAD + d));
+#pragma unroll 8
+        for (int p = 0; p < at.y; ++p) add4(x, w[pieces + p], *(const float4*)(part_o + p * stride + i));
+        float l = whole[2 * r + 1];
+        if (a.sinks && l > 0.f) l += ex2(fmaf(a.sinks[hk * group + g0 + r], 1.4426950408889634f, -whole[2 * r]));   // the sink: a weight without a value
+        const float inv = l > 0.f || l != l ? 1.f / l : 0.f;        // (a sum that is no number gives none)
+        const uint2 v = make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
+        *(uint2*)(out + i) = l > 0.f || l != l ? v : make_uint2(0u, 0u);
     }
 }
 
 template <int D_PAD, bool KV8> static size_t rows_smem(int splits, int group, int head_dim) {
     const int g = group < AR_HEADS ? group : AR_HEADS;
-    const size_t recv = splits > 1 ? (size_t)(g * head_dim + splits + splits * g * 2) * 4 : 0;      // (a share is rounded up)
+    const size_t recv = splits > 1 ? (size_t)(g * head_dim + 4 * splits + splits * g * 2) * 4 : 0;  // (a share is rounded up)
     return Tile<D_PAD, KV8>::RECV + recv + 1024;                    // (and the way to a boundary of 1,024 bytes)
 }
 
@@ -503,7 +531,7 @@ extern "C" int hb_attention_rows(void* out, const void* q, const void* kv, int k
     const int group = heads / kv_heads;
     if ((long)kv_heads * ((group + AR_HEADS - 1) / AR_HEADS) > 65535) HB_REFUSE("attention_rows: %d heads", heads);
     if (pages < 1 || (long)pages * 2 * kv_heads > 0x7ffffffel) HB_REFUSE("attention_rows: %d pages of %d kv heads", pages, kv_heads);
-    if (((uintptr_t)kv % 16) || ((uintptr_t)q % 8)) HB_REFUSE("attention_rows: the cache must start on 16 bytes, q on 8");
+    if (((uintptr_t)kv % 16) || (((uintptr_t)q | (uintptr_t)out) % 8)) HB_REFUSE("attention_rows: the cache must start on 16 bytes, q and out on 8");
     if (skip && (!part_o || !part_ml || !part_at || window > 0)) HB_REFUSE("attention_rows: shared keys need their partial results, and no window");
     RowsArgs a = {(bf16*)out, (const bf16*)q, (const unsigned char*)kv, block_table, row_slot, query_start, kv_len, sinks, skip, part_o,
                   part_ml, (const int4*)part_at, part_rows, table_stride, heads, kv_heads, head_dim, pages, page_size, 0, window, splits,

@@ -654,13 +654,17 @@ class CudaKernels:
 
     def _shares(self, heads: int, kv_heads: int, head_dim: int, kv, q, out) -> bool:
         """Whether the kernels for shared beginnings take these sizes (other sizes attend row by row)."""
-        return head_dim % 16 == 0 and head_dim <= 256 and kv.shape[3] % 16 == 0 and heads // kv_heads <= self._prefix_rows() \
+        return kv.shape[3] % 16 == 0 and self._prefix_plan(heads // kv_heads, head_dim, kv.shape[3])[0] > 0 \
             and not (kv.data_ptr() | q.data_ptr()) % 16 and out.data_ptr() % 8 == 0
 
-    def _prefix_rows(self) -> int:
-        key = ("prefix rows",)
+    def _prefix_plan(self, group: int, head_dim: int, page_size: int) -> tuple[int, int, int]:
+        """(CTAs of the kernel for shared keys, query rows a piece of its work leaves results for, rows of the step a tile holds);
+        no CTAs where it does not take the sizes."""
+        key = ("prefix plan", group, head_dim, page_size)
         if key not in self._splits:
-            self._splits[key] = int(self.lib.hb_attention_prefix_rows())
+            part, tile = ctypes.c_int(0), ctypes.c_int(0)
+            per_sm = int(self.lib.hb_attention_prefix_plan(head_dim, page_size, group, ctypes.byref(part), ctypes.byref(tile)))
+            self._splits[key] = (per_sm * self.sms, part.value, tile.value)
         return self._splits[key]
 
     def _attention_rows(self, out, q, kv, common, rows, kv_heads: int, page_size: int, scale, window: int, sinks, shared) -> None:
@@ -669,16 +673,15 @@ class CudaKernels:
         part = (None, None, None, None, 0)
         longest = rows.max_kv
         if shared is not None:
-            tile, ctas = self._prefix_rows(), self.sms * self.PREFIX_CTAS
-            units = self._prefix_units(n, heads, kv_heads)
-            floats = units * tile * (head_dim + 2)
-            scratch = torch.empty(self.shared_scratch(n, heads, kv_heads, head_dim), dtype=torch.float32, device=self.device)
-            at = scratch.data_ptr()
-            part_o, part_ml, part_at = (ctypes.c_void_p(at + 4 * i) for i in (0, units * tile * head_dim, floats))
+            ctas, part_rows, _ = self._prefix_plan(heads // kv_heads, head_dim, page_size)
+            rows_left = self._prefix_units(n, heads, kv_heads, head_dim, page_size) * part_rows
+            scratch = torch.empty(rows_left * (head_dim + 2) + 4 * n, dtype=torch.float32, device=self.device)
+            part_o, part_ml, part_at = (ctypes.c_void_p(scratch.data_ptr() + 4 * i)
+                                        for i in (0, rows_left * head_dim, rows_left * (head_dim + 2)))
             self._call("hb_attention_prefix", part_o, part_ml, part_at, self._p(q), self._p(kv), kv8, *common[:4], self._p(shared.members),
                        self._p(shared.groups), shared.groups.shape[0] // 3, heads, kv_heads, head_dim, kv.shape[0], page_size,
                        ctypes.c_float(scale), ctas)
-            part = (self._p(shared.skip), part_o, part_ml, part_at, tile)
+            part = (self._p(shared.skip), part_o, part_ml, part_at, part_rows)
             longest = shared.longest_own
         if window > 0:
             longest = min(longest, window)
@@ -686,17 +689,16 @@ class CudaKernels:
         self._call("hb_attention_rows", self._p(out), self._p(q), self._p(kv), kv8, *common, n, heads, kv_heads, head_dim, kv.shape[0],
                    page_size, ctypes.c_float(scale), window, splits, self._p(sinks), *part)
 
-    PREFIX_CTAS = 2                           # CTAs an SM of the kernel for shared keys
-
-    def _prefix_units(self, rows: int, heads: int, kv_heads: int) -> int:
+    def _prefix_units(self, rows: int, heads: int, kv_heads: int, head_dim: int, page_size: int) -> int:
         """Partial results that `rows` one-token rows may leave at most for what they share, whatever their groups are: a tile for
         every so many rows that fill one, and one more for each group."""
-        per_tile = max(1, self._prefix_rows() // (heads // kv_heads))
-        return max(self.sms * self.PREFIX_CTAS, kv_heads * (rows // per_tile + rows // 2))
+        ctas, _, tile_rows = self._prefix_plan(heads // kv_heads, head_dim, page_size)
+        return max(ctas, kv_heads * (rows // tile_rows + rows // 2))
 
-    def shared_scratch(self, rows: int, heads: int, kv_heads: int, head_dim: int) -> int:
+    def shared_scratch(self, rows: int, heads: int, kv_heads: int, head_dim: int, page_size: int) -> int:
         """32-bit words of scratch for what `rows` one-token rows share."""
-        return self._prefix_units(rows, heads, kv_heads) * self._prefix_rows() * (head_dim + 2) + 4 * rows
+        ctas, part_rows, _ = self._prefix_plan(heads // kv_heads, head_dim, page_size)
+        return self._prefix_units(rows, heads, kv_heads, head_dim, page_size) * part_rows * (head_dim + 2) + 4 * rows if ctas else 0
 
     def _row_splits(self, kv8: int, rows: int, heads: int, kv_heads: int, head_dim: int, longest: int) -> int:
         """Into how many CTAs (a cluster) the keys of a one-token row are cut: the number with the least waves x (64-key tiles a

@@ -101,7 +101,7 @@ class GQA(Part):
         if self.fp8:                                                 # (a captured step reads all its portions back at once)
             bytes_ += portions * -(-longest // page_size) * page_size * 4 * self.kv_heads * self.head_dim
         if self.ctx.shared_prefix and hasattr(k, "shared_scratch"):
-            bytes_ += 4 * k.shared_scratch(rows, self.heads, self.kv_heads, self.head_dim)
+            bytes_ += 4 * k.shared_scratch(rows, self.heads, self.kv_heads, self.head_dim, page_size)
         return bytes_
 
     @property

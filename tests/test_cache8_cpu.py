@@ -187,7 +187,11 @@ class Noted(CudaKernels):
     def __init__(self):
         self.device, self.called, self._pending, self._splits, self.sms = torch.device("cpu"), [], [], {}, 148
         self.prefill_attention, self.prefill_tile, self.attention_bf16 = "tcgen05", None, "fast"
-        self.lib = types.SimpleNamespace(hb_attention_prefix_rows=lambda: 64, hb_attention_rows_capacity=lambda kv8, dim, group, s: 3 if s == 1 else 400 // s)
+        self.lib = types.SimpleNamespace(hb_attention_prefix_plan=self.plan, hb_attention_rows_capacity=lambda kv8, dim, group, s: 3 if s == 1 else 400 // s)
+
+    def plan(self, dim, page, group, part_rows, tile_rows):
+        part_rows._obj.value, tile_rows._obj.value = 64, 64 // group
+        return 2 if group <= 64 else 0
 
     def _check(self, *tensors):
         assert all(t is None or t.is_contiguous() for t in tensors)
@@ -239,4 +243,5 @@ def test_a_captured_step_is_planned_for_a_bucket_of_own_keys():
     shared = SharedPrefix(None, None, None, 2, 70)
     plan = k.attention_capture_plan(rows, 4096)
     assert len(plan) == 2 and k.attention_capture_plan(rows, 4096, shared) == (*plan, 128) and shared.longest_own == 128
-    assert k._prefix_units(64, 32, 8) == max(148 * k.PREFIX_CTAS, 8 * (4 + 32)) and k.shared_scratch(1, 32, 8, 128) > 0
+    assert k._prefix_units(64, 32, 8, 128, 64) == max(148 * 2, 8 * (4 + 32)) and k._prefix_units(256, 32, 8, 128, 64) == 8 * (16 + 128)
+    assert k.shared_scratch(1, 32, 8, 128, 64) == 296 * 64 * 130 + 4 and k.shared_scratch(1, 130, 1, 128, 64) == 0

@@ -57,7 +57,7 @@ def run(K, q, kv, table, rows, scale, sinks, shared):
     return out
 
 
-CASES = [([(16, [1, 130, 64, 3])], [], 16, 8, 128, 64), ([(5, [9, 70]), (33, [1, 200, 500])], [77, 3], 8, 2, 128, 64),
+CASES = [([(16, [1, 130, 64, 3])], [], 16, 8, 128, 64), ([(9, [7] * 70), (3, [80] * 9)], [4], 12, 2, 128, 64), ([(5, [3] * 3)], [9], 100, 1, 128, 128), ([(5, [9, 70]), (33, [1, 200, 500])], [77, 3], 8, 2, 128, 64),
          ([(30, [1 + 7 * i for i in range(40)])], [5], 4, 1, 96, 16), ([(4, [5] * 17), (9, [300] * 3), (2, [1] * 130)], [1], 6, 2, 64, 128),
          ([(6, [90] * 3)], [200], 5, 5, 80, 64), ([(7, [11] * 70)], [], 2, 1, 256, 80), ([(3, [40, 50])], [], 48, 1, 32, 128),
          ([(40, [20] * 6)], [30] * 3, 128, 2, 128, 16)]
@@ -87,17 +87,18 @@ def test_beside_a_portion(K, page, fp8):
 @pytest.mark.parametrize("fp8", [True, False])
 def test_more_tiles_than_ctas(K, fp8, monkeypatch):
     """Units in turns: fewer CTAs than there are pieces of work, and one CTA for all."""
-    monkeypatch.setattr(K, "PREFIX_CTAS", 1, raising=False)
-    for sms in (7, 1):
-        monkeypatch.setattr(K, "sms", sms, raising=False)
-        q, kv, table, rows, shared = case([(6, [9] * 9), (11, [30] * 5), (5, [2, 2])], [5], 32, 2, 128, 64, fp8, seed=1)
+    plan = K._prefix_plan
+    for ctas, dim, page in ((7, 128, 64), (1, 128, 64), (7, 64, 16), (1, 80, 64)):
+        monkeypatch.setattr(K, "_prefix_plan", lambda *a: (ctas, *plan(*a)[1:]), raising=False)
+        q, kv, table, rows, shared = case([(6 * 64 // page, [9] * 9), (11 * 64 // page, [30] * 5), (5 * 64 // page, [2, 2])], [5], 32, 2, dim, page,
+                                          fp8, seed=1)
         want, mass = c8.attend(q, kv, table, rows, 0.1)
         within(run(K, q, kv, table, rows, 0.1, None, shared), want, mass)
 
 
 def test_sizes_that_the_shared_kernels_do_not_take(K):
     """Such rows attend by themselves, sharing or not."""
-    q, kv, table, rows, shared = case([(6, [9] * 3)], [], 72, 1, 128, 64, False)         # (72 heads a kv head)
+    q, kv, table, rows, shared = case([(6, [9] * 3)], [], 72, 1, 64, 64, False)          # (72 heads a kv head)
     want, mass = c8.attend(q, kv, table, rows, 0.1)
     within(run(K, q, kv, table, rows, 0.1, None, shared), want, mass)
     with pytest.raises(KernelError):
