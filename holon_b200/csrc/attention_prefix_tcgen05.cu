@@ -6,12 +6,11 @@
 // operands in shared memory, S in one of two 64-column buffers of tensor memory); softmax with a query row a thread, the weights go back
 // over the S they came from; O += P V (128 x 128 x 16, four products, P from tensor memory). The running maximum may lag by 2^8
 // before O is rescaled. No key is masked: shared pages are whole, and whole numbers of 64 keys.
-// bfloat16 pages: keys and values come by TMA as the products want them. 8-bit pages: TMA brings the codes, two warps turn them
-// into halves (exactly) in the same layout, and the softmax applies the rows' scales as attention_rows.cu does: u = s 2^(a + c) scale
-// log2(e) + b, weights 2^(u - M) times 2^7 so that with the lag they stay below a half's largest, sums with 2^-b.
+// bfloat16 pages: keys and values come by TMA as the products want them. 8-bit pages: TMA brings the codes, and four warps turn them
+// into bfloat16, scale and all (exactly), in the same layout: six instructions for two codes, where halves without the scale would be one
+// and leave the scales to the softmax (a factor and a term a score, a factor a weight: as many instructions once there are
+// 128 query rows, and registers that it does not have).
 // Barriers keep their phases from unit to unit; every role counts the tiles that it has seen.
-#include <cuda_fp16.h>
-
 #include "cache8.cuh"
 #include "prefix_units.cuh"
 #include "tcgen05.cuh"
@@ -26,18 +25,16 @@
 #define PT_RAW_STAGE (2 * PT_RAW_BYTES + 1024)    // keys, values, 64 + 64 scale bytes
 #define PT_TMEM_COLS 512                          // per group: S0 [0, 64), S1 [64, 128), O [128, 256)
 #define PT_RESCALE 8.0f
-#define PT_BIAS 7.0f                              // 8-bit pages: what the weights are raised by
-#define PT_MMA_WARP1 10                           // warps 10, 11: the groups' P V; 2 - 9: softmax; 0: loads; 1: Q K^T; 12, 13: codes to halves
-#define PT_CONVERTERS 2
+#define PT_MMA_WARP1 10                           // warps 10, 11: the groups' P V; 2 - 9: softmax; 0: loads; 1: Q K^T; 12 - 15: codes to bfloat16
+#define PT_CONVERTERS 4
 
 template <bool KV8> struct Shape {
-    static constexpr int THREADS = KV8 ? 448 : 384;
-    static constexpr int STAGES = KV8 ? 2 : 3;    // of keys and values as the products read them
-    static constexpr int RAW = KV8 ? 4 : 1;       // of codes (bfloat16: none, and no barrier of theirs is used)
-    static constexpr int KV = PT_GROUPS * PT_Q_BYTES, RAWS = KV + STAGES * 2 * PT_KV_BYTES, SCALES = RAWS + (KV8 ? RAW * PT_RAW_STAGE : 0);
-    static constexpr int UP = SCALES + (KV8 ? STAGES * 3 * PT_BN * 4 : 0);           // [256] floats: what undoes a query's scale
-    static constexpr int BARS = UP + (KV8 ? PT_GROUPS * PT_BM * 4 : 0);
-    static constexpr int SMEM = BARS + 512 + 1024;
+    static constexpr int THREADS = KV8 ? 512 : 384;
+    static constexpr int STAGES = 3;              // of keys and values as the products read them
+    static constexpr int RAW = KV8 ? 3 : 1;       // of codes (bfloat16: none, and no barrier of theirs is used)
+    static constexpr int KV = PT_GROUPS * PT_Q_BYTES, RAWS = KV + STAGES * 2 * PT_KV_BYTES;
+    static constexpr int BARS = RAWS + (KV8 ? RAW * PT_RAW_STAGE : 0);
+    static constexpr int SMEM = BARS + 256 + 1024;
 };
 
 struct PrefixTcArgs {
@@ -45,7 +42,7 @@ struct PrefixTcArgs {
     int4* part_at;
     const bf16* q;
     const unsigned char* kv;
-    const int32_t *block_table, *row_slot, *query_start, *members, *groups;
+    const int32_t *block_table, *row_slot, *members, *groups;
     int n_groups, table_stride, heads, kv_heads, pages, page_size;
     float scale_log2;
 };
@@ -53,11 +50,6 @@ struct PrefixTcArgs {
 __device__ __forceinline__ void pt_bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n"
                  ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t d;
-    asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
-    return d;
 }
 __device__ __forceinline__ void st_shared16(uint32_t at, const uint4& v) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
@@ -68,48 +60,19 @@ __device__ __forceinline__ uint4 ld_shared16(uint32_t at) {
     return v;
 }
 
-// The tile's queries, row by row (eight lanes a row): group g's row r is head r % group of the tile's row g * per_group + r / group.
-// Rows without a query are zeros. 8-bit pages: as halves, each row divided by a power of two that brings its largest number near 2^6.
-template <bool KV8>
-__device__ __forceinline__ void load_queries(unsigned char* smem, uint32_t q_s, const PrefixTcArgs& a, const PrefixUnit& u, int group, int per_group) {
-    const int sub = threadIdx.x & 7;
-    for (int i = threadIdx.x >> 3; i < PT_GROUPS * PT_BM; i += Shape<KV8>::THREADS / 8) {
-        const int g = i / PT_BM, r = i % PT_BM, row = g * per_group + r / group;
-        const bool live = r < per_group * group && row < u.count;
-        uint4 x = make_uint4(0, 0, 0, 0), y = x;
-        if (live) {
-            const bf16* src = a.q + ((size_t)a.query_start[a.members[u.start + row]] * a.heads + u.hk * group + r % group) * PT_D;
-            x = *(const uint4*)(src + sub * 8);
-            y = *(const uint4*)(src + 64 + sub * 8);
-        }
-        if (KV8) {
-            uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-            float m = 0.f;
+// One query row `src` (null: zeros) into row r of a group's operand.
+__device__ __forceinline__ void load_query(uint32_t q_s, const bf16* src, int r) {
+    uint4 x[PT_D / 8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const float2 v = __bfloat1622float2(*(const __nv_bfloat162*)&w[k]);
-                m = fmaxf(m, fmaxf(c8_magnitude(v.x), c8_magnitude(v.y)));
-            }
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
-            const int e = min(max((int)(__float_as_uint(m) >> 23) - 127 - 6, -100), 121);
-            const float down = c8_power(-e);
+    for (int c = 0; c < PT_D / 8; ++c) x[c] = src ? ((const uint4*)src)[c] : make_uint4(0, 0, 0, 0);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const float2 v = __bfloat1622float2(*(const __nv_bfloat162*)&w[k]);
-                const __half2 h = __floats2half2_rn(v.x * down, v.y * down);
-                w[k] = *(const uint32_t*)&h;
-            }
-            x = make_uint4(w[0], w[1], w[2], w[3]);
-            y = make_uint4(w[4], w[5], w[6], w[7]);
-            if (sub == 0) ((float*)(smem + Shape<KV8>::UP))[i] = c8_power(e);
-        }
-        const uint32_t at = q_s + g * PT_Q_BYTES + r * 128 + ((sub ^ (r & 7)) << 4);
-        st_shared16(at, x);
-        st_shared16(at + PT_Q_BYTES / 2, y);
-    }
+    for (int c = 0; c < PT_D / 8; ++c)                                // (eight rows at one chunk: eight groups of banks)
+        st_shared16(q_s + (c >> 3) * (PT_Q_BYTES / 2) + r * 128 + (((c & 7) ^ (r & 7)) << 4), x[c]);
     fence_async_smem();                                               // (the products read them through the async proxy)
+}
+__device__ __forceinline__ void st_global32(float* dst, const uint32_t* v) {      // 32 bytes: a whole sector a thread
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n"
+                 ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
 }
 
 template <bool KV8>
@@ -121,41 +84,42 @@ __global__ void __launch_bounds__(Shape<KV8>::THREADS, 1) prefix_tcgen05_kernel(
     const uint32_t q_s = base, kv_s = base + H::KV, bars = base + H::BARS;
     const uint32_t kv_full0 = bars, kv_empty0 = kv_full0 + 8 * H::STAGES, raw_full0 = kv_empty0 + 8 * H::STAGES, raw_empty0 = raw_full0 + 8 * H::RAW;
     // per group g and buffer i, at index (g * 2 + i): scores computed; weights written; weights read (O holds the tile)
-    const uint32_t s_full0 = raw_empty0 + 8 * H::RAW, p_full0 = s_full0 + 32, p_empty0 = p_full0 + 32, o_full0 = p_empty0 + 32, slot = o_full0 + 16;
+    const uint32_t s_full0 = raw_empty0 + 8 * H::RAW, p_full0 = s_full0 + 32, p_empty0 = p_full0 + 32, o_full0 = p_empty0 + 32, q_full = o_full0 + 16, slot = q_full + 8;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int group = a.heads / a.kv_heads, per_group = PT_BM / group, per_tile = PT_GROUPS * per_group;
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");   // (attention_rows.cu may begin with the rows' own keys)
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < H::STAGES; ++s) { mbar_init(kv_full0 + 8 * s, KV8 ? PT_CONVERTERS : 1); mbar_init(kv_empty0 + 8 * s, 1 + PT_GROUPS); }
         for (int s = 0; s < H::RAW; ++s) { mbar_init(raw_full0 + 8 * s, 1); mbar_init(raw_empty0 + 8 * s, PT_CONVERTERS); }
         for (int i = 0; i < 2 * PT_GROUPS; ++i) { mbar_init(s_full0 + 8 * i, 1); mbar_init(p_full0 + 8 * i, 4); mbar_init(p_empty0 + 8 * i, 1); }
         for (int g = 0; g < PT_GROUPS; ++g) mbar_init(o_full0 + 8 * g, 1);
+        mbar_init(q_full, 4 * PT_GROUPS);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(slot), "r"(PT_TMEM_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
     }
-    const PrefixUnits all = prefix_units(a.groups, a.n_groups, per_tile, a.kv_heads, gridDim.x);
+    const PrefixGroups known(a.groups, a.n_groups, per_tile);
+    const PrefixUnits all = prefix_units(known, a.kv_heads, gridDim.x);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     uint32_t tmem;
     asm volatile("ld.shared.b32 %0, [%1];\n" : "=r"(tmem) : "r"(slot));
 
-    int seen = 0, g_seen[PT_GROUPS] = {0, 0}, g_units[PT_GROUPS] = {0, 0};       // tiles before this unit: of all, of a group's own; its units
+    int seen = 0, turn = 0, g_seen[PT_GROUPS] = {0, 0}, g_units[PT_GROUPS] = {0, 0};   // tiles and units before this one: of all, of a group's own
     bool ok = true;
-    for (int w = blockIdx.x; w < all.units; w += gridDim.x) {
-        const PrefixUnit u = prefix_unit(a.groups, a.n_groups, per_tile, a.kv_heads, all.chunk, w);
-        const int first = u.split * all.chunk, tiles = min(u.tokens / PT_BN, first + all.chunk) - first;
+    for (int w = blockIdx.x; w < all.units; w += gridDim.x, ++turn) {
+        const PrefixUnit u = prefix_unit(known, a.kv_heads, all.chunk, w);
+        const int first = u.split * all.chunk, tiles = min(u.blocks, first + all.chunk) - first;
         int g_rows[PT_GROUPS];                                        // query rows of each group
 #pragma unroll
         for (int g = 0; g < PT_GROUPS; ++g) g_rows[g] = max(0, min(per_group, u.count - g * per_group)) * group;
         if (warp == 0 && u.hk == 0 && u.split == 0)
             for (int i = lane; i < u.count; i += 32)
                 a.part_at[a.members[u.start + i]] = make_int4(u.first, u.splits, i / per_group * PT_BM + i % per_group * group, 0);
-        load_queries<KV8>(smem, q_s, a, u, group, per_group);
-        __syncthreads();
 
         if (warp == 0) {
             const int32_t* table = a.block_table + (size_t)a.row_slot[a.members[u.start]] * a.table_stride;
@@ -168,8 +132,8 @@ __global__ void __launch_bounds__(Shape<KV8>::THREADS, 1) prefix_tcgen05_kernel(
                 const size_t bytes = (size_t)a.page_size * (PT_D + 1);
                 const unsigned char* k_scale = a.kv + (size_t)(there ? k_block : u.hk) * bytes + (size_t)a.page_size * PT_D + in;
                 for (int i = 0; i < 32 && t0 + i < tiles; ++i) {
-                    const int n = seen + t0 + i, s = n % (KV8 ? H::RAW : H::STAGES), turn = n / (KV8 ? H::RAW : H::STAGES);
-                    ok = __all_sync(0xffffffffu, mbar_wait((KV8 ? raw_empty0 : kv_empty0) + 8 * s, (turn & 1) ^ 1, 1));
+                    const int n = seen + t0 + i, s = n % (KV8 ? H::RAW : H::STAGES), round = n / (KV8 ? H::RAW : H::STAGES);
+                    ok = __all_sync(0xffffffffu, mbar_wait((KV8 ? raw_empty0 : kv_empty0) + 8 * s, (round & 1) ^ 1, 1));
                     if (!ok) break;
                     if (lane != i) continue;
                     if (KV8) {
@@ -197,27 +161,19 @@ __global__ void __launch_bounds__(Shape<KV8>::THREADS, 1) prefix_tcgen05_kernel(
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 const uint32_t raw = base + H::RAWS + s * PT_RAW_STAGE, dst = kv_s + d * 2 * PT_KV_BYTES;
-                float* scales = (float*)(smem + H::SCALES + d * 3 * PT_BN * 4);
-                {
-                    const int key = part * 32 + lane;
-                    const unsigned char* b = smem + H::RAWS + s * PT_RAW_STAGE + 2 * PT_RAW_BYTES + key;
-                    const int kb = min((int)b[0], 254), vb = min(max((int)b[64], C8_LOW + 127), 254);
-                    scales[key] = __uint_as_float((uint32_t)kb << 23);
-                    scales[PT_BN + key] = (float)(vb - 127);
-                    scales[2 * PT_BN + key] = __uint_as_float((uint32_t)(254 - vb) << 23);
-                }
-                // Eight lanes read four chunks of 16 codes of a row and of row ^ 5, and write them as halves: no two of either in one
-                // group of banks. One warp takes the first halves of all rows, the other the second ones.
+                // Eight lanes read four chunks of 16 codes of a row and of row ^ 5, and write them as bfloat16: no two of either in one
+                // group of banks. Warps 0 and 1 take the first halves of keys' and of values' rows, 2 and 3 the second ones.
+                const int ch = (part >> 1) * 4 + (sub & 3), v = part & 1;
+                const unsigned char* scales = smem + H::RAWS + s * PT_RAW_STAGE + 2 * PT_RAW_BYTES + v * PT_BN;
+                const uint32_t to0 = dst + v * PT_KV_BYTES + (part >> 1) * (PT_KV_BYTES / 2);
 #pragma unroll 4
-                for (int i = 0; i < 16; ++i) {
-                    const int row = (i & 7) * 8 + ((lane >> 3) ^ (sub >> 2) * 5), ch = part * 4 + (sub & 3);
-                    const uint32_t from = raw + (i >> 3) * PT_RAW_BYTES + row * 128 + ((ch ^ (row & 7)) << 4);
-                    const uint4 c = ld_shared16(from);
-                    const uint4 lo = make_uint4(c8_halves(c.x), c8_halves(c.x >> 16), c8_halves(c.y), c8_halves(c.y >> 16));
-                    const uint4 hi = make_uint4(c8_halves(c.z), c8_halves(c.z >> 16), c8_halves(c.w), c8_halves(c.w >> 16));
-                    const uint32_t to = dst + (i >> 3) * PT_KV_BYTES + part * (PT_KV_BYTES / 2) + row * 128;
-                    st_shared16(to + (((2 * (ch & 3)) ^ (row & 7)) << 4), lo);
-                    st_shared16(to + (((2 * (ch & 3) + 1) ^ (row & 7)) << 4), hi);
+                for (int i = 0; i < 8; ++i) {
+                    const int row = i * 8 + ((lane >> 3) ^ (sub >> 2) * 5);
+                    const uint4 c = ld_shared16(raw + v * PT_RAW_BYTES + row * 128 + ((ch ^ (row & 7)) << 4));
+                    uint4 lo, hi;
+                    c8_unpack16(c, c8_power(min((int)scales[row], 254) - 127), lo, hi);
+                    st_shared16(to0 + row * 128 + (((2 * (ch & 3)) ^ (row & 7)) << 4), lo);
+                    st_shared16(to0 + row * 128 + (((2 * (ch & 3) + 1) ^ (row & 7)) << 4), hi);
                 }
                 fence_async_smem();
                 __syncwarp();
@@ -225,11 +181,12 @@ __global__ void __launch_bounds__(Shape<KV8>::THREADS, 1) prefix_tcgen05_kernel(
             }
         } else if (warp == 1 || (warp >= PT_MMA_WARP1 && warp < 12)) {
             if (lane == 0) {
-                // kind::f16, D float32, A and B bfloat16 or half; N / 8 at bit 17, M / 16 at bit 24; bit 16: B is MN-major
-                const uint32_t types = (1u << 4) | (KV8 ? 0u : (1u << 7) | (1u << 10));
+                // kind::f16, D float32, A and B bfloat16; N / 8 at bit 17, M / 16 at bit 24; bit 16: B is MN-major
+                const uint32_t types = (1u << 4) | (1u << 7) | (1u << 10);
                 const uint32_t idesc_qk = types | ((uint32_t)(PT_BN >> 3) << 17) | ((uint32_t)(PT_BM >> 4) << 24);
                 const uint32_t idesc_pv = types | (1u << 16) | ((uint32_t)(PT_D >> 3) << 17) | ((uint32_t)(PT_BM >> 4) << 24);
                 if (warp == 1) {
+                    ok = mbar_wait(q_full, turn & 1, 12);
                     for (int j = 0; j < tiles && ok; ++j) {
                         const int n = seen + j, s = n % H::STAGES;
                         ok = mbar_wait(kv_full0 + 8 * s, (n / H::STAGES) & 1, 4);
@@ -283,13 +240,18 @@ __global__ void __launch_bounds__(Shape<KV8>::THREADS, 1) prefix_tcgen05_kernel(
             const uint32_t lane_t = tmem + g * 256 + ((uint32_t)(quarter * 32) << 16);
             const uint32_t o_t = lane_t + 2 * PT_BN;
             float m_used = -INFINITY, l = 0.f;                        // in log2 units; the maximum may lag by PT_RESCALE
-            const float factor = KV8 ? a.scale_log2 * ((const float*)(smem + H::UP))[g * PT_BM + r] : a.scale_log2;
-            const uint64_t factor2 = pack2(factor, factor);
+            if (g_rows[g] > 0) {
+                const bf16* src = nullptr;
+                if (r < g_rows[g]) src = a.q + ((size_t)a.members[u.start + g * per_group + r / group] * a.heads + u.hk * group + r % group) * PT_D;
+                load_query(q_s + g * PT_Q_BYTES, src, r);             // (one-token rows come first: a row's number is its token's)
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full);
+            const uint64_t factor2 = pack2(a.scale_log2, a.scale_log2);
             if (g_rows[g] > 0) {
                 for (int j = 0; j < tiles && ok; ++j) {
                     const int k = g_seen[g] + j, gb = g * 2 + (k & 1);
                     ok = mbar_wait(s_full0 + 8 * gb, (k >> 1) & 1, 8);
-                    if (KV8 && ok) ok = mbar_wait(kv_full0 + 8 * ((seen + j) % H::STAGES), ((seen + j) / H::STAGES) & 1, 9);   // (the scales)
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     tc_fence_after();
@@ -297,28 +259,13 @@ __global__ void __launch_bounds__(Shape<KV8>::THREADS, 1) prefix_tcgen05_kernel(
                     tc_ld32_nowait(lane_t + (k & 1) * PT_BN, sr[0]);
                     tc_ld32_nowait(lane_t + (k & 1) * PT_BN + 32, sr[1]);
                     tc_ld_wait();
-                    const uint32_t scales = base + H::SCALES + ((seen + j) % H::STAGES) * 3 * PT_BN * 4;
-                    if (KV8) {
-#pragma unroll
-                        for (int i = 0; i < PT_BN; i += 4) {
-                            const uint4 ka = ld_shared16(scales + i * 4), vb = ld_shared16(scales + (PT_BN + i) * 4);
-                            uint32_t* x = &sr[i >> 5][i & 31];
-                            float f0, f1;
-                            unpack2(fma2(mul2(pack2(__uint_as_float(x[0]), __uint_as_float(x[1])), pack2(__uint_as_float(ka.x), __uint_as_float(ka.y))),
-                                         factor2, pack2(__uint_as_float(vb.x), __uint_as_float(vb.y))), f0, f1);
-                            x[0] = __float_as_uint(f0); x[1] = __float_as_uint(f1);
-                            unpack2(fma2(mul2(pack2(__uint_as_float(x[2]), __uint_as_float(x[3])), pack2(__uint_as_float(ka.z), __uint_as_float(ka.w))),
-                                         factor2, pack2(__uint_as_float(vb.z), __uint_as_float(vb.w))), f0, f1);
-                            x[2] = __float_as_uint(f0); x[3] = __float_as_uint(f1);
-                        }
-                    }
                     float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};   // four chains instead of one of 64
 #pragma unroll
                     for (int c = 0; c < 2; ++c)
 #pragma unroll
                         for (int i = 0; i < 32; ++i) mx4[i & 3] = fmaxf(mx4[i & 3], __uint_as_float(sr[c][i]));
                     const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-                    const float mt = KV8 ? mx - PT_BIAS : mx * factor;
+                    const float mt = mx * a.scale_log2;
                     const bool grow = mt > m_used + PT_RESCALE || (m_used == -INFINITY && mt > -INFINITY);
                     if (__any_sync(0xffffffffu, grow)) {              // rescale what is summed (whole warp: the TMEM ops are collective)
                         const float m_new = grow ? mt : m_used;
@@ -350,20 +297,12 @@ __global__ void __launch_bounds__(Shape<KV8>::THREADS, 1) prefix_tcgen05_kernel(
                         for (int i = 0; i < 32; i += 2) {
                             float x, y;
                             const uint64_t pair = pack2(__uint_as_float(sr[c][i]), __uint_as_float(sr[c][i + 1]));
-                            unpack2(KV8 ? add2(pair, off2) : fma2(pair, factor2, off2), x, y);
+                            unpack2(fma2(pair, factor2, off2), x, y);
                             x = at_ex2(x);
                             y = at_ex2(y);
-                            if (KV8) {
-                                uint64_t drop;
-                                asm volatile("ld.shared.b64 %0, [%1];\n" : "=l"(drop) : "r"(scales + (2 * PT_BN + c * 32 + i) * 4));
-                                sum2[(i >> 1) & 3] = fma2(pack2(x, y), drop, sum2[(i >> 1) & 3]);
-                                const __half2 h = __floats2half2_rn(x, y);
-                                pk[c * 16 + i / 2] = *(const uint32_t*)&h;
-                            } else {
-                                sum2[(i >> 1) & 3] = add2(sum2[(i >> 1) & 3], pack2(x, y));
-                                const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-                                pk[c * 16 + i / 2] = *(const uint32_t*)&h;
-                            }
+                            sum2[(i >> 1) & 3] = add2(sum2[(i >> 1) & 3], pack2(x, y));
+                            const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+                            pk[c * 16 + i / 2] = *(const uint32_t*)&h;
                         }
                     float lo, hi;
                     unpack2(add2(add2(sum2[0], sum2[1]), add2(sum2[2], sum2[3])), lo, hi);
@@ -385,8 +324,7 @@ __global__ void __launch_bounds__(Shape<KV8>::THREADS, 1) prefix_tcgen05_kernel(
                         tc_ld32(o_t + c * 32, o);
                         if (mine) {
 #pragma unroll
-                            for (int i = 0; i < 32; i += 4)
-                                *(uint4*)(a.part_o + at * PT_D + c * 32 + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                            for (int i = 0; i < 32; i += 8) st_global32(a.part_o + at * PT_D + c * 32 + i, o + i);
                         }
                     }
                     tc_fence_before();
@@ -436,9 +374,9 @@ template <bool KV8> static int launch(const PrefixTcArgs& a, int ctas, cudaStrea
 
 // hb_attention_prefix's work where head_dim is 128 and pages are multiples of 64 tokens (its checks are done).
 int hb_attention_prefix_tcgen05(float* part_o, float* part_ml, int32_t* part_at, const void* q, const void* kv, int kv8, const int32_t* block_table,
-                                int table_stride, const int32_t* row_slot, const int32_t* query_start, const int32_t* members, const int32_t* groups,
+                                int table_stride, const int32_t* row_slot, const int32_t* members, const int32_t* groups,
                                 int n_groups, int heads, int kv_heads, int pages, int page_size, float scale, int ctas, cudaStream_t s) {
-    const PrefixTcArgs a = {part_o, part_ml, (int4*)part_at, (const bf16*)q, (const unsigned char*)kv, block_table, row_slot, query_start, members,
+    const PrefixTcArgs a = {part_o, part_ml, (int4*)part_at, (const bf16*)q, (const unsigned char*)kv, block_table, row_slot, members,
                             groups, n_groups, table_stride, heads, kv_heads, pages, page_size, scale * 1.4426950408889634f};
     return kv8 ? launch<true>(a, ctas, s) : launch<false>(a, ctas, s);
 }

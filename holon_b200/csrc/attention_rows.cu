@@ -29,6 +29,7 @@
 #define AR_THREADS (32 * AR_WARPS + 32)
 #define AR_HEADS 8
 #define AR_BIAS 14.f
+#define AR_BY_LENGTH 1024             // rows up to which a launch may take the longest first
 #ifndef AR_NK
 #define AR_NK(D_PAD, KV8) ((KV8) || (D_PAD) <= 64 ? 2 : 1)
 #define AR_STAGES(BYTES) ((BYTES) <= 16384 ? 4 : (BYTES) <= 32768 ? 3 : 2)
@@ -74,7 +75,7 @@ struct RowsArgs {
     const int32_t* skip;           // tokens a row shares (their partial results are in part_*), or null
     const float *part_o, *part_ml; // [units, part_rows, head_dim] and [units, part_rows, 2]
     const int4* part_at;           // per row: the first unit of kv head 0, units a kv head, where the row's heads start among a unit's part_rows
-    int part_rows, table_stride, heads, kv_heads, head_dim, pages, page_size, box, window, splits;
+    int part_rows, table_stride, rows, heads, kv_heads, head_dim, pages, page_size, page_shift, box, window, splits, by_length;
     float scale_log2;
 };
 
@@ -108,7 +109,7 @@ __device__ __forceinline__ void load_tiles(const CUtensorMap* map, const RowsArg
     const uint32_t bytes = T::STAGE + (KV8 ? 2 * T::KEYS : 0);
     const size_t block = (size_t)a.page_size * (a.head_dim + 1);
     for (int t0 = first; t0 < last; t0 += batch) {
-        const int key = t0 * T::KEYS + lane * a.box, pi = key / a.page_size, in = key - pi * a.page_size;     // this lane's box
+        const int key = t0 * T::KEYS + lane * a.box, pi = a.page_shift >= 0 ? key >> a.page_shift : key / a.page_size, in = key - pi * a.page_size;   // this lane's box
         const int page = lane < batch * boxes && key < n ? table[pi] : -1;
         const bool there = page >= 0 && page < a.pages;
         const int k_block = there ? page * 2 * a.kv_heads + hk : 2 * a.pages * a.kv_heads, v_block = there ? k_block + a.kv_heads : k_block;
@@ -364,7 +365,27 @@ __device__ __forceinline__ void add4(float4& x, float w, const float4& y) {
     x.x = fmaf(w, y.x, x.x); x.y = fmaf(w, y.y, x.y); x.z = fmaf(w, y.z, x.z); x.w = fmaf(w, y.w, x.w);
 }
 
-// grid (rows, kv_heads * ceil(group / 8), splits), a cluster along z.
+// The row whose own keys are `rank` rows' from the longest (of equal ones the first): where CTAs are more than run at once, the long
+// ones start first, and the short ones fill the end of the launch.
+__device__ __forceinline__ int row_by_length(unsigned char* smem, const RowsArgs& a, int rank) {
+    int* own = (int*)smem;                                           // (the tiles' memory, before the first tile comes)
+    __shared__ int found;
+    for (int i = threadIdx.x; i < a.rows; i += AR_THREADS) {
+        const int n = a.kv_len[i], from = max(a.skip ? a.skip[i] : 0, a.window > 0 ? n - a.window : 0);
+        own[i] = n - max(0, from);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.rows; i += AR_THREADS) {
+        const int mine = own[i];
+        int before = 0;
+        for (int j = 0; j < a.rows; ++j) before += own[j] > mine || (own[j] == mine && j < i);
+        if (before == rank) found = i;
+    }
+    __syncthreads();
+    return found;
+}
+
+// grid (kv_heads * ceil(group / 8), rows, splits), a cluster along z.
 template <int D_PAD, bool KV8>
 __global__ void __launch_bounds__(AR_THREADS, D_PAD > 128 ? 1 : 3) rows_kernel(const __grid_constant__ CUtensorMap map, const RowsArgs a) {
     extern __shared__ unsigned char smem_raw[];
@@ -380,18 +401,20 @@ __global__ void __launch_bounds__(AR_THREADS, D_PAD > 128 ? 1 : 3) rows_kernel(c
         }
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
-    const int b = blockIdx.x, split = blockIdx.z, splits = a.splits;
     const int group = a.heads / a.kv_heads, m_tiles = (group + AR_HEADS - 1) / AR_HEADS;
-    const int hk = blockIdx.y / m_tiles, g0 = blockIdx.y % m_tiles * AR_HEADS, g = min(AR_HEADS, group - g0);
-    const int n = a.kv_len[b], t = a.query_start[b];
+    const int hk = blockIdx.x / m_tiles, g0 = blockIdx.x % m_tiles * AR_HEADS, g = min(AR_HEADS, group - g0);
+    const int split = blockIdx.z, splits = a.splits;
+    const int b = a.by_length ? row_by_length(smem, a, blockIdx.y) : (int)blockIdx.y;
+    const int n = a.kv_len[b], t = a.query_start[b], row_slot = a.row_slot[b];
     const int shared = a.skip ? a.skip[b] : 0;
     const int lo = max(shared, a.window > 0 ? max(0, n - a.window) : 0);          // the one query sits at position n - 1
     const int tile_lo = lo / T::KEYS, tile_hi = (n + T::KEYS - 1) / T::KEYS;
     const int per = max(0, tile_hi - tile_lo + splits - 1) / splits;
     const int first = tile_lo + split * per, last = min(tile_hi, first + per);
+    if (a.by_length) fence_async_smem();                             // (what was written where the first tiles go)
     __syncthreads();
     if (threadIdx.x >= 32 * AR_WARPS)
-        load_tiles<D_PAD, KV8>(&map, a, base, a.block_table + (size_t)a.row_slot[b] * a.table_stride, hk, first, last, n);
+        load_tiles<D_PAD, KV8>(&map, a, base, a.block_table + (size_t)row_slot * a.table_stride, hk, first, last, n);
     else
         walk<D_PAD, KV8>(smem, base, a, a.q + ((size_t)t * a.heads + hk * group + g0) * a.head_dim, g, first, last, lo, n);
     __syncthreads();
@@ -406,6 +429,7 @@ __global__ void __launch_bounds__(AR_THREADS, D_PAD > 128 ? 1 : 3) rows_kernel(c
     float* recv_ml = recv_o + splits * share;
     bf16* out = a.out + ((size_t)t * a.heads + hk * group + g0) * a.head_dim;
     int4 at = make_int4(0, 0, 0, 0);
+    if (a.skip) asm volatile("griddepcontrol.wait;\n" ::: "memory");   // (this launch may have begun before the one that leaves them ended)
     if (shared > 0) at = a.part_at[b];
     const size_t slot = (size_t)(at.x + hk * at.y) * a.part_rows + at.z + g0;
     const float* part_ml = shared > 0 ? a.part_ml + slot * 2 : nullptr;
@@ -440,7 +464,7 @@ __global__ void __launch_bounds__(AR_THREADS, D_PAD > 128 ? 1 : 3) rows_kernel(c
         float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int p = 0; p < pieces; ++p)
             add4(x, w[p], *(const float4*)(cluster ? recv_o + p * share + (i - from) : wo + (p * AR_HEADS + r) * D_PAD + d));
-#pragma unroll 8
+#pragma unroll 16
         for (int p = 0; p < at.y; ++p) add4(x, w[pieces + p], *(const float4*)(part_o + p * stride + i));
         float l = whole[2 * r + 1];
         if (a.sinks && l > 0.f) l += ex2(fmaf(a.sinks[hk * group + g0 + r], 1.4426950408889634f, -whole[2 * r]));   // the sink: a weight without a value
@@ -470,15 +494,21 @@ static int launch_rows(RowsArgs* a, int rows, int splits, int group, int head_di
         if (device < 64) prepared |= 1ull << device;
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = capacity ? dim3(1, 1, splits) : dim3(rows, a->kv_heads * ((group + AR_HEADS - 1) / AR_HEADS), splits);
+    cfg.gridDim = capacity ? dim3(1, 1, splits) : dim3(a->kv_heads * ((group + AR_HEADS - 1) / AR_HEADS), rows, splits);
     cfg.blockDim = dim3(AR_THREADS);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
-    cudaLaunchAttribute attr = {};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = 1; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = splits;
-    cfg.attrs = &attr;
-    cfg.numAttrs = splits > 1 ? 1 : 0;
+    cudaLaunchAttribute attrs[2] = {};
+    cfg.attrs = attrs;
+    if (splits > 1) {
+        attrs[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attrs[cfg.numAttrs].val.clusterDim.x = attrs[cfg.numAttrs].val.clusterDim.y = 1;
+        attrs[cfg.numAttrs++].val.clusterDim.z = splits;
+    }
+    if (!capacity && a->skip) {                                     // behind attention_prefix, whose CTAs say when they have all begun
+        attrs[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attrs[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
     if (capacity) {
         if (splits > 1) HB_CUDA(cudaOccupancyMaxActiveClusters(capacity, kernel, &cfg));
         else HB_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(capacity, kernel, AR_THREADS, smem));
@@ -519,7 +549,7 @@ extern "C" int hb_attention_rows_capacity(int kv8, int head_dim, int group, int 
 
 extern "C" int hb_attention_rows(void* out, const void* q, const void* kv, int kv8, const int32_t* block_table, int table_stride,
                                  const int32_t* row_slot, const int32_t* query_start, const int32_t* kv_len, int rows, int heads, int kv_heads,
-                                 int head_dim, int pages, int page_size, float scale, int window, int splits, const float* sinks,
+                                 int head_dim, int pages, int page_size, float scale, int window, int splits, int by_length, const float* sinks,
                                  const int32_t* skip, const float* part_o, const float* part_ml, const int32_t* part_at, int part_rows,
                                  hb_stream stream) {
     if (rows == 0) return 0;
@@ -529,13 +559,13 @@ extern "C" int hb_attention_rows(void* out, const void* q, const void* kv, int k
     if (splits < 1 || splits > 16) HB_REFUSE("attention_rows: %d splits (1 to 16, a cluster's size)", splits);
     if (!(scale > 0.f)) HB_REFUSE("attention_rows: the score scale must be positive");
     const int group = heads / kv_heads;
-    if ((long)kv_heads * ((group + AR_HEADS - 1) / AR_HEADS) > 65535) HB_REFUSE("attention_rows: %d heads", heads);
+    if (rows > 65535) HB_REFUSE("attention_rows: %d rows", rows);
     if (pages < 1 || (long)pages * 2 * kv_heads > 0x7ffffffel) HB_REFUSE("attention_rows: %d pages of %d kv heads", pages, kv_heads);
     if (((uintptr_t)kv % 16) || (((uintptr_t)q | (uintptr_t)out) % 8)) HB_REFUSE("attention_rows: the cache must start on 16 bytes, q and out on 8");
     if (skip && (!part_o || !part_ml || !part_at || window > 0)) HB_REFUSE("attention_rows: shared keys need their partial results, and no window");
     RowsArgs a = {(bf16*)out, (const bf16*)q, (const unsigned char*)kv, block_table, row_slot, query_start, kv_len, sinks, skip, part_o,
-                  part_ml, (const int4*)part_at, part_rows, table_stride, heads, kv_heads, head_dim, pages, page_size, 0, window, splits,
-                  scale * 1.4426950408889634f};
+                  part_ml, (const int4*)part_at, part_rows, table_stride, rows, heads, kv_heads, head_dim, pages, page_size,
+                  log2_exact(page_size), 0, window, splits, by_length && rows <= AR_BY_LENGTH, scale * 1.4426950408889634f};
     return kv8 ? any_rows<true>(&a, rows, splits, group, head_dim, nullptr, (cudaStream_t)stream)
                : any_rows<false>(&a, rows, splits, group, head_dim, nullptr, (cudaStream_t)stream);
 }

@@ -11,9 +11,10 @@ template <typename TW> __device__ __forceinline__ float2 load_w2(const TW* w);
 template <> __device__ __forceinline__ float2 load_w2<float>(const float* w) { return make_float2(w[0], w[1]); }
 template <> __device__ __forceinline__ float2 load_w2<bf16>(const bf16* w) { return make_float2(to_f32(w[0]), to_f32(w[1])); }
 
-// One warp per (token, head): query heads first, then key heads, then value heads; a row goes through shared memory.
+// One warp per (token, head): query heads first, then key heads, then value heads; a row goes through shared memory. Any rotation, any
+// head size, any alignment.
 template <typename TW>
-__global__ void __launch_bounds__(256) qk_norm_rope_kv_write8_kernel(
+__global__ void __launch_bounds__(128) qk_norm_rope_kv_write8_kernel(
         bf16* __restrict__ q_out, const bf16* __restrict__ qkv, const int32_t* __restrict__ positions,
         const float* __restrict__ table, int rotary_dim, int max_positions, const TW* __restrict__ q_weight,
         const TW* __restrict__ k_weight, float eps, float offset, unsigned char* __restrict__ kv,
@@ -83,6 +84,135 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kv_write8_kernel(
     if (lane == 0) base[(size_t)page_size * head_dim + off] = (unsigned char)(e + 127);
 }
 
+// The same with LANES lanes a (token, head), heads of up to 16 LANES numbers and rotations of a multiple of 16: a lane holds two
+// chunks of 8, where the head turns the two that pair (chunk c of the first half of the turned numbers and c of the second), so
+// that every access is 16 bytes wide, sums and maxima are shuffles and nothing goes through shared memory. 4,096 tokens of 32 + 8
+// heads of 128: 90 us in the kernel above, WRITE_US here (92 MB).
+__device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 p = __bfloat1622float2(*(const __nv_bfloat162*)&w[i]);
+        f[2 * i] = p.x; f[2 * i + 1] = p.y;
+    }
+}
+__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        __nv_bfloat162 p = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+        w[i] = *(uint32_t*)&p;
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <typename TW> __device__ __forceinline__ void load8(const TW* w, float (&f)[8]);
+template <> __device__ __forceinline__ void load8<bf16>(const bf16* w, float (&f)[8]) { unpack8(*(const uint4*)w, f); }
+template <> __device__ __forceinline__ void load8<float>(const float* w, float (&f)[8]) {
+    const float4 a = *(const float4*)w, b = *(const float4*)(w + 4);
+    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+}
+
+template <typename TW, int LANES>
+__global__ void __launch_bounds__(256, 3) qk_norm_rope_kv_write8_lanes_kernel(
+        bf16* __restrict__ q_out, const bf16* __restrict__ qkv, const int32_t* __restrict__ positions,
+        const float* __restrict__ table, int rotary_dim, int max_positions, const TW* __restrict__ q_weight,
+        const TW* __restrict__ k_weight, float eps, float offset, unsigned char* __restrict__ kv,
+        const int32_t* __restrict__ write_index, int pages, int page_size, unsigned units, int heads, int kv_heads, int head_dim,
+        const bf16* __restrict__ bias) {
+    const unsigned items = heads + (kv ? 2 * kv_heads : 0), step = gridDim.x * (256 / LANES);
+    const int sub = threadIdx.x & (LANES - 1);
+    const bool pairs = sub < rotary_dim >> 4, inside = sub < head_dim >> 4;      // (a value head's chunks are cut alike)
+    const int c0 = pairs ? sub * 8 : rotary_dim + (sub - (rotary_dim >> 4)) * 16, c1 = pairs ? c0 + (rotary_dim >> 1) : c0 + 8;
+    const bf16* first = qkv + (inside ? c0 : 0);
+    const int apart = inside ? c1 - c0 : 0, width = (heads + 2 * kv_heads) * head_dim;
+    // A unit's numbers, its position and its place in the cache are asked for a turn ahead: what a turn waits for is the rotation's row.
+    uint4 na = make_uint4(0, 0, 0, 0), nb = na;
+    int n_pos = 0, n_write = 0;
+    unsigned t = 0, item = 0;
+    auto ask = [&](unsigned u) {
+        if (u >= units) return;
+        t = u / items;
+        item = u - t * items;
+        const bf16* src = first + (size_t)t * width + item * head_dim;
+        if (inside) { na = *(const uint4*)src; nb = *(const uint4*)(src + apart); }
+        if (rotary_dim) n_pos = positions[t];
+        if (kv) n_write = write_index[t];
+    };
+    // (every lane of a warp makes as many turns: the shuffles are the whole warp's)
+    const unsigned mine = blockIdx.x * (256 / LANES) + threadIdx.x / LANES, warps_first = mine - (threadIdx.x & 31) / LANES;
+    ask(mine);
+    for (unsigned u0 = warps_first, u = mine; u0 < units; u0 += step, u += step) {
+        const uint4 ra = na, rb = nb;
+        const int write = n_write, head = (int)item;
+        const unsigned token = t;
+        const bool is_q = head < heads, is_v = head >= heads + kv_heads, turns = !is_v && pairs;
+        bool live = inside && u < units;
+        int pos = n_pos;
+        float a[8], b[8], wa[8], wb[8], cs[8], sn[8];
+        const TW* weight = is_q ? q_weight : is_v ? nullptr : k_weight;
+        if (live && turns) {
+            pos = pos < 0 ? 0 : (pos >= max_positions ? max_positions - 1 : pos);
+            const float* row = table + (size_t)pos * rotary_dim + sub * 8;
+            load8<float>(row, cs);
+            load8<float>(row + (rotary_dim >> 1), sn);
+        }
+        if (live && weight) { load8<TW>(weight + c0, wa); load8<TW>(weight + c1, wb); }
+        ask(u + step);
+        unpack8(ra, a);
+        unpack8(rb, b);
+        if (bias && live) {
+            float x[8], y[8];
+            load8<bf16>(bias + (size_t)head * head_dim + c0, x);
+            load8<bf16>(bias + (size_t)head * head_dim + c1, y);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) { a[i] += x[i]; b[i] += y[i]; }
+        }
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss += a[i] * a[i] + b[i] * b[i];
+        if (!inside) ss = 0.f;                                       // (lanes behind the head's end take part with zeros)
+#pragma unroll
+        for (int o = 1; o < LANES; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        if (weight && live) {
+            const float rstd = rsqrtf(ss / (float)head_dim + eps);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) { a[i] *= rstd * (wa[i] + offset); b[i] *= rstd * (wb[i] + offset); }
+        }
+        if (live && turns) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float x = a[i] * cs[i] - b[i] * sn[i];
+                b[i] = b[i] * cs[i] + a[i] * sn[i];
+                a[i] = x;
+            }
+        }
+        float largest = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) largest = fmaxf(largest, fmaxf(c8_magnitude(a[i]), c8_magnitude(b[i])));
+        if (!inside) largest = 0.f;
+#pragma unroll
+        for (int o = 1; o < LANES; o <<= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+        if (live && is_q) {
+            bf16* dst = q_out + ((size_t)token * heads + head) * head_dim;
+            *(uint4*)(dst + c0) = pack8(a);
+            *(uint4*)(dst + c1) = pack8(b);
+        } else if (live && write >= 0) {
+            const int page = write / page_size, off = write - page * page_size;
+            if (page < pages) {
+                unsigned char* base = kv + (((size_t)page * 2 + is_v) * kv_heads + (head - heads - (is_v ? kv_heads : 0))) * ((size_t)page_size * (head_dim + 1));
+                const int e = c8_exponent(largest);
+                const float inv = c8_power(-e);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) { a[i] *= inv; b[i] *= inv; }
+                unsigned char* row = base + (size_t)off * head_dim;
+                *(uint2*)(row + c0) = make_uint2(c8_pack4(a[0], a[1], a[2], a[3]), c8_pack4(a[4], a[5], a[6], a[7]));
+                *(uint2*)(row + c1) = make_uint2(c8_pack4(b[0], b[1], b[2], b[3]), c8_pack4(b[4], b[5], b[6], b[7]));
+                if (sub == 0) base[(size_t)page_size * head_dim + off] = (unsigned char)(e + 127);
+            }
+        }
+    }
+}
+
 extern "C" int hb_qk_norm_rope_kv_write8(void* q_out, const void* qkv, const int32_t* positions, const float* table,
                                          int rotary_dim, int max_positions, const void* q_weight, const void* k_weight,
                                          int weight_dtype, float eps, float offset, void* kv, const int32_t* write_index,
@@ -100,15 +230,29 @@ extern "C" int hb_qk_norm_rope_kv_write8(void* q_out, const void* qkv, const int
     if (((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)bias | (uintptr_t)kv) % 4) HB_REFUSE("qk_norm_rope_kv_write8: tensors must start on 4 bytes");
     cudaStream_t s = (cudaStream_t)stream;
     const long units = (long)tokens * (heads + (kv ? 2 * kv_heads : 0));
-    const int warps = 4;
-    const long blocks = (units + warps - 1) / warps;
-    if (blocks > 0x7fffffffl) HB_REFUSE("qk_norm_rope_kv_write8: %d tokens in one step", tokens);
 #define HB_ARGS(TW) (bf16*)q_out, (const bf16*)qkv, positions, table, rotary_dim, max_positions, (const TW*)q_weight, (const TW*)k_weight, \
     eps, offset, (unsigned char*)kv, write_index, pages, page_size, units, heads, kv_heads, head_dim, (const bf16*)bias
-    if (weight_dtype == HB_BF16)
-        qk_norm_rope_kv_write8_kernel<bf16><<<(unsigned)blocks, warps * 32, warps * head_dim * sizeof(float), s>>>(HB_ARGS(bf16));
-    else
-        qk_norm_rope_kv_write8_kernel<float><<<(unsigned)blocks, warps * 32, warps * head_dim * sizeof(float), s>>>(HB_ARGS(float));
+    const bool aligned = ((uintptr_t)q_out | (uintptr_t)qkv | (uintptr_t)table | (uintptr_t)q_weight | (uintptr_t)k_weight | (uintptr_t)kv | (uintptr_t)bias) % 16 == 0;
+    const bool lanes = aligned && rotary_dim % 16 == 0 && head_dim <= 256 && units < (1l << 31);
+    const int width = !lanes ? 64 : head_dim <= 32 ? 2 : head_dim <= 64 ? 4 : head_dim <= 128 ? 8 : 16;      // threads a unit; the general kernel: 4 units a block
+    const long blocks = (units + 256 / width - 1) / (256 / width);
+    if (blocks > 0x7fffffffl) HB_REFUSE("qk_norm_rope_kv_write8: %d tokens in one step", tokens);
+    static int sms = 0;                                              // (three blocks an SM hold all of a step's tokens in turns)
+    if (sms == 0) HB_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, 0));
+#define HB_LANES(TW, N) qk_norm_rope_kv_write8_lanes_kernel<TW, N><<<(unsigned)min(blocks, 3l * sms), 256, 0, s>>>( \
+        (bf16*)q_out, (const bf16*)qkv, positions, table, rotary_dim, max_positions, (const TW*)q_weight, (const TW*)k_weight, eps, offset, \
+        (unsigned char*)kv, write_index, pages, page_size, (unsigned)units, heads, kv_heads, head_dim, (const bf16*)bias)
+#define HB_WRITE(TW) do { \
+        if (!lanes) qk_norm_rope_kv_write8_kernel<TW><<<(unsigned)blocks, 128, 4 * head_dim * sizeof(float), s>>>(HB_ARGS(TW)); \
+        else if (width == 2) HB_LANES(TW, 2); \
+        else if (width == 4) HB_LANES(TW, 4); \
+        else if (width == 8) HB_LANES(TW, 8); \
+        else HB_LANES(TW, 16); \
+    } while (0)
+    if (weight_dtype == HB_BF16) HB_WRITE(bf16);
+    else HB_WRITE(float);
+#undef HB_WRITE
+#undef HB_LANES
 #undef HB_ARGS
     HB_LAUNCH_CHECK("qk_norm_rope_kv_write8");
     return 0;
@@ -116,56 +260,70 @@ extern "C" int hb_qk_norm_rope_kv_write8(void* q_out, const void* qkv, const int
 
 // ---------------------------------------------------------------- reading back
 template <typename T> __device__ __forceinline__ void store16(T* dst, const uint4& codes, float scale);
+__device__ __forceinline__ void store32(void* dst, const uint4& a, const uint4& b) {             // 32 bytes in one store: a whole sector a lane
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n"
+                 ::"l"(dst), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w) : "memory");
+}
 template <> __device__ __forceinline__ void store16<bf16>(bf16* dst, const uint4& codes, float scale) {
     uint4 a, b;
     c8_unpack16(codes, scale, a, b);
-    *(uint4*)dst = a;
-    *(uint4*)(dst + 8) = b;
+    store32(dst, a, b);
 }
 template <> __device__ __forceinline__ void store16<float>(float* dst, const uint4& codes, float scale) {
     uint4 a, b;
     c8_unpack16(codes, scale, a, b);                 // (exact in bfloat16, so through it)
     const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    uint32_t f[16];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) *(float2*)(dst + 2 * i) = __bfloat1622float2(*(const __nv_bfloat162*)&w[i]);
+    for (int i = 0; i < 8; ++i) { f[2 * i] = w[i] << 16; f[2 * i + 1] = w[i] & 0xffff0000u; }
+    store32(dst, make_uint4(f[0], f[1], f[2], f[3]), make_uint4(f[4], f[5], f[6], f[7]));
+    store32(dst + 8, make_uint4(f[8], f[9], f[10], f[11]), make_uint4(f[12], f[13], f[14], f[15]));
 }
 
-// One page, 16 codes a thread and turn; rows [0, keep) of every block as they are, the others as zeros.
+// One (part, kv head) block of a page, blockIdx.y's, 16 codes a thread and turn, four turns' loads at once; rows [0, keep) as they are,
+// the others as zeros. per_row: chunks of 16 codes a row, shift its log2 or -1.
+#define RD_THREADS 128
+#define RD_TURNS 4
 template <typename T>
-__device__ __forceinline__ void read_page(T* __restrict__ out, const unsigned char* __restrict__ kv, bool valid, int keep,
-                                          int kv_heads, int page_size, int head_dim) {
-    const int per_row = head_dim >> 4, chunks = 2 * kv_heads * page_size * per_row;
-    for (int i = blockIdx.y * blockDim.x + threadIdx.x; i < chunks; i += gridDim.y * blockDim.x) {
-        const int row = i / per_row, at = i - row * per_row, blk = row / page_size, r = row - blk * page_size;
-        uint4 codes = make_uint4(0, 0, 0, 0);
-        float scale = 0.f;
-        if (valid && r < keep) {
-            const unsigned char* b = kv + (size_t)blk * page_size * (head_dim + 1);
-            codes = *(const uint4*)(b + (size_t)r * head_dim + at * 16);
-            scale = c8_power((int)b[(size_t)page_size * head_dim + r] - 127);
+__device__ __forceinline__ void read_block(T* __restrict__ out, const unsigned char* __restrict__ kv, bool valid, int keep, int page_size, int head_dim, int shift) {
+    const int per_row = head_dim >> 4, chunks = page_size * per_row;
+    const size_t blk = blockIdx.y, codes_of = (size_t)page_size * head_dim;
+    const unsigned char* b = kv + blk * (codes_of + page_size);
+    out += blk * codes_of;
+    for (int i0 = threadIdx.x; i0 < chunks; i0 += RD_THREADS * RD_TURNS) {
+        uint4 codes[RD_TURNS];
+        float scale[RD_TURNS];
+#pragma unroll
+        for (int k = 0; k < RD_TURNS; ++k) {
+            const int i = i0 + k * RD_THREADS, r = shift >= 0 ? i >> shift : i / per_row;
+            const bool take = valid && i < chunks && r < keep;
+            codes[k] = take ? *(const uint4*)(b + (size_t)i * 16) : make_uint4(0, 0, 0, 0);
+            scale[k] = take ? c8_power((int)b[codes_of + r] - 127) : 0.f;
         }
-        store16<T>(out + (size_t)i * 16, codes, scale);
+#pragma unroll
+        for (int k = 0; k < RD_TURNS; ++k)
+            if (i0 + k * RD_THREADS < chunks) store16<T>(out + (size_t)(i0 + k * RD_THREADS) * 16, codes[k], scale[k]);
     }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) kv_read_kernel(T* __restrict__ out, const unsigned char* __restrict__ kv,
-                                                      const int32_t* __restrict__ index, int pages, int kv_heads, int page_size, int head_dim) {
+__global__ void __launch_bounds__(RD_THREADS) kv_read_kernel(T* __restrict__ out, const unsigned char* __restrict__ kv,
+                                                             const int32_t* __restrict__ index, int pages, int page_size, int head_dim, int shift) {
     const int page = index[blockIdx.x];
     const bool valid = page >= 0 && page < pages;
-    const size_t rows = (size_t)2 * kv_heads * page_size;
-    read_page<T>(out + (size_t)blockIdx.x * rows * head_dim, kv + (valid ? (size_t)page * rows * (head_dim + 1) : 0), valid, page_size,
-                 kv_heads, page_size, head_dim);
+    const size_t rows = (size_t)gridDim.y * page_size;
+    read_block<T>(out + (size_t)blockIdx.x * rows * head_dim, kv + (valid ? (size_t)page * rows * (head_dim + 1) : 0), valid, page_size, page_size,
+                  head_dim, shift);
 }
 
 // Rows row0 .. rows - 1: the pages that hold keys which one of a row's new tokens sees go to out, page i of row b at
 // (b - row0) * stride + i, and the tables with which an attention kernel finds them there are made: table [rows - row0, stride]
 // and slots [rows] (slots[b] = b - row0).
-__global__ void __launch_bounds__(256) kv_read_rows_kernel(bf16* __restrict__ out, int32_t* __restrict__ table, int32_t* __restrict__ slots,
-                                                           const unsigned char* __restrict__ kv, const int32_t* __restrict__ block_table,
-                                                           int table_stride, const int32_t* __restrict__ row_slot,
-                                                           const int32_t* __restrict__ query_start, const int32_t* __restrict__ kv_len, int row0,
-                                                           int stride, int pages, int kv_heads, int page_size, int head_dim, int window) {
+__global__ void __launch_bounds__(RD_THREADS) kv_read_rows_kernel(bf16* __restrict__ out, int32_t* __restrict__ table, int32_t* __restrict__ slots,
+                                                                  const unsigned char* __restrict__ kv, const int32_t* __restrict__ block_table,
+                                                                  int table_stride, const int32_t* __restrict__ row_slot,
+                                                                  const int32_t* __restrict__ query_start, const int32_t* __restrict__ kv_len, int row0,
+                                                                  int stride, int pages, int page_size, int head_dim, int window, int shift) {
     const int r = blockIdx.z, i = blockIdx.x, b = row0 + r;
     if (threadIdx.x == 0 && blockIdx.y == 0) {
         table[(size_t)r * stride + i] = r * stride + i;
@@ -176,33 +334,35 @@ __global__ void __launch_bounds__(256) kv_read_rows_kernel(bf16* __restrict__ ou
     if (i * page_size >= n || (i + 1) * page_size <= lo) return;
     const int page = block_table[(size_t)row_slot[b] * table_stride + i];
     const bool valid = page >= 0 && page < pages;
-    const size_t size = (size_t)2 * kv_heads * page_size;
-    read_page<bf16>(out + ((size_t)r * stride + i) * size * head_dim, kv + (valid ? (size_t)page * size * (head_dim + 1) : 0), valid,
-                    n - i * page_size, kv_heads, page_size, head_dim);
+    const size_t rows = (size_t)gridDim.y * page_size;
+    read_block<bf16>(out + ((size_t)r * stride + i) * rows * head_dim, kv + (valid ? (size_t)page * rows * (head_dim + 1) : 0), valid,
+                     n - i * page_size, page_size, head_dim, shift);
 }
 
 static int check_pages(const char* who, const void* out, const void* kv, int kv_heads, int page_size, int head_dim) {
     if (head_dim < 16 || head_dim % 16) HB_REFUSE("%s: head_dim %d is no multiple of 16", who, head_dim);
     if (page_size < 16 || page_size % 16) HB_REFUSE("%s: page size %d is no multiple of 16", who, page_size);
     if (kv_heads < 1 || (long)2 * kv_heads * page_size * head_dim > 0x7fffffffl) HB_REFUSE("%s: %d kv heads of %d in pages of %d", who, kv_heads, head_dim, page_size);
-    if (((uintptr_t)out | (uintptr_t)kv) % 16) HB_REFUSE("%s: tensors must start on 16 bytes", who);
+    if (2 * kv_heads > 65535) HB_REFUSE("%s: %d kv heads", who, kv_heads);
+    if ((uintptr_t)out % 32 || (uintptr_t)kv % 16) HB_REFUSE("%s: out must start on 32 bytes, the cache on 16", who);
     return 0;
 }
-static unsigned slices(int kv_heads, int page_size, int head_dim) {      // blocks a page: about 1,024 chunks each
-    const long chunks = (long)2 * kv_heads * page_size * (head_dim / 16);
-    return (unsigned)min(65535l, (chunks + 1023) / 1024);
+static int chunk_shift(int head_dim) {                // log2 of the chunks of 16 a row, or -1
+    const int n = head_dim / 16;
+    return (n & (n - 1)) == 0 ? __builtin_ctz(n) : -1;
 }
 
 extern "C" int hb_kv_read(void* out, int dtype, const void* kv, const int32_t* index, int count, int pages, int kv_heads, int page_size,
                           int head_dim, hb_stream stream) {
     if (count == 0) return 0;
     if (int rc = check_pages("kv_read", out, kv, kv_heads, page_size, head_dim)) return rc;
-    const dim3 grid(count, slices(kv_heads, page_size, head_dim));
+    const dim3 grid(count, 2 * kv_heads);
+    const int shift = chunk_shift(head_dim);
     cudaStream_t s = (cudaStream_t)stream;
     if (dtype == HB_BF16)
-        kv_read_kernel<bf16><<<grid, 256, 0, s>>>((bf16*)out, (const unsigned char*)kv, index, pages, kv_heads, page_size, head_dim);
+        kv_read_kernel<bf16><<<grid, RD_THREADS, 0, s>>>((bf16*)out, (const unsigned char*)kv, index, pages, page_size, head_dim, shift);
     else if (dtype == HB_F32)
-        kv_read_kernel<float><<<grid, 256, 0, s>>>((float*)out, (const unsigned char*)kv, index, pages, kv_heads, page_size, head_dim);
+        kv_read_kernel<float><<<grid, RD_THREADS, 0, s>>>((float*)out, (const unsigned char*)kv, index, pages, page_size, head_dim, shift);
     else HB_REFUSE("kv_read: no kernel for dtype %d", dtype);
     HB_LAUNCH_CHECK("kv_read");
     return 0;
@@ -215,9 +375,9 @@ extern "C" int hb_kv_read_rows(void* out, int32_t* table, int32_t* slots, const 
     if (int rc = check_pages("kv_read_rows", out, kv, kv_heads, page_size, head_dim)) return rc;
     if (stride > table_stride) HB_REFUSE("kv_read_rows: %d pages a row, the block table has %d", stride, table_stride);
     if (rows - row0 > 65535) HB_REFUSE("kv_read_rows: %d rows", rows - row0);
-    kv_read_rows_kernel<<<dim3(stride, slices(kv_heads, page_size, head_dim), rows - row0), 256, 0, (cudaStream_t)stream>>>(
+    kv_read_rows_kernel<<<dim3(stride, 2 * kv_heads, rows - row0), RD_THREADS, 0, (cudaStream_t)stream>>>(
         (bf16*)out, table, slots, (const unsigned char*)kv, block_table, table_stride, row_slot, query_start, kv_len, row0, stride, pages,
-        kv_heads, page_size, head_dim, window);
+        page_size, head_dim, window, chunk_shift(head_dim));
     HB_LAUNCH_CHECK("kv_read_rows");
     return 0;
 }

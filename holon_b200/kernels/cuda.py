@@ -678,16 +678,16 @@ class CudaKernels:
             scratch = torch.empty(rows_left * (head_dim + 2) + 4 * n, dtype=torch.float32, device=self.device)
             part_o, part_ml, part_at = (ctypes.c_void_p(scratch.data_ptr() + 4 * i)
                                         for i in (0, rows_left * head_dim, rows_left * (head_dim + 2)))
-            self._call("hb_attention_prefix", part_o, part_ml, part_at, self._p(q), self._p(kv), kv8, *common[:4], self._p(shared.members),
+            self._call("hb_attention_prefix", part_o, part_ml, part_at, self._p(q), self._p(kv), kv8, *common[:3], self._p(shared.members),
                        self._p(shared.groups), shared.groups.shape[0] // 3, heads, kv_heads, head_dim, kv.shape[0], page_size,
                        ctypes.c_float(scale), ctas)
             part = (self._p(shared.skip), part_o, part_ml, part_at, part_rows)
             longest = shared.longest_own
         if window > 0:
             longest = min(longest, window)
-        splits = self._row_splits(kv8, n, heads, kv_heads, head_dim, longest)
+        splits, by_length = self._row_splits(kv8, n, heads, kv_heads, head_dim, longest)
         self._call("hb_attention_rows", self._p(out), self._p(q), self._p(kv), kv8, *common, n, heads, kv_heads, head_dim, kv.shape[0],
-                   page_size, ctypes.c_float(scale), window, splits, self._p(sinks), *part)
+                   page_size, ctypes.c_float(scale), window, splits, by_length, self._p(sinks), *part)
 
     def _prefix_units(self, rows: int, heads: int, kv_heads: int, head_dim: int, page_size: int) -> int:
         """Partial results that `rows` one-token rows may leave at most for what they share, whatever their groups are: a tile for
@@ -700,19 +700,19 @@ class CudaKernels:
         ctas, part_rows, _ = self._prefix_plan(heads // kv_heads, head_dim, page_size)
         return self._prefix_units(rows, heads, kv_heads, head_dim, page_size) * part_rows * (head_dim + 2) + 4 * rows if ctas else 0
 
-    def _row_splits(self, kv8: int, rows: int, heads: int, kv_heads: int, head_dim: int, longest: int) -> int:
+    def _row_splits(self, kv8: int, rows: int, heads: int, kv_heads: int, head_dim: int, longest: int) -> tuple[int, int]:
         """Into how many CTAs (a cluster) the keys of a one-token row are cut: the number with the least waves x (64-key tiles a
-        CTA walks + its start)."""
+        CTA walks + its start); and whether there are more CTAs than run at once, so that the longest rows should start first."""
         key = ("rows", kv8, rows, heads, kv_heads, head_dim, -(-longest // 64))
         if key not in self._splits:
             group, tiles = heads // kv_heads, max(1, -(-longest // 64))
             pairs = rows * kv_heads * -(-group // 8)
-            best = (math.inf, 1)
+            best = (math.inf, 1, 0)
             for s in range(1, min(16, tiles) + 1):
                 room = int(self.lib.hb_attention_rows_capacity(kv8, head_dim, group, s)) * (self.sms if s == 1 else 1)
                 if room > 0:
-                    best = min(best, (-(-pairs // room) * (-(-tiles // s) + 2 + (s > 1)), s))
-            self._splits[key] = best[1]
+                    best = min(best, (-(-pairs // room) * (-(-tiles // s) + 2 + (s > 1)), s, int(pairs > room)))
+            self._splits[key] = best[1:]
         return self._splits[key]
 
     KV_BUCKET_MIN = 512                       # the smallest number of keys a captured decode launch is planned for
