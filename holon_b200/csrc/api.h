@@ -110,25 +110,26 @@ int hb_attention_decode_bf16_cluster(void* out, const void* q, const void* kv, c
 // One-token rows 0 .. rows - 1 over a cache of 8-bit codes (`kv8`) or of bfloat16, pages of a multiple of 16 tokens, 1 to 16 splits that
 // merge inside the kernel as a cluster (csrc/attention_rows.cu). `skip` (or null): tokens at a row's start that it shares with other
 // rows; it attends to those behind them, and the partial results of hb_attention_prefix (part_o, part_ml, part_at, and part_rows of its
-// plan) are joined with that; the call then follows that one on its stream. `by_length`: the rows with most keys first. hb_attention_rows_capacity: clusters of that many CTAs that run at once (splits 1: CTAs an SM), -1
+// plan) are joined with that; the call then follows that one on its stream. `few`: the form for rows of
+// few keys each (64 a tile, less memory a CTA). `by_length`: the rows with most keys first. hb_attention_rows_capacity: clusters of that many CTAs that run at once (splits 1: CTAs an SM), -1
 // for sizes that are refused.
-int hb_attention_rows_capacity(int kv8, int head_dim, int group, int splits);
+int hb_attention_rows_capacity(int kv8, int few, int head_dim, int group, int splits);
 int hb_attention_rows(void* out, const void* q, const void* kv, int kv8, const int32_t* block_table, int table_stride,
                       const int32_t* row_slot, const int32_t* query_start, const int32_t* kv_len, int rows, int heads, int kv_heads,
-                      int head_dim, int pages, int page_size, float scale, int window, int splits, int by_length, const float* sinks,
+                      int head_dim, int pages, int page_size, float scale, int window, int splits, int few, int by_length, const float* sinks,
                       const int32_t* skip, const float* part_o, const float* part_ml, const int32_t* part_at, int part_rows,
                       hb_stream stream);
 // Groups of one-token rows that hold the same first tokens in the same pages, over the keys of those (csrc/attention_prefix.cu;
-// head_dim 128 and pages of a multiple of 64 tokens: csrc/attention_prefix_tcgen05.cu): groups [n_groups][3] = (start in `members`,
-// rows, tokens), rows 0 for a group that is not there; `members` names rows of the
+// head_dim 128 and pages of a multiple of 64 tokens: csrc/attention_prefix_tcgen05.cu): groups [n_groups][4] = (start in `members`,
+// rows, tokens, the block table's row of one of them), rows 0 for a group that is not there; `members` names rows of the
 // step, and row b's query is token b. Leaves unnormalised results of `units` pieces
 // of work, at most max(ctas, kv_heads * tiles): part_o [units, part_rows, head_dim], part_ml [units, part_rows, 2] and per row of the
 // step part_at int32 [rows, 4]. hb_attention_prefix_plan: part_rows and the rows of the step a tile holds for a kv head of `group` query
 // heads; returns the CTAs an SM that suit the kernel, 0 where it does not take the sizes.
 int hb_attention_prefix_plan(int head_dim, int page_size, int group, int* part_rows, int* tile_rows);
 int hb_attention_prefix(float* part_o, float* part_ml, int32_t* part_at, const void* q, const void* kv, int kv8,
-                        const int32_t* block_table, int table_stride, const int32_t* row_slot, const int32_t* members, const int32_t* groups,
-                        int n_groups, int heads, int kv_heads, int head_dim, int pages, int page_size, float scale, int ctas,
+                        const int32_t* block_table, int table_stride, const int32_t* members, const int32_t* groups, int n_groups,
+                         int heads, int kv_heads, int head_dim, int pages, int page_size, float scale, int ctas,
                         hb_stream stream);
 
 // The same rows with the keys of all of them shared out evenly over `ctas` CTAs (one wave that fills the GPU): each

@@ -15,7 +15,7 @@ struct PrefixArgs {
     int4* part_at;
     const bf16* q;
     const unsigned char* kv;
-    const int32_t *block_table, *row_slot, *members, *groups;
+    const int32_t *block_table, *members, *groups;
     int n_groups, table_stride, heads, kv_heads, head_dim, pages, page_size;
     float scale_log2;
 };
@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(PX_THREADS) prefix_kernel(const PrefixArgs a) 
     constexpr bool Q_IN_REGS = D_PAD <= 128;
     for (int w = blockIdx.x; w < all.units; w += gridDim.x) {
         const PrefixUnit u = prefix_unit(known, a.kv_heads, all.chunk, w);
-        const int mrows = u.count * group, tokens = a.groups[3 * u.group + 2];
+        const int mrows = u.count * group;
         if (u.hk == 0 && u.split == 0 && threadIdx.x < u.count)
             a.part_at[a.members[u.start + threadIdx.x]] = make_int4(u.first, u.splits, (int)threadIdx.x * group, 0);
         __syncthreads();                                            // (the tiles are no longer read by the unit before)
@@ -90,9 +90,9 @@ __global__ void __launch_bounds__(PX_THREADS) prefix_kernel(const PrefixArgs a) 
             cp_async16(q_s + tile_off<D_PAD>(r, ch), src, valid);
         }
         cp_async_commit();
-        const int32_t* table = a.block_table + (size_t)a.row_slot[a.members[u.start]] * a.table_stride;
-        const int first = u.split * all.chunk, last = min(u.blocks, first + all.chunk);
-        load_shared_tile<D_PAD, KV8>(kv_s, kv_s + TILE_BYTES, a, table, u.hk, first * TILE_N, tokens);
+        const int32_t* table = a.block_table + (size_t)u.slot * a.table_stride;
+        const int first = u.split * all.chunk, last = min((u.tokens + 63) / 64, first + all.chunk);
+        load_shared_tile<D_PAD, KV8>(kv_s, kv_s + TILE_BYTES, a, table, u.hk, first * TILE_N, u.tokens);
         cp_async_commit();
         uint32_t qf[Q_IN_REGS ? D_PAD / 16 : 1][4];
         float o[D_PAD / 8][4];
@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(PX_THREADS) prefix_kernel(const PrefixArgs a) 
             __syncthreads();
             if (tile + 1 < last) {
                 const uint32_t next = kv_s + ((tile + 1 - first) & 1) * 2 * TILE_BYTES;
-                load_shared_tile<D_PAD, KV8>(next, next + TILE_BYTES, a, table, u.hk, (tile + 1) * TILE_N, tokens);
+                load_shared_tile<D_PAD, KV8>(next, next + TILE_BYTES, a, table, u.hk, (tile + 1) * TILE_N, u.tokens);
             }
             cp_async_commit();
             if (warp * 16 >= mrows) continue;                       // (uniform per warp; the barrier is above)
@@ -129,12 +129,12 @@ __global__ void __launch_bounds__(PX_THREADS) prefix_kernel(const PrefixArgs a) 
                     }
                 }
             }
-            if (tile * TILE_N + TILE_N > tokens) {
+            if (tile * TILE_N + TILE_N > u.tokens) {
 #pragma unroll
                 for (int nt = 0; nt < 8; ++nt)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (tile * TILE_N + nt * 8 + (lane & 3) * 2 + (e & 1) >= tokens) s[nt][e] = -INFINITY;
+                        if (tile * TILE_N + nt * 8 + (lane & 3) * 2 + (e & 1) >= u.tokens) s[nt][e] = -INFINITY;
             }
             float c0, c1;
             softmax_step<8>(s, m0, m1, l0, l1, a.scale_log2, c0, c1);
@@ -184,7 +184,7 @@ template <int D_PAD, bool KV8> static int launch_prefix(const PrefixArgs& a, int
 }
 
 int hb_attention_prefix_tcgen05(float* part_o, float* part_ml, int32_t* part_at, const void* q, const void* kv, int kv8, const int32_t* block_table,
-                                int table_stride, const int32_t* row_slot, const int32_t* members, const int32_t* groups, int n_groups,
+                                int table_stride, const int32_t* members, const int32_t* groups, int n_groups,
                                 int heads, int kv_heads, int pages, int page_size, float scale, int ctas, cudaStream_t s);
 static bool on_tcgen05(int head_dim, int page_size, int group) { return head_dim == 128 && page_size % 64 == 0 && group <= 128; }
 
@@ -201,7 +201,7 @@ extern "C" int hb_attention_prefix_plan(int head_dim, int page_size, int group, 
 }
 
 extern "C" int hb_attention_prefix(float* part_o, float* part_ml, int32_t* part_at, const void* q, const void* kv, int kv8,
-                                   const int32_t* block_table, int table_stride, const int32_t* row_slot, const int32_t* members,
+                                   const int32_t* block_table, int table_stride, const int32_t* members,
                                    const int32_t* groups, int n_groups, int heads, int kv_heads, int head_dim, int pages, int page_size, float scale,
                                    int ctas, hb_stream stream) {
     if (n_groups < 1 || ctas < 1) return 0;
@@ -211,11 +211,11 @@ extern "C" int hb_attention_prefix(float* part_o, float* part_ml, int32_t* part_
     if (page_size < 16 || page_size % 16) HB_REFUSE("attention_prefix: page size %d is no multiple of 16", page_size);
     if (!(scale > 0.f)) HB_REFUSE("attention_prefix: the score scale must be positive");
     if (pages < 1 || (long)pages * 2 * kv_heads > 0x7ffffffel) HB_REFUSE("attention_prefix: %d pages of %d kv heads", pages, kv_heads);
-    if (((uintptr_t)kv | (uintptr_t)q | (uintptr_t)part_at | (uintptr_t)part_o) % 16 || (uintptr_t)part_ml % 8) HB_REFUSE("attention_prefix: tensors must start on 16 bytes");
+    if (((uintptr_t)kv | (uintptr_t)q | (uintptr_t)part_at | (uintptr_t)groups) % 16 || (uintptr_t)part_o % 32 || (uintptr_t)part_ml % 8) HB_REFUSE("attention_prefix: tensors must start on 16 bytes");
     if (on_tcgen05(head_dim, page_size, heads / kv_heads))
-        return hb_attention_prefix_tcgen05(part_o, part_ml, part_at, q, kv, kv8, block_table, table_stride, row_slot, members, groups,
+        return hb_attention_prefix_tcgen05(part_o, part_ml, part_at, q, kv, kv8, block_table, table_stride, members, groups,
                                            n_groups, heads, kv_heads, pages, page_size, scale, ctas, (cudaStream_t)stream);
-    const PrefixArgs a = {part_o, part_ml, (int4*)part_at, (const bf16*)q, (const unsigned char*)kv, block_table, row_slot, members,
+    const PrefixArgs a = {part_o, part_ml, (int4*)part_at, (const bf16*)q, (const unsigned char*)kv, block_table, members,
                           groups, n_groups, table_stride, heads, kv_heads, head_dim, pages, page_size, scale * 1.4426950408889634f};
     cudaStream_t s = (cudaStream_t)stream;
     if (kv8) return head_dim <= 64 ? launch_prefix<64, true>(a, ctas, s) : head_dim <= 128 ? launch_prefix<128, true>(a, ctas, s) : launch_prefix<256, true>(a, ctas, s);

@@ -25,7 +25,7 @@
 #define PT_RAW_STAGE (2 * PT_RAW_BYTES + 1024)    // keys, values, 64 + 64 scale bytes
 #define PT_TMEM_COLS 512                          // per group: S0 [0, 64), S1 [64, 128), O [128, 256)
 #define PT_RESCALE 8.0f
-#define PT_MMA_WARP1 10                           // warps 10, 11: the groups' P V; 2 - 9: softmax; 0: loads; 1: Q K^T; 12 - 15: codes to bfloat16
+#define PT_MMA_WARP1 10                           // warps 1 and 10: Q K^T of the groups; 11: P V; 2 - 9: softmax; 0: loads; 12 - 15: codes to bfloat16
 #define PT_CONVERTERS 4
 
 template <bool KV8> struct Shape {
@@ -42,7 +42,7 @@ struct PrefixTcArgs {
     int4* part_at;
     const bf16* q;
     const unsigned char* kv;
-    const int32_t *block_table, *row_slot, *members, *groups;
+    const int32_t *block_table, *members, *groups;
     int n_groups, table_stride, heads, kv_heads, pages, page_size;
     float scale_log2;
 };
@@ -60,14 +60,25 @@ __device__ __forceinline__ uint4 ld_shared16(uint32_t at) {
     return v;
 }
 
-// One query row `src` (null: zeros) into row r of a group's operand.
-__device__ __forceinline__ void load_query(uint32_t q_s, const bf16* src, int r) {
-    uint4 x[PT_D / 8];
+// A warp's 32 query rows into rows r0 .. r0 + 31 of a group's operand: lane i says where row r0 + i begins among the queries
+// (negative: zeros). Eight lanes read a row, four rows at a time (a row a lane would ask for 32 lines an instruction, 16 times).
+__device__ __forceinline__ void load_queries(uint32_t q_s, const bf16* q, long mine, int r0) {
+    const int lane = threadIdx.x & 31, sub = lane & 7;
+    uint4 x[8][2];
 #pragma unroll
-    for (int c = 0; c < PT_D / 8; ++c) x[c] = src ? ((const uint4*)src)[c] : make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < 8; ++i) {
+        const long at = __shfl_sync(0xffffffffu, mine, i * 4 + (lane >> 3));
+        const uint4* src = (const uint4*)(q + (at < 0 ? 0 : at));
+        x[i][0] = at < 0 ? make_uint4(0, 0, 0, 0) : src[sub];
+        x[i][1] = at < 0 ? make_uint4(0, 0, 0, 0) : src[8 + sub];
+    }
 #pragma unroll
-    for (int c = 0; c < PT_D / 8; ++c)                                // (eight rows at one chunk: eight groups of banks)
-        st_shared16(q_s + (c >> 3) * (PT_Q_BYTES / 2) + r * 128 + (((c & 7) ^ (r & 7)) << 4), x[c]);
+    for (int i = 0; i < 8; ++i) {
+        const int r = r0 + i * 4 + (lane >> 3);
+        const uint32_t to = q_s + r * 128 + ((sub ^ (r & 7)) << 4);
+        st_shared16(to, x[i][0]);
+        st_shared16(to + PT_Q_BYTES / 2, x[i][1]);
+    }
     fence_async_smem();                                               // (the products read them through the async proxy)
 }
 __device__ __forceinline__ void st_global32(float* dst, const uint32_t* v) {      // 32 bytes: a whole sector a thread
@@ -90,6 +101,7 @@ __global__ void __launch_bounds__(Shape<KV8>::THREADS, 1) prefix_tcgen05_kernel(
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");   // (attention_rows.cu may begin with the rows' own keys)
 
     if (threadIdx.x == 0) {
+        asm volatile("prefetch.tensormap [%0];\n" ::"l"(&map_kv) : "memory");
         for (int s = 0; s < H::STAGES; ++s) { mbar_init(kv_full0 + 8 * s, KV8 ? PT_CONVERTERS : 1); mbar_init(kv_empty0 + 8 * s, 1 + PT_GROUPS); }
         for (int s = 0; s < H::RAW; ++s) { mbar_init(raw_full0 + 8 * s, 1); mbar_init(raw_empty0 + 8 * s, PT_CONVERTERS); }
         for (int i = 0; i < 2 * PT_GROUPS; ++i) { mbar_init(s_full0 + 8 * i, 1); mbar_init(p_full0 + 8 * i, 4); mbar_init(p_empty0 + 8 * i, 1); }
@@ -113,7 +125,7 @@ __global__ void __launch_bounds__(Shape<KV8>::THREADS, 1) prefix_tcgen05_kernel(
     bool ok = true;
     for (int w = blockIdx.x; w < all.units; w += gridDim.x, ++turn) {
         const PrefixUnit u = prefix_unit(known, a.kv_heads, all.chunk, w);
-        const int first = u.split * all.chunk, tiles = min(u.blocks, first + all.chunk) - first;
+        const int first = u.split * all.chunk, tiles = min(u.tokens / PT_BN, first + all.chunk) - first;
         int g_rows[PT_GROUPS];                                        // query rows of each group
 #pragma unroll
         for (int g = 0; g < PT_GROUPS; ++g) g_rows[g] = max(0, min(per_group, u.count - g * per_group)) * group;
@@ -122,7 +134,7 @@ __global__ void __launch_bounds__(Shape<KV8>::THREADS, 1) prefix_tcgen05_kernel(
                 a.part_at[a.members[u.start + i]] = make_int4(u.first, u.splits, i / per_group * PT_BM + i % per_group * group, 0);
 
         if (warp == 0) {
-            const int32_t* table = a.block_table + (size_t)a.row_slot[a.members[u.start]] * a.table_stride;
+            const int32_t* table = a.block_table + (size_t)u.slot * a.table_stride;
             for (int t0 = 0; t0 < tiles && ok; t0 += 32) {
                 const int key = (first + t0 + lane) * PT_BN, pi = key / a.page_size, in = key - pi * a.page_size;     // this lane's tile
                 int page = t0 + lane < tiles ? table[pi] : 0;
@@ -185,20 +197,19 @@ __global__ void __launch_bounds__(Shape<KV8>::THREADS, 1) prefix_tcgen05_kernel(
                 const uint32_t types = (1u << 4) | (1u << 7) | (1u << 10);
                 const uint32_t idesc_qk = types | ((uint32_t)(PT_BN >> 3) << 17) | ((uint32_t)(PT_BM >> 4) << 24);
                 const uint32_t idesc_pv = types | (1u << 16) | ((uint32_t)(PT_D >> 3) << 17) | ((uint32_t)(PT_BM >> 4) << 24);
-                if (warp == 1) {
-                    ok = mbar_wait(q_full, turn & 1, 12);
-                    for (int j = 0; j < tiles && ok; ++j) {
+                if (warp <= PT_MMA_WARP1) {                           // the scores of group 0 or 1
+                    const int g = warp == 1 ? 0 : 1;
+                    ok = mbar_wait(q_full, turn & 1, 4);
+                    for (int j = 0; j < tiles && ok; ++j) {           // (a group without rows still paces the stages)
                         const int n = seen + j, s = n % H::STAGES;
-                        ok = mbar_wait(kv_full0 + 8 * s, (n / H::STAGES) & 1, 4);
-                        const uint32_t k_src = kv_s + s * 2 * PT_KV_BYTES;
-                        for (int g = 0; g < PT_GROUPS && ok; ++g) {
-                            if (g_rows[g] == 0) continue;
+                        ok = mbar_wait(kv_full0 + 8 * s, (n / H::STAGES) & 1, 5);
+                        if (ok && g_rows[g] > 0) {
                             const int k = g_seen[g] + j, gb = g * 2 + (k & 1);
                             // S overwrites S and P of two tiles ago: wait until their P V has read them
-                            ok = mbar_wait(p_empty0 + 8 * gb, ((k >> 1) & 1) ^ 1, 5);
+                            ok = mbar_wait(p_empty0 + 8 * gb, ((k >> 1) & 1) ^ 1, 6);
                             if (!ok) break;
                             tc_fence_after();
-                            const uint32_t s_t = tmem + g * 256 + (k & 1) * PT_BN;
+                            const uint32_t k_src = kv_s + s * 2 * PT_KV_BYTES, s_t = tmem + g * 256 + (k & 1) * PT_BN;
 #pragma unroll
                             for (int kk = 0; kk < PT_D / 16; ++kk) {  // d 0..63 in the first block, 64..127 in the second
                                 const uint32_t blk = kk >> 2, within = (kk & 3) * 2;
@@ -210,18 +221,17 @@ __global__ void __launch_bounds__(Shape<KV8>::THREADS, 1) prefix_tcgen05_kernel(
                         if (ok) tc_commit(kv_empty0 + 8 * s);         // the keys of the stage have been read (all three must arrive)
                     }
                 } else {
-                    const int g = warp - PT_MMA_WARP1;
-                    const uint32_t o_t = tmem + g * 256 + 2 * PT_BN;
-                    for (int j = 0; j < tiles && ok; ++j) {           // (a group without rows still paces the stages)
+                    for (int j = 0; j < tiles && ok; ++j) {
                         const int n = seen + j, s = n % H::STAGES;
-                        ok = mbar_wait(kv_full0 + 8 * s, (n / H::STAGES) & 1, 6);
-                        if (ok && g_rows[g] > 0) {                    // O_g += P_g V
+                        ok = mbar_wait(kv_full0 + 8 * s, (n / H::STAGES) & 1, 7);
+                        for (int g = 0; g < PT_GROUPS && ok; ++g) {   // O_g += P_g V
+                            if (g_rows[g] == 0) continue;
                             const int k = g_seen[g] + j, gb = g * 2 + (k & 1);
-                            ok = mbar_wait(p_full0 + 8 * gb, (k >> 1) & 1, 7);
+                            ok = mbar_wait(p_full0 + 8 * gb, (k >> 1) & 1, 8);
                             if (!ok) break;
                             tc_fence_after();
                             const uint32_t v_src = kv_s + s * 2 * PT_KV_BYTES + PT_KV_BYTES;
-                            const uint32_t p_t = tmem + g * 256 + (k & 1) * PT_BN;   // P lies over the first half of its own S
+                            const uint32_t o_t = tmem + g * 256 + 2 * PT_BN, p_t = tmem + g * 256 + (k & 1) * PT_BN;   // P lies over the first half of its own S
 #pragma unroll
                             for (int kk = 0; kk < PT_BN / 16; ++kk)   // 16 keys a step: 8 columns along P, 16 rows down V
                                 tc_mma_f16_ts(o_t, p_t + kk * 8, tc_smem_desc_mn(v_src + kk * 16 * 128, PT_KV_BYTES / 2), idesc_pv, (j | kk) != 0);
@@ -241,9 +251,9 @@ __global__ void __launch_bounds__(Shape<KV8>::THREADS, 1) prefix_tcgen05_kernel(
             const uint32_t o_t = lane_t + 2 * PT_BN;
             float m_used = -INFINITY, l = 0.f;                        // in log2 units; the maximum may lag by PT_RESCALE
             if (g_rows[g] > 0) {
-                const bf16* src = nullptr;
-                if (r < g_rows[g]) src = a.q + ((size_t)a.members[u.start + g * per_group + r / group] * a.heads + u.hk * group + r % group) * PT_D;
-                load_query(q_s + g * PT_Q_BYTES, src, r);             // (one-token rows come first: a row's number is its token's)
+                long mine = -1;                                       // (one-token rows come first: a row's number is its token's)
+                if (r < g_rows[g]) mine = ((long)a.members[u.start + g * per_group + r / group] * a.heads + u.hk * group + r % group) * PT_D;
+                load_queries(q_s + g * PT_Q_BYTES, a.q, mine, quarter * 32);
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(q_full);
@@ -251,7 +261,7 @@ __global__ void __launch_bounds__(Shape<KV8>::THREADS, 1) prefix_tcgen05_kernel(
             if (g_rows[g] > 0) {
                 for (int j = 0; j < tiles && ok; ++j) {
                     const int k = g_seen[g] + j, gb = g * 2 + (k & 1);
-                    ok = mbar_wait(s_full0 + 8 * gb, (k >> 1) & 1, 8);
+                    ok = mbar_wait(s_full0 + 8 * gb, (k >> 1) & 1, 9);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     tc_fence_after();
@@ -374,9 +384,9 @@ template <bool KV8> static int launch(const PrefixTcArgs& a, int ctas, cudaStrea
 
 // hb_attention_prefix's work where head_dim is 128 and pages are multiples of 64 tokens (its checks are done).
 int hb_attention_prefix_tcgen05(float* part_o, float* part_ml, int32_t* part_at, const void* q, const void* kv, int kv8, const int32_t* block_table,
-                                int table_stride, const int32_t* row_slot, const int32_t* members, const int32_t* groups,
+                                int table_stride, const int32_t* members, const int32_t* groups,
                                 int n_groups, int heads, int kv_heads, int pages, int page_size, float scale, int ctas, cudaStream_t s) {
-    const PrefixTcArgs a = {part_o, part_ml, (int4*)part_at, (const bf16*)q, (const unsigned char*)kv, block_table, row_slot, members,
+    const PrefixTcArgs a = {part_o, part_ml, (int4*)part_at, (const bf16*)q, (const unsigned char*)kv, block_table, members,
                             groups, n_groups, table_stride, heads, kv_heads, pages, page_size, scale * 1.4426950408889634f};
     return kv8 ? launch<true>(a, ctas, s) : launch<false>(a, ctas, s);
 }

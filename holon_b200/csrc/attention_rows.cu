@@ -79,31 +79,32 @@ struct RowsArgs {
     float scale_log2;
 };
 
-// A stage's tile of KEYS keys: keys, then values, each as column blocks [KEYS rows][SUB bytes] that TMA swizzles over SUB bytes.
-template <int D_PAD, bool KV8> struct Tile {
+// A stage's tile of KEYS keys (FEW: 64, two stages: for rows of a few hundred keys, whose time is a CTA's start and end; four such
+// CTAs fit an SM): keys, then values, each as column blocks [KEYS rows][SUB bytes] that TMA swizzles over SUB bytes.
+template <int D_PAD, bool KV8, bool FEW> struct Tile {
     static constexpr int ROW = KV8 ? D_PAD : 2 * D_PAD;              // bytes of a key
-    static constexpr int NK = AR_NK(D_PAD, KV8), KEYS = 16 * AR_WARPS * NK;   // a warp takes NK times 16 keys of a tile
+    static constexpr int NK = FEW ? 1 : AR_NK(D_PAD, KV8), KEYS = 16 * AR_WARPS * NK;   // a warp takes NK times 16 keys of a tile
     static constexpr int SUB = ROW < 128 ? ROW : 128, NSUB = ROW / SUB, BLOCK = KEYS * SUB;
     static constexpr int PART = NSUB * BLOCK, STAGE = 2 * PART;
-    static constexpr int STAGES = AR_STAGES(STAGE);
+    static constexpr int STAGES = FEW ? 2 : AR_STAGES(STAGE);
     static constexpr int SUMS = (AR_WARPS * AR_HEADS * (D_PAD + 2)) * 4;      // what the warps leave, over the tiles
     static constexpr int BODY = STAGES * STAGE > SUMS ? STAGES * STAGE : SUMS;
     static constexpr int BARS = BODY + STAGES * 2 * KEYS;            // behind the tiles: a stage's scale bytes, then the barriers
     static constexpr int RECV = BARS + 16 * STAGES;                  // then what the other CTAs of a cluster send
 };
 // Byte offset of (row, 16-byte chunk) in a part of a tile: eight rows at one chunk lie in eight bank groups.
-template <int D_PAD, bool KV8> __device__ __forceinline__ uint32_t tile_at(int row, int chunk) {
-    using T = Tile<D_PAD, KV8>;
+template <int D_PAD, bool KV8, bool FEW> __device__ __forceinline__ uint32_t tile_at(int row, int chunk) {
+    using T = Tile<D_PAD, KV8, FEW>;
     if (T::SUB == 64) return (uint32_t)(row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4));
     return (uint32_t)((chunk >> 3) * T::BLOCK + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
 }
 
 // The loading warp: tiles [first, last) of (row, kv head). A tile is KEYS / box boxes of `box` keys that lie in one page each. Keys in
 // pages that do not exist, and boxes behind the row's last key, are zeros (their scales: those of the first page).
-template <int D_PAD, bool KV8>
+template <int D_PAD, bool KV8, bool FEW>
 __device__ __forceinline__ void load_tiles(const CUtensorMap* map, const RowsArgs& a, uint32_t base, const int32_t* table, int hk, int first, int last,
                                            int n) {
-    using T = Tile<D_PAD, KV8>;
+    using T = Tile<D_PAD, KV8, FEW>;
     const int lane = threadIdx.x & 31, boxes = T::KEYS / a.box, batch = 32 / boxes;
     const uint32_t full = base + T::BARS, empty = full + 8 * T::STAGES;
     const uint32_t bytes = T::STAGE + (KV8 ? 2 * T::KEYS : 0);
@@ -188,9 +189,9 @@ __device__ __forceinline__ float column_sum(float v) {
 
 // A computing warp's walk over tiles [first, last); leaves its sums over the tiles' memory: [warp][8][D_PAD] floats and
 // [warp][g][2] (maximum in log2 units, sum), once every warp is done with the tiles.
-template <int D_PAD, bool KV8>
+template <int D_PAD, bool KV8, bool FEW>
 __device__ __forceinline__ void walk(unsigned char* smem, uint32_t base, const RowsArgs& a, const bf16* q, int g, int first, int last, int lo, int n) {
-    using T = Tile<D_PAD, KV8>;
+    using T = Tile<D_PAD, KV8, FEW>;
     constexpr int NK = T::NK;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
     const uint32_t full = base + T::BARS, empty = full + 8 * T::STAGES;
@@ -218,7 +219,7 @@ __device__ __forceinline__ void walk(unsigned char* smem, uint32_t base, const R
 #pragma unroll
                 for (int ks = 0; ks < D_PAD / 16; ks += KV8 ? 2 : 1) {
                     uint32_t x[4];
-                    ldmatrix_x4(x, kt + tile_at<D_PAD, KV8>(row + 16 * kk, (KV8 ? ks : 2 * ks) + ch));
+                    ldmatrix_x4(x, kt + tile_at<D_PAD, KV8, FEW>(row + 16 * kk, (KV8 ? ks : 2 * ks) + ch));
                     if constexpr (KV8) {
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
@@ -264,7 +265,7 @@ __device__ __forceinline__ void walk(unsigned char* smem, uint32_t base, const R
                 for (int i = lane; i < 16 * NK * (T::ROW / 16); i += 32) {
                     const int at = i / (T::ROW / 16), key = key0 + at;
                     if (key < lo || key >= n)
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};\n" ::"r"(vt + tile_at<D_PAD, KV8>(warp * 16 * NK + at, i % (T::ROW / 16))), "r"(0u) : "memory");
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};\n" ::"r"(vt + tile_at<D_PAD, KV8, FEW>(warp * 16 * NK + at, i % (T::ROW / 16))), "r"(0u) : "memory");
                 }
                 fence_async_smem();
                 __syncwarp();
@@ -300,7 +301,7 @@ __device__ __forceinline__ void walk(unsigned char* smem, uint32_t base, const R
 #pragma unroll
                 for (int d = 0; d < D_PAD / 16; d += KV8 ? 2 : 1) {
                     uint32_t x[4];
-                    ldmatrix_x4_trans(x, vt + tile_at<D_PAD, KV8>(row + 16 * kk, (KV8 ? d : 2 * d) + ch));
+                    ldmatrix_x4_trans(x, vt + tile_at<D_PAD, KV8, FEW>(row + 16 * kk, (KV8 ? d : 2 * d) + ch));
                     if constexpr (KV8) {
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {                // two neighbouring codes of two keys -> pairs of keys: even numbers, odd ones
@@ -386,15 +387,16 @@ __device__ __forceinline__ int row_by_length(unsigned char* smem, const RowsArgs
 }
 
 // grid (kv_heads * ceil(group / 8), rows, splits), a cluster along z.
-template <int D_PAD, bool KV8>
-__global__ void __launch_bounds__(AR_THREADS, D_PAD > 128 ? 1 : 3) rows_kernel(const __grid_constant__ CUtensorMap map, const RowsArgs a) {
+template <int D_PAD, bool KV8, bool FEW>
+__global__ void __launch_bounds__(AR_THREADS, D_PAD > 128 ? 1 : FEW ? 4 : 3) rows_kernel(const __grid_constant__ CUtensorMap map, const RowsArgs a) {
     extern __shared__ unsigned char smem_raw[];
-    using T = Tile<D_PAD, KV8>;
+    using T = Tile<D_PAD, KV8, FEW>;
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     unsigned char* smem = smem_raw + (base - smem_u32(smem_raw));
     const bool cluster = a.splits > 1;
     if (cluster) asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");   // (this CTA runs: waited for before anybody writes here)
     if (threadIdx.x == 0) {
+        asm volatile("prefetch.tensormap [%0];\n" ::"l"(&map) : "memory");
         for (int s = 0; s < T::STAGES; ++s) {
             mbar_init(base + T::BARS + 8 * s, 1);
             mbar_init(base + T::BARS + 8 * (T::STAGES + s), AR_WARPS);
@@ -414,9 +416,9 @@ __global__ void __launch_bounds__(AR_THREADS, D_PAD > 128 ? 1 : 3) rows_kernel(c
     if (a.by_length) fence_async_smem();                             // (what was written where the first tiles go)
     __syncthreads();
     if (threadIdx.x >= 32 * AR_WARPS)
-        load_tiles<D_PAD, KV8>(&map, a, base, a.block_table + (size_t)row_slot * a.table_stride, hk, first, last, n);
+        load_tiles<D_PAD, KV8, FEW>(&map, a, base, a.block_table + (size_t)row_slot * a.table_stride, hk, first, last, n);
     else
-        walk<D_PAD, KV8>(smem, base, a, a.q + ((size_t)t * a.heads + hk * group + g0) * a.head_dim, g, first, last, lo, n);
+        walk<D_PAD, KV8, FEW>(smem, base, a, a.q + ((size_t)t * a.heads + hk * group + g0) * a.head_dim, g, first, last, lo, n);
     __syncthreads();
     // What the four warps left becomes one result a head, or, in a cluster, goes to the CTAs that combine it: each takes a share of
     // the numbers of all splits. The shared keys' partial results join the last step, and the sink.
@@ -455,17 +457,31 @@ __global__ void __launch_bounds__(AR_THREADS, D_PAD > 128 ? 1 : 3) rows_kernel(c
         cluster_barrier();                                          // everything sent has arrived; nobody reads another's memory after it
     }
     const int pieces = cluster ? splits : AR_WARPS, count = pieces + at.y;
+    const int from = cluster ? split * share : 0, upto = cluster ? min(total, from + share) : total;
+    constexpr int AHEAD = FEW ? 8 : 16;
+    float4 ahead[AHEAD];                                         // of a thread's first numbers, asked for before the weights are known
+    {
+        const int i = from + threadIdx.x * 4;
+#pragma unroll
+        for (int p = 0; p < AHEAD; ++p)
+            ahead[p] = i < upto && p < at.y ? *(const float4*)(part_o + p * stride + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
     weigh(weights, whole, cluster ? recv_ml : wml, pieces, g, part_ml, (size_t)a.part_rows * 2, at.y);
     __syncthreads();
-    const int from = cluster ? split * share : 0, upto = cluster ? min(total, from + share) : total;
     for (int i = from + threadIdx.x * 4; i < upto; i += AR_THREADS * 4) {
         const int r = i / a.head_dim, d = i - r * a.head_dim;
         const float* w = weights + r * count;
         float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int p = 0; p < pieces; ++p)
             add4(x, w[p], *(const float4*)(cluster ? recv_o + p * share + (i - from) : wo + (p * AR_HEADS + r) * D_PAD + d));
-#pragma unroll 16
-        for (int p = 0; p < at.y; ++p) add4(x, w[pieces + p], *(const float4*)(part_o + p * stride + i));
+        int p0 = 0;
+        if (i == from + (int)threadIdx.x * 4) {
+#pragma unroll
+            for (int p = 0; p < AHEAD; ++p) if (p < at.y) add4(x, w[pieces + p], ahead[p]);
+            p0 = AHEAD;
+        }
+#pragma unroll 8
+        for (int p = p0; p < at.y; ++p) add4(x, w[pieces + p], *(const float4*)(part_o + p * stride + i));
         float l = whole[2 * r + 1];
         if (a.sinks && l > 0.f) l += ex2(fmaf(a.sinks[hk * group + g0 + r], 1.4426950408889634f, -whole[2 * r]));   // the sink: a weight without a value
         const float inv = l > 0.f || l != l ? 1.f / l : 0.f;        // (a sum that is no number gives none)
@@ -474,22 +490,22 @@ __global__ void __launch_bounds__(AR_THREADS, D_PAD > 128 ? 1 : 3) rows_kernel(c
     }
 }
 
-template <int D_PAD, bool KV8> static size_t rows_smem(int splits, int group, int head_dim) {
+template <int D_PAD, bool KV8, bool FEW> static size_t rows_smem(int splits, int group, int head_dim) {
     const int g = group < AR_HEADS ? group : AR_HEADS;
     const size_t recv = splits > 1 ? (size_t)(g * head_dim + 4 * splits + splits * g * 2) * 4 : 0;  // (a share is rounded up)
-    return Tile<D_PAD, KV8>::RECV + recv + 1024;                    // (and the way to a boundary of 1,024 bytes)
+    return Tile<D_PAD, KV8, FEW>::RECV + recv + 1024;                    // (and the way to a boundary of 1,024 bytes)
 }
 
-template <int D_PAD, bool KV8>
+template <int D_PAD, bool KV8, bool FEW>
 static int launch_rows(RowsArgs* a, int rows, int splits, int group, int head_dim, int* capacity, cudaStream_t s) {
-    using T = Tile<D_PAD, KV8>;
-    auto kernel = rows_kernel<D_PAD, KV8>;
-    const size_t smem = rows_smem<D_PAD, KV8>(splits, group, head_dim);
+    using T = Tile<D_PAD, KV8, FEW>;
+    auto kernel = rows_kernel<D_PAD, KV8, FEW>;
+    const size_t smem = rows_smem<D_PAD, KV8, FEW>(splits, group, head_dim);
     static unsigned long long prepared = 0;                         // devices that the kernel's limits are set on
     int device = 0;
     HB_CUDA(cudaGetDevice(&device));
     if (device >= 64 || !(prepared >> device & 1)) {
-        HB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)rows_smem<D_PAD, KV8>(16, AR_HEADS, D_PAD)));
+        HB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)rows_smem<D_PAD, KV8, FEW>(16, AR_HEADS, D_PAD)));
         HB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
         if (device < 64) prepared |= 1ull << device;
     }
@@ -528,19 +544,24 @@ static int launch_rows(RowsArgs* a, int rows, int splits, int group, int head_di
     HB_CUDA(cudaLaunchKernelEx(&cfg, kernel, (const CUtensorMap)map, (const RowsArgs)*a));
     return 0;
 }
-template <bool KV8> static int any_rows(RowsArgs* a, int rows, int splits, int group, int head_dim, int* capacity, cudaStream_t s) {
-    if (head_dim <= 64) return launch_rows<64, KV8>(a, rows, splits, group, head_dim, capacity, s);
-    if (head_dim <= 128) return launch_rows<128, KV8>(a, rows, splits, group, head_dim, capacity, s);
-    return launch_rows<256, KV8>(a, rows, splits, group, head_dim, capacity, s);
+template <bool KV8, bool FEW> static int any_rows(RowsArgs* a, int rows, int splits, int group, int head_dim, int* capacity, cudaStream_t s) {
+    if (head_dim <= 64) return launch_rows<64, KV8, FEW>(a, rows, splits, group, head_dim, capacity, s);
+    if (head_dim <= 128) return launch_rows<128, KV8, FEW>(a, rows, splits, group, head_dim, capacity, s);
+    return launch_rows<256, KV8, FEW>(a, rows, splits, group, head_dim, capacity, s);
 }
 
 HB_DEFINE_STATUS_MIRROR(hb_attention_rows_status_mirror)
 
+static int forms(int kv8, int few, RowsArgs* a, int rows, int splits, int group, int head_dim, int* capacity, cudaStream_t s) {
+    if (kv8) return few ? any_rows<true, true>(a, rows, splits, group, head_dim, capacity, s) : any_rows<true, false>(a, rows, splits, group, head_dim, capacity, s);
+    return few ? any_rows<false, true>(a, rows, splits, group, head_dim, capacity, s) : any_rows<false, false>(a, rows, splits, group, head_dim, capacity, s);
+}
+
 // Clusters of `splits` CTAs that run at once (splits 1: CTAs an SM); -1 where the sizes are refused.
-extern "C" int hb_attention_rows_capacity(int kv8, int head_dim, int group, int splits) {
+extern "C" int hb_attention_rows_capacity(int kv8, int few, int head_dim, int group, int splits) {
     int n = 0;
     if (head_dim < 16 || head_dim > 256 || head_dim % 16 || group < 1 || splits < 1 || splits > 16) return -1;
-    if ((kv8 ? any_rows<true>(nullptr, 1, splits, group, head_dim, &n, 0) : any_rows<false>(nullptr, 1, splits, group, head_dim, &n, 0)) != 0) {
+    if (forms(kv8, few, nullptr, 1, splits, group, head_dim, &n, 0) != 0) {
         (void)cudaGetLastError();
         return 0;
     }
@@ -549,7 +570,7 @@ extern "C" int hb_attention_rows_capacity(int kv8, int head_dim, int group, int 
 
 extern "C" int hb_attention_rows(void* out, const void* q, const void* kv, int kv8, const int32_t* block_table, int table_stride,
                                  const int32_t* row_slot, const int32_t* query_start, const int32_t* kv_len, int rows, int heads, int kv_heads,
-                                 int head_dim, int pages, int page_size, float scale, int window, int splits, int by_length, const float* sinks,
+                                 int head_dim, int pages, int page_size, float scale, int window, int splits, int few, int by_length, const float* sinks,
                                  const int32_t* skip, const float* part_o, const float* part_ml, const int32_t* part_at, int part_rows,
                                  hb_stream stream) {
     if (rows == 0) return 0;
@@ -566,6 +587,5 @@ extern "C" int hb_attention_rows(void* out, const void* q, const void* kv, int k
     RowsArgs a = {(bf16*)out, (const bf16*)q, (const unsigned char*)kv, block_table, row_slot, query_start, kv_len, sinks, skip, part_o,
                   part_ml, (const int4*)part_at, part_rows, table_stride, rows, heads, kv_heads, head_dim, pages, page_size,
                   log2_exact(page_size), 0, window, splits, by_length && rows <= AR_BY_LENGTH, scale * 1.4426950408889634f};
-    return kv8 ? any_rows<true>(&a, rows, splits, group, head_dim, nullptr, (cudaStream_t)stream)
-               : any_rows<false>(&a, rows, splits, group, head_dim, nullptr, (cudaStream_t)stream);
+    return forms(kv8, few, &a, rows, splits, group, head_dim, nullptr, (cudaStream_t)stream);
 }

@@ -117,9 +117,10 @@ __global__ void __launch_bounds__(256, 3) qk_norm_rope_kv_write8_lanes_kernel(
         bf16* __restrict__ q_out, const bf16* __restrict__ qkv, const int32_t* __restrict__ positions,
         const float* __restrict__ table, int rotary_dim, int max_positions, const TW* __restrict__ q_weight,
         const TW* __restrict__ k_weight, float eps, float offset, unsigned char* __restrict__ kv,
-        const int32_t* __restrict__ write_index, int pages, int page_size, unsigned units, int heads, int kv_heads, int head_dim,
+        const int32_t* __restrict__ write_index, int pages, int page_size, int page_shift, unsigned units, int heads, int kv_heads, int head_dim,
         const bf16* __restrict__ bias) {
     const unsigned items = heads + (kv ? 2 * kv_heads : 0), step = gridDim.x * (256 / LANES);
+    const unsigned step_t = step / items, step_item = step - step_t * items;
     const int sub = threadIdx.x & (LANES - 1);
     const bool pairs = sub < rotary_dim >> 4, inside = sub < head_dim >> 4;      // (a value head's chunks are cut alike)
     const int c0 = pairs ? sub * 8 : rotary_dim + (sub - (rotary_dim >> 4)) * 16, c1 = pairs ? c0 + (rotary_dim >> 1) : c0 + 8;
@@ -128,18 +129,16 @@ __global__ void __launch_bounds__(256, 3) qk_norm_rope_kv_write8_lanes_kernel(
     // A unit's numbers, its position and its place in the cache are asked for a turn ahead: what a turn waits for is the rotation's row.
     uint4 na = make_uint4(0, 0, 0, 0), nb = na;
     int n_pos = 0, n_write = 0;
-    unsigned t = 0, item = 0;
+    const unsigned mine = blockIdx.x * (256 / LANES) + threadIdx.x / LANES, warps_first = mine - (threadIdx.x & 31) / LANES;
+    unsigned t = mine / items, item = mine - t * items;
     auto ask = [&](unsigned u) {
         if (u >= units) return;
-        t = u / items;
-        item = u - t * items;
         const bf16* src = first + (size_t)t * width + item * head_dim;
         if (inside) { na = *(const uint4*)src; nb = *(const uint4*)(src + apart); }
         if (rotary_dim) n_pos = positions[t];
         if (kv) n_write = write_index[t];
     };
     // (every lane of a warp makes as many turns: the shuffles are the whole warp's)
-    const unsigned mine = blockIdx.x * (256 / LANES) + threadIdx.x / LANES, warps_first = mine - (threadIdx.x & 31) / LANES;
     ask(mine);
     for (unsigned u0 = warps_first, u = mine; u0 < units; u0 += step, u += step) {
         const uint4 ra = na, rb = nb;
@@ -157,6 +156,9 @@ __global__ void __launch_bounds__(256, 3) qk_norm_rope_kv_write8_lanes_kernel(
             load8<float>(row + (rotary_dim >> 1), sn);
         }
         if (live && weight) { load8<TW>(weight + c0, wa); load8<TW>(weight + c1, wb); }
+        t += step_t;
+        item += step_item;
+        if (item >= items) { item -= items; ++t; }
         ask(u + step);
         unpack8(ra, a);
         unpack8(rb, b);
@@ -186,18 +188,34 @@ __global__ void __launch_bounds__(256, 3) qk_norm_rope_kv_write8_lanes_kernel(
                 a[i] = x;
             }
         }
-        float largest = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) largest = fmaxf(largest, fmaxf(c8_magnitude(a[i]), c8_magnitude(b[i])));
-        if (!inside) largest = 0.f;
-#pragma unroll
-        for (int o = 1; o < LANES; o <<= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
         if (live && is_q) {
             bf16* dst = q_out + ((size_t)token * heads + head) * head_dim;
             *(uint4*)(dst + c0) = pack8(a);
             *(uint4*)(dst + c1) = pack8(b);
-        } else if (live && write >= 0) {
-            const int page = write / page_size, off = write - page * page_size;
+        }
+        if (!__any_sync(0xffffffffu, live && !is_q)) continue;
+        // The largest magnitude by its bits: they order as the numbers do, and what is not finite lies above all that is.
+        uint32_t bits = 0;
+        if (inside)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) bits = max(bits, max(__float_as_uint(a[i]) & 0x7fffffffu, __float_as_uint(b[i]) & 0x7fffffffu));
+#pragma unroll
+        for (int o = 1; o < LANES; o <<= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
+        float largest = __uint_as_float(bits);
+        if (__any_sync(0xffffffffu, bits >= 0x7f800000u)) {           // (rows with infinities or NaN: the largest finite one, and NaN for the others)
+            largest = 0.f;
+            if (inside)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    largest = fmaxf(largest, fmaxf(c8_magnitude(a[i]), c8_magnitude(b[i])));
+                    if (fabsf(a[i]) == INFINITY) a[i] = __uint_as_float(0x7fc00000u);
+                    if (fabsf(b[i]) == INFINITY) b[i] = __uint_as_float(0x7fc00000u);
+                }
+#pragma unroll
+            for (int o = 1; o < LANES; o <<= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+        }
+        if (live && !is_q && write >= 0) {
+            const int page = page_shift >= 0 ? write >> page_shift : write / page_size, off = write - page * page_size;
             if (page < pages) {
                 unsigned char* base = kv + (((size_t)page * 2 + is_v) * kv_heads + (head - heads - (is_v ? kv_heads : 0))) * ((size_t)page_size * (head_dim + 1));
                 const int e = c8_exponent(largest);
@@ -205,8 +223,8 @@ __global__ void __launch_bounds__(256, 3) qk_norm_rope_kv_write8_lanes_kernel(
 #pragma unroll
                 for (int i = 0; i < 8; ++i) { a[i] *= inv; b[i] *= inv; }
                 unsigned char* row = base + (size_t)off * head_dim;
-                *(uint2*)(row + c0) = make_uint2(c8_pack4(a[0], a[1], a[2], a[3]), c8_pack4(a[4], a[5], a[6], a[7]));
-                *(uint2*)(row + c1) = make_uint2(c8_pack4(b[0], b[1], b[2], b[3]), c8_pack4(b[4], b[5], b[6], b[7]));
+                *(uint2*)(row + c0) = make_uint2(c8_pack4_finite(a[0], a[1], a[2], a[3]), c8_pack4_finite(a[4], a[5], a[6], a[7]));
+                *(uint2*)(row + c1) = make_uint2(c8_pack4_finite(b[0], b[1], b[2], b[3]), c8_pack4_finite(b[4], b[5], b[6], b[7]));
                 if (sub == 0) base[(size_t)page_size * head_dim + off] = (unsigned char)(e + 127);
             }
         }
@@ -241,7 +259,7 @@ extern "C" int hb_qk_norm_rope_kv_write8(void* q_out, const void* qkv, const int
     if (sms == 0) HB_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, 0));
 #define HB_LANES(TW, N) qk_norm_rope_kv_write8_lanes_kernel<TW, N><<<(unsigned)min(blocks, 3l * sms), 256, 0, s>>>( \
         (bf16*)q_out, (const bf16*)qkv, positions, table, rotary_dim, max_positions, (const TW*)q_weight, (const TW*)k_weight, eps, offset, \
-        (unsigned char*)kv, write_index, pages, page_size, (unsigned)units, heads, kv_heads, head_dim, (const bf16*)bias)
+        (unsigned char*)kv, write_index, pages, page_size, page_size & (page_size - 1) ? -1 : __builtin_ctz(page_size | (page_size == 0)), (unsigned)units, heads, kv_heads, head_dim, (const bf16*)bias)
 #define HB_WRITE(TW) do { \
         if (!lanes) qk_norm_rope_kv_write8_kernel<TW><<<(unsigned)blocks, 128, 4 * head_dim * sizeof(float), s>>>(HB_ARGS(TW)); \
         else if (width == 2) HB_LANES(TW, 2); \

@@ -26,13 +26,17 @@ __device__ __forceinline__ float c8_magnitude(float x) {
 }
 __device__ __forceinline__ float c8_power(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
-// Codes of a (low byte) and b, already divided by their scale; infinities become NaN, as NaN does.
-__device__ __forceinline__ uint32_t c8_pack2(float a, float b) {
-    if (fabsf(a) == INFINITY) a = __uint_as_float(0x7fc00000u);
-    if (fabsf(b) == INFINITY) b = __uint_as_float(0x7fc00000u);
+// Codes of a (low byte) and b, already divided by their scale; NaN stays NaN. c8_pack2: infinities become NaN, too.
+__device__ __forceinline__ uint32_t c8_pack2_finite(float a, float b) {
     uint16_t r;
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;\n" : "=h"(r) : "f"(b), "f"(a));
     return r;
+}
+__device__ __forceinline__ uint32_t c8_pack4_finite(float a, float b, float c, float d) { return c8_pack2_finite(a, b) | c8_pack2_finite(c, d) << 16; }
+__device__ __forceinline__ uint32_t c8_pack2(float a, float b) {
+    if (fabsf(a) == INFINITY) a = __uint_as_float(0x7fc00000u);
+    if (fabsf(b) == INFINITY) b = __uint_as_float(0x7fc00000u);
+    return c8_pack2_finite(a, b);
 }
 __device__ __forceinline__ uint32_t c8_pack4(float a, float b, float c, float d) { return c8_pack2(a, b) | c8_pack2(c, d) << 16; }
 

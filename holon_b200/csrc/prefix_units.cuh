@@ -16,38 +16,27 @@ struct PrefixUnits {
 struct PrefixUnit {
     int group, tile, first;           // the group, the tile's number in it, the first unit of (tile, kv head 0)
     int splits, hk, split;            // units of each (tile, kv head); this one's kv head and place
-    int start, count, blocks;         // the tile's rows in `members`, and the blocks of 64 keys they share (the last may be cut short)
+    int start, count, tokens, slot;   // the tile's rows in `members`, the tokens they share, the block table's row where those lie
 };
-
-__device__ __forceinline__ int pu_sum(int v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
-}
-__device__ __forceinline__ int pu_max(int v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
-}
 
 // What a lane holds of up to 32 groups, g0 + lane: the first ones are read once (few steps have more).
 struct PrefixGroups {
-    const int32_t* groups;            // [n_groups][3]: start, count (0: none), tokens
+    const int4* groups;               // [n_groups]: start, count (0: none), tokens, the block table's row of one of them
     int n_groups, rows_per_tile;
-    int start, tiles, count, blocks;  // of group `lane`
-    __device__ __forceinline__ void read(int g, int& start_, int& tiles_, int& count_, int& blocks_) const {
-        const bool there = g < n_groups;
-        start_ = there ? groups[3 * g] : 0;
-        count_ = there ? groups[3 * g + 1] : 0;
-        blocks_ = there ? (groups[3 * g + 2] + 63) >> 6 : 0;
-        tiles_ = (int)((unsigned)(count_ + rows_per_tile - 1) / (unsigned)rows_per_tile);
+    int start, tiles, count, blocks, tokens, slot;  // of group `lane`
+    __device__ __forceinline__ void read(int g) {
+        const int4 x = g < n_groups ? groups[g] : make_int4(0, 0, 0, 0);
+        start = x.x; count = x.y; tokens = x.z; slot = x.w;
+        blocks = (tokens + 63) >> 6;
+        tiles = (int)((unsigned)(count + rows_per_tile - 1) / (unsigned)rows_per_tile);
     }
-    __device__ __forceinline__ PrefixGroups(const int32_t* groups_, int n, int rows) : groups(groups_), n_groups(n), rows_per_tile(rows) {
-        read(threadIdx.x & 31, start, tiles, count, blocks);
+    __device__ __forceinline__ PrefixGroups(const int32_t* groups_, int n, int rows) : groups((const int4*)groups_), n_groups(n), rows_per_tile(rows) {
+        read(threadIdx.x & 31);
     }
-    __device__ __forceinline__ void at(int g0, int& start_, int& tiles_, int& count_, int& blocks_) const {
-        if (g0 == 0) { start_ = start; tiles_ = tiles; count_ = count; blocks_ = blocks; }
-        else read(g0 + (threadIdx.x & 31), start_, tiles_, count_, blocks_);
+    __device__ __forceinline__ PrefixGroups from(int g0) const {     // groups g0 ..
+        PrefixGroups x = *this;
+        if (g0 > 0) x.read(g0 + (threadIdx.x & 31));
+        return x;
     }
 };
 
@@ -55,11 +44,10 @@ struct PrefixGroups {
 __device__ __forceinline__ PrefixUnits prefix_units(const PrefixGroups& all, int kv_heads, int slots) {
     int tiles = 0, blocks = 0, longest = 0;
     for (int g0 = 0; g0 < all.n_groups; g0 += 32) {
-        int s, t, c, k;
-        all.at(g0, s, t, c, k);
-        tiles += t; blocks += t * k; longest = max(longest, t > 0 ? k : 0);
+        const PrefixGroups x = all.from(g0);
+        tiles += x.tiles; blocks += x.tiles * x.blocks; longest = max(longest, x.tiles > 0 ? x.blocks : 0);
     }
-    tiles = pu_sum(tiles); blocks = pu_sum(blocks); longest = pu_max(longest);
+    tiles = __reduce_add_sync(0xffffffffu, tiles); blocks = __reduce_add_sync(0xffffffffu, blocks); longest = __reduce_max_sync(0xffffffffu, longest);
     const int each = slots / kv_heads, budget = each - tiles;        // units a kv head; those beyond one a tile
     const int most = max(PU_MIN_CHUNK, budget > 0 ? min(longest, (blocks + budget - 1) / budget) : longest);   // surely enough
     PrefixUnits u;
@@ -67,11 +55,10 @@ __device__ __forceinline__ PrefixUnits prefix_units(const PrefixGroups& all, int
     while (true) {
         int units = 0;
         for (int g0 = 0; g0 < all.n_groups; g0 += 32) {
-            int s, t, c, k;
-            all.at(g0, s, t, c, k);
-            units += t * (int)((unsigned)(k + u.chunk - 1) / (unsigned)u.chunk);
+            const PrefixGroups x = all.from(g0);
+            units += x.tiles * (int)((unsigned)(x.blocks + u.chunk - 1) / (unsigned)u.chunk);
         }
-        u.units = pu_sum(units) * kv_heads;
+        u.units = __reduce_add_sync(0xffffffffu, units) * kv_heads;
         if (u.chunk >= most || u.units <= slots) return u;
         ++u.chunk;
     }
@@ -83,14 +70,13 @@ __device__ __forceinline__ PrefixUnit prefix_unit(const PrefixGroups& all, int k
     PrefixUnit u = {};
     int before = 0;
     for (int g0 = 0; g0 < all.n_groups; g0 += 32) {
-        int start, tiles, count, blocks;
-        all.at(g0, start, tiles, count, blocks);
-        const int splits = (int)((unsigned)(blocks + chunk - 1) / (unsigned)chunk), mine = tiles * splits * kv_heads;
+        const PrefixGroups x = all.from(g0);
+        const int splits = (int)((unsigned)(x.blocks + chunk - 1) / (unsigned)chunk), mine = x.tiles * splits * kv_heads;
         int upto = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int x = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += x;
+            const int below = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += below;
         }
         const unsigned hit = __ballot_sync(0xffffffffu, before + upto > want);
         if (hit) {
@@ -98,8 +84,9 @@ __device__ __forceinline__ PrefixUnit prefix_unit(const PrefixGroups& all, int k
             const int at = __shfl_sync(0xffffffffu, before + upto - mine, src);
             u.group = g0 + src;
             u.splits = __shfl_sync(0xffffffffu, splits, src);
-            u.blocks = __shfl_sync(0xffffffffu, blocks, src);
-            const int in_group = __shfl_sync(0xffffffffu, count, src), first_row = __shfl_sync(0xffffffffu, start, src);
+            u.tokens = __shfl_sync(0xffffffffu, x.tokens, src);
+            u.slot = __shfl_sync(0xffffffffu, x.slot, src);
+            const int in_group = __shfl_sync(0xffffffffu, x.count, src), first_row = __shfl_sync(0xffffffffu, x.start, src);
             const unsigned rest = want - at, pair = rest / (unsigned)u.splits;    // the unit's (tile, kv head)
             u.split = (int)(rest - pair * u.splits);
             u.tile = (int)(pair / (unsigned)kv_heads);

@@ -48,8 +48,8 @@ class SharedPrefix:
 
     A group is two or more rows and the tokens that all of them share (whole pages, and fewer than any of them holds); a
     row is in one group at most. Device, int32: `skip` [rows] (tokens that the row shares, 0 outside the groups), `members`
-    [rows] (the groups' rows, one group after the other; what follows is not read) and `groups` [3 · (rows // 2)] ((start in `members`,
-    rows, tokens) a group, zeros behind the last). Host: `rows`, and `longest_own`, the most tokens any row has beside those it shares."""
+    [rows] (the groups' rows, one group after the other; what follows is not read) and `groups` [4 · (rows // 2)] ((start in `members`,
+    rows, tokens, the block-table row of one of them) a group, zeros behind the last). Host: `rows`, and `longest_own`, the most tokens any row has beside those it shares."""
 
     __slots__ = ("skip", "members", "groups", "rows", "longest_own")
 
@@ -59,9 +59,9 @@ class SharedPrefix:
         self.skip, self.members, self.groups, self.rows, self.longest_own = skip, members, groups, rows, longest_own
 
     @classmethod
-    def find(cls, table: np.ndarray, kv_len: np.ndarray, page_size: int) -> dict | None:
-        """The arrays (host) and `longest_own` for rows that hold `kv_len` tokens in the pages `table` [rows, pages]; None where
-        no group is worth it. Rows that share more with some than with others go with the cut that saves most."""
+    def find(cls, table: np.ndarray, kv_len: np.ndarray, page_size: int, row_slot: np.ndarray) -> dict | None:
+        """The arrays (host) and `longest_own` for rows that hold `kv_len` tokens in the pages `table` [rows, pages], the rows
+        `row_slot` of the block table; None where no group is worth it. Rows that share more with some than with others go with the cut that saves most."""
         n = len(kv_len)
         limit = np.maximum((np.asarray(kv_len, dtype=np.int64) - 1) // page_size, 0)      # (a row's last token stays its own)
         first = table[:, 0] if n > 1 and table.shape[1] else np.zeros(0, dtype=np.int32)
@@ -72,12 +72,12 @@ class SharedPrefix:
             found += cls._cut(rows, table, limit, 0, page_size)[1]
         if not found:
             return None
-        skip, members, groups = np.zeros(n, dtype=np.int32), np.zeros(n, dtype=np.int32), np.zeros(3 * (n // 2), dtype=np.int32)
+        skip, members, groups = np.zeros(n, dtype=np.int32), np.zeros(n, dtype=np.int32), np.zeros(4 * (n // 2), dtype=np.int32)
         at = 0
         for i, (rows, pages) in enumerate(found):
             skip[rows] = pages * page_size
             members[at:at + len(rows)] = rows
-            groups[3 * i:3 * i + 3] = at, len(rows), pages * page_size
+            groups[4 * i:4 * i + 4] = at, len(rows), pages * page_size, row_slot[rows[0]]
             at += len(rows)
         return {"skip": skip, "members": members, "groups": groups, "longest_own": int((np.asarray(kv_len) - skip).max())}
 
@@ -104,9 +104,9 @@ class SharedPrefix:
         return apart if apart[0] > whole[0] else whole
 
     @classmethod
-    def of(cls, table: np.ndarray, kv_len: np.ndarray, page_size: int, device) -> "SharedPrefix | None":
-        """`find`, its arrays on the device."""
-        found = cls.find(table, kv_len, page_size)
+    def of(cls, table: np.ndarray, kv_len: np.ndarray, page_size: int, device, row_slot: np.ndarray | None = None) -> "SharedPrefix | None":
+        """`find`, its arrays on the device. `row_slot` None: `table` is the block table itself, a row of the step a row of it."""
+        found = cls.find(table, kv_len, page_size, np.arange(len(kv_len)) if row_slot is None else row_slot)
         if found is None:
             return None
         on = [torch.from_numpy(found[name]).to(device) for name in ("skip", "members", "groups")]

@@ -55,7 +55,7 @@ class Runner:
         tables = sum(s * (group.max_pages + 1) + 8 for group in cache.groups)     # every block-table row changed at once
         self._sharing = [group.index for group in cache.groups if build_ctx.shared_prefix and isinstance(group.decl, PagedKV)
                          and group.decl.window <= 0]              # groups whose rows are looked over for pages that they share
-        self.uploader = Uploader(t * (3 + g) + 16 * s + 64 + tables + len(self._sharing) * (4 * s + 16), self.device)
+        self.uploader = Uploader(t * (3 + g) + 16 * s + 64 + tables + len(self._sharing) * (5 * s + 16), self.device)
         self.vocab = model.spec.vocab
         self._reads = None                                        # what recorded steps read (None: not looked at)
         self._use_graphs = self._graphs and Reads.declared(model) # whether steps may be recorded, as far as known
@@ -141,7 +141,7 @@ class Runner:
         one = n_decode + pad_rows
         sharing = {}
         for i in self._sharing if n_decode > 1 else ():
-            found = SharedPrefix.find(c.groups[i].table[row_slot[:one]], kv_len[:one], c.groups[i].page_size)
+            found = SharedPrefix.find(c.groups[i].table[row_slot[:one]], kv_len[:one], c.groups[i].page_size, row_slot)
             if found is not None:
                 sharing[i] = found
                 for name in ("skip", "members", "groups"):

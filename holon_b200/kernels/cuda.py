@@ -224,10 +224,19 @@ class CudaKernels:
         if fn is None:
             fn = self._fn[name] = getattr(self.lib, name)
             fn.restype = ctypes.c_int
+            if name in self.ARGUMENTS:
+                fn.argtypes = [{"p": ctypes.c_void_p, "i": ctypes.c_int, "f": ctypes.c_float}[c] for c in self.ARGUMENTS[name] + "p"]
         code = fn(*args, ctypes.c_void_p(self._stream()))
         self.launches += 1
         if code:
             raise KernelError(f"{name}: {self.lib.hb_last_error().decode()}")
+
+    # The arguments of functions that are handed addresses and numbers as they are (pointer, int, float; behind them the stream):
+    # a wrapper object an argument is a third of what a small step's call costs the host.
+    ARGUMENTS = {"hb_qk_norm_rope_kv_write8": "pppp" "ii" "pp" "i" "ff" "pp" "iiiiii" "p",
+                 "hb_kv_read": "pi" "pp" "iiiii",
+                 "hb_attention_prefix": "ppp" "ppi" "pi" "pp" "iiiiii" "f" "i",
+                 "hb_attention_rows": "ppp" "i" "pi" "ppp" "iiiiii" "f" "iiii" "p" "pppp" "i"}
 
     def _call_in(self, lib, cache: dict, name: str, *args) -> None:
         """`_call` for a function of another library (an extension's)."""
@@ -319,7 +328,7 @@ class CudaKernels:
     def _check(self, *tensors: torch.Tensor | None) -> None:
         index = self._index
         for t in tensors:
-            if t is None or (t.is_cuda and t.get_device() == index and t.is_contiguous()):
+            if t is None or (t.get_device() == index and t.is_contiguous()):      # (a host tensor's device is -1)
                 continue
             if t.device != self.device:
                 raise KernelError(f"a tensor lives on {t.device}, the kernels run on {self.device}")
@@ -429,38 +438,42 @@ class CudaKernels:
                               "[tokens, heads, head_dim]")
         if bias is not None and (bias.shape != (width,) or bias.dtype != qkv.dtype):
             raise KernelError("qk_norm_rope_kv_write: bias must be one row of qkv's width and dtype")
-        if table is not None and (table.dtype != torch.float32 or table.shape[1] != rotary_dim):
+        if table is not None and (table.dtype != torch.float32 or table.dim() != 2 or table.shape[1] != rotary_dim):
             raise KernelError("qk_norm_rope_kv_write: the rotation table must be float32 [positions, rotary_dim]")
-        if positions.shape != (t,) or write_index is None or write_index.shape != (t,):
+        if write_index is None or positions.shape != (t,) or write_index.shape != (t,) \
+                or positions.dtype != torch.int32 or write_index.dtype != torch.int32:
             raise KernelError("qk_norm_rope_kv_write: positions and write_index are int32 [tokens]")
-        gains = [w for w in (q_weight, k_weight) if w is not None]
-        if any(w.shape != (head_dim,) or w.dtype != gains[0].dtype for w in gains):
-            raise KernelError("qk_norm_rope_kv_write: the two norm weights are [head_dim], of one dtype")
+        if (q_weight is None) != (k_weight is None) \
+                or q_weight is not None and (q_weight.shape != (head_dim,) or k_weight.shape != (head_dim,) or k_weight.dtype != q_weight.dtype):
+            raise KernelError("qk_norm_rope_kv_write: the two norm weights are [head_dim], of one dtype (or there are none)")
         pages, page_size = self._pages8(kv, kv_heads, head_dim)
-        self._call("hb_qk_norm_rope_kv_write8", self._p(q_out), self._p(qkv), self._i32(positions, "positions"), self._p(table),
-                   rotary_dim, table.shape[0] if table is not None else 0, self._p(q_weight), self._p(k_weight),
-                   _code(q_weight) if q_weight is not None else 0, ctypes.c_float(eps), ctypes.c_float(offset), self._p(kv),
-                   self._i32(write_index, "write_index"), pages, page_size, t, heads, kv_heads, head_dim, self._p(bias))
+        address = torch.Tensor.data_ptr
+        self._call("hb_qk_norm_rope_kv_write8", address(q_out), address(qkv), address(positions), address(table) if table is not None else None,
+                   rotary_dim, table.shape[0] if table is not None else 0, address(q_weight) if q_weight is not None else None,
+                   address(k_weight) if k_weight is not None else None, _code(q_weight) if q_weight is not None else 0, eps, offset,
+                   address(kv), address(write_index), pages, page_size, t, heads, kv_heads, head_dim,
+                   address(bias) if bias is not None else None)
 
     @staticmethod
     def _pages8(kv, kv_heads: int, head_dim: int) -> tuple[int, int]:
         """(pages, page size) of an 8-bit cache whose heads are these."""
-        if kv.dim() != 5 or kv.dtype != torch.uint8 or kv.shape[1:3] != (2, kv_heads) or kv.shape[4] != head_dim + 1:
-            raise KernelError(f"an 8-bit cache is uint8 [pages, 2, kv_heads, page_size, head_dim + 1]; got {kv.dtype} {tuple(kv.shape)} for "
+        shape = tuple(kv.shape)
+        if kv.dtype != torch.uint8 or len(shape) != 5 or shape[1] != 2 or shape[2] != kv_heads or shape[4] != head_dim + 1:
+            raise KernelError(f"an 8-bit cache is uint8 [pages, 2, kv_heads, page_size, head_dim + 1]; got {kv.dtype} {shape} for "
                               f"{kv_heads} kv heads of {head_dim}")
-        if head_dim % 16 or kv.shape[3] % 16:
-            raise KernelError(f"an 8-bit cache has head sizes and page sizes that are multiples of 16, not {head_dim} and {kv.shape[3]}")
-        return kv.shape[0], kv.shape[3]
+        if head_dim % 16 or shape[3] % 16:
+            raise KernelError(f"an 8-bit cache has head sizes and page sizes that are multiples of 16, not {head_dim} and {shape[3]}")
+        return shape[0], shape[3]
 
     def kv_read(self, out, kv, pages) -> None:
         """out [n, 2, kv_heads, page_size, head_dim] (bfloat16 or float32) = the values that pages `pages` (int32 [n]) of the
         8-bit cache `kv` stand for; exact in both types. A number that names no page gives zeros."""
         self._check(out, kv, pages)
         count, page_size = self._pages8(kv, kv.shape[2] if kv.dim() == 5 else 0, kv.shape[-1] - 1)
-        if pages.dim() != 1 or out.shape != (pages.shape[0], 2, kv.shape[2], page_size, kv.shape[4] - 1):
+        kv_heads, head_dim = kv.shape[2], kv.shape[4] - 1
+        if pages.dim() != 1 or pages.dtype != torch.int32 or out.shape != (pages.shape[0], 2, kv_heads, page_size, head_dim):
             raise KernelError("kv_read: out must be [n, 2, kv_heads, page_size, head_dim] for int32 pages [n]")
-        self._call("hb_kv_read", self._p(out), _code(out), self._p(kv), self._i32(pages, "pages"), pages.shape[0], count, kv.shape[2],
-                   page_size, kv.shape[4] - 1)
+        self._call("hb_kv_read", out.data_ptr(), _code(out), kv.data_ptr(), pages.data_ptr(), pages.shape[0], count, kv_heads, page_size, head_dim)
 
     def qkv_rope(self, q_out, x, weight, positions, table, rotary_dim, q_weight, k_weight, eps, offset, kv,
                  write_index, heads, kv_heads, head_dim) -> bool:
@@ -557,7 +570,7 @@ class CudaKernels:
             return self._call("hb_attention_f32", self._p(out), self._p(q), self._p(kv), *common, rows.n_decode,
                               rows.n_rows, tiles, *sizes, self._p(sinks))
         if shared is not None and rows.n_decode and self._shares(heads, kv_heads, head_dim, kv, q, out):
-            self._attention_rows(out, q, kv, common, rows, kv_heads, kv.shape[3], scale, 0, sinks, shared)
+            self._attention_rows(out, q, kv, block_table, rows, scale, 0, sinks, shared)
         elif rows.n_decode:
             splits = self.decode_splits(rows.n_decode, heads, kv_heads, rows.max_kv)
             mode = self._decode_mode_of(rows)
@@ -603,17 +616,19 @@ class CudaKernels:
     READ_BACK_TOKENS = 65536                  # tokens of scratch that rows of several tokens read an 8-bit cache back into at once
 
     def _attention8(self, out, q, kv, block_table, rows, scale, window: int, sinks, shared) -> None:
-        t, heads, head_dim = q.shape
+        heads, head_dim = q.shape[1:]
         kv_heads = kv.shape[2] if kv.dim() == 5 else 0
         pages, page_size = self._pages8(kv, kv_heads, head_dim)
-        if q.dtype != torch.bfloat16 or out.dtype != q.dtype or out.shape != q.shape or heads % kv_heads or head_dim > 256:
+        if q.dtype != torch.bfloat16 or out.dtype != torch.bfloat16 or out.shape != q.shape or heads % kv_heads or head_dim > 256:
             raise KernelError("paged_attention: an 8-bit cache takes bfloat16 q and out [tokens, heads, head_dim] with head sizes up to 256")
-        common = (self._i32(block_table, "block_table"), block_table.shape[1], self._i32(rows.row_slot, "row_slot"),
-                  self._i32(rows.query_start, "query_start"), self._i32(rows.kv_len, "kv_len"))
         if rows.n_decode:
             if shared is not None and not self._shares(heads, kv_heads, head_dim, kv, q, out):
                 shared = None
-            self._attention_rows(out, q, kv, common, rows, kv_heads, page_size, scale, window, sinks, shared)
+            self._attention_rows(out, q, kv, block_table, rows, scale, window, sinks, shared)
+        if rows.n_rows == rows.n_decode:
+            return
+        common = (self._i32(block_table, "block_table"), block_table.shape[1], self._i32(rows.row_slot, "row_slot"),
+                  self._i32(rows.query_start, "query_start"), self._i32(rows.kv_len, "kv_len"))
         for first, last, stride in self._read_back_portions(rows, page_size, block_table.shape[1]):
             count = last - first
             back = torch.empty((count * stride, 2, kv_heads, page_size, head_dim), dtype=torch.bfloat16, device=self.device)
@@ -667,27 +682,37 @@ class CudaKernels:
             self._splits[key] = (per_sm * self.sms, part.value, tile.value)
         return self._splits[key]
 
-    def _attention_rows(self, out, q, kv, common, rows, kv_heads: int, page_size: int, scale, window: int, sinks, shared) -> None:
+    def _attention_rows(self, out, q, kv, block_table, rows, scale, window: int, sinks, shared) -> None:
         """The step's one-token rows over 8-bit pages, or over either kind with the beginnings that some of them share."""
-        heads, head_dim, n, kv8 = q.shape[1], q.shape[2], rows.n_decode, int(kv.dtype == torch.uint8)
-        part = (None, None, None, None, 0)
-        longest = rows.max_kv
+        heads, head_dim = q.shape[1:]
+        pages, _, kv_heads, page_size, _ = kv.shape
+        n, kv8 = rows.n_decode, int(kv.dtype == torch.uint8)
+        if not (block_table.dtype == rows.row_slot.dtype == rows.query_start.dtype == rows.kv_len.dtype == torch.int32):
+            raise KernelError("paged_attention: the block table and the rows' numbers must be int32")
+        q_at, kv_at, table, slots, stride = q.data_ptr(), kv.data_ptr(), block_table.data_ptr(), rows.row_slot.data_ptr(), block_table.shape[1]
+        part, longest = (None, None, None, None, 0), rows.max_kv
         if shared is not None:
-            ctas, part_rows, _ = self._prefix_plan(heads // kv_heads, head_dim, page_size)
-            rows_left = self._prefix_units(n, heads, kv_heads, head_dim, page_size) * part_rows
+            self._check(shared.skip, shared.members, shared.groups)
+            if not (shared.skip.dtype == shared.members.dtype == shared.groups.dtype == torch.int32) or shared.skip.shape != (n,) \
+                    or shared.members.shape != (n,) or shared.groups.dim() != 1 or shared.groups.shape[0] < 4 or shared.groups.shape[0] % 4:
+                raise KernelError("paged_attention: shared beginnings are int32: skip [rows], members [rows], groups [4 times as many as there may be]")
+            key = ("shared", n, heads, kv_heads, head_dim, page_size)
+            plan = self._splits.get(key)
+            if plan is None:
+                ctas, part_rows, _ = self._prefix_plan(heads // kv_heads, head_dim, page_size)
+                plan = self._splits[key] = ctas, part_rows, self._prefix_units(n, heads, kv_heads, head_dim, page_size) * part_rows
+            ctas, part_rows, rows_left = plan
             scratch = torch.empty(rows_left * (head_dim + 2) + 4 * n, dtype=torch.float32, device=self.device)
-            part_o, part_ml, part_at = (ctypes.c_void_p(scratch.data_ptr() + 4 * i)
-                                        for i in (0, rows_left * head_dim, rows_left * (head_dim + 2)))
-            self._call("hb_attention_prefix", part_o, part_ml, part_at, self._p(q), self._p(kv), kv8, *common[:3], self._p(shared.members),
-                       self._p(shared.groups), shared.groups.shape[0] // 3, heads, kv_heads, head_dim, kv.shape[0], page_size,
-                       ctypes.c_float(scale), ctas)
-            part = (self._p(shared.skip), part_o, part_ml, part_at, part_rows)
-            longest = shared.longest_own
-        if window > 0:
-            longest = min(longest, window)
-        splits, by_length = self._row_splits(kv8, n, heads, kv_heads, head_dim, longest)
-        self._call("hb_attention_rows", self._p(out), self._p(q), self._p(kv), kv8, *common, n, heads, kv_heads, head_dim, kv.shape[0],
-                   page_size, ctypes.c_float(scale), window, splits, by_length, self._p(sinks), *part)
+            part_o = scratch.data_ptr()
+            part_ml = part_o + 4 * rows_left * head_dim
+            part_at = part_ml + 8 * rows_left
+            self._call("hb_attention_prefix", part_o, part_ml, part_at, q_at, kv_at, kv8, table, stride, shared.members.data_ptr(),
+                       shared.groups.data_ptr(), shared.groups.shape[0] // 4, heads, kv_heads, head_dim, pages, page_size, scale, ctas)
+            part, longest = (shared.skip.data_ptr(), part_o, part_ml, part_at, part_rows), shared.longest_own
+        splits, few, by_length = self._row_splits(kv8, n, heads, kv_heads, head_dim, longest, window, shared is not None)
+        self._call("hb_attention_rows", out.data_ptr(), q_at, kv_at, kv8, table, stride, slots, rows.query_start.data_ptr(),
+                   rows.kv_len.data_ptr(), n, heads, kv_heads, head_dim, pages, page_size, scale, window, splits, few, by_length,
+                   sinks.data_ptr() if sinks is not None else None, *part)
 
     def _prefix_units(self, rows: int, heads: int, kv_heads: int, head_dim: int, page_size: int) -> int:
         """Partial results that `rows` one-token rows may leave at most for what they share, whatever their groups are: a tile for
@@ -700,20 +725,31 @@ class CudaKernels:
         ctas, part_rows, _ = self._prefix_plan(heads // kv_heads, head_dim, page_size)
         return self._prefix_units(rows, heads, kv_heads, head_dim, page_size) * part_rows * (head_dim + 2) + 4 * rows if ctas else 0
 
-    def _row_splits(self, kv8: int, rows: int, heads: int, kv_heads: int, head_dim: int, longest: int) -> tuple[int, int]:
-        """Into how many CTAs (a cluster) the keys of a one-token row are cut: the number with the least waves x (64-key tiles a
-        CTA walks + its start); and whether there are more CTAs than run at once, so that the longest rows should start first."""
-        key = ("rows", kv8, rows, heads, kv_heads, head_dim, -(-longest // 64))
-        if key not in self._splits:
-            group, tiles = heads // kv_heads, max(1, -(-longest // 64))
-            pairs = rows * kv_heads * -(-group // 8)
-            best = (math.inf, 1, 0)
+    FEW_KEYS = 512                            # keys a row up to which the form for few keys pays, where CTAs are more than run at once
+
+    def _row_splits(self, kv8: int, rows: int, heads: int, kv_heads: int, head_dim: int, longest: int, window: int, shared: bool) -> tuple[int, int, int]:
+        """Into how many CTAs (a cluster) the keys of a one-token row are cut: the number with the least waves x (tiles a CTA walks
+        + 4 for its start), and what a cluster costs: 1 tile's time, 4 where every CTA of it also joins shared keys' results. A
+        tile is 128 keys, 64 of bfloat16 heads above 64. Measured: one row of 400 keys of 16 / 8 heads 7.2 us in one CTA, 6.3 in four; 8
+        rows of 8,192 keys 53.5 / 31.0 / 29.7 / 27.4 / 40.9 us in 1 to 5 (the fifth is a second wave); 4 rows with 65 own keys behind
+        1,024 shared ones 12.5 / 13.7 us in 1 and 2. Second: whether they run in the form for few keys, four of whose CTAs an SM
+        holds in place of two: 64 rows with up to 256 own keys 43.2 us with it off, 38.0 on; 64 rows of up to 4,096 keys
+        55 and 69. Third: whether there are more CTAs than run at once, so that the longest rows should start first (64 rows of up
+        to 4,096 keys 54.8 us, in any order 67.0)."""
+        if 0 < window < longest:
+            longest = window + 127                                   # (a window may begin within a tile)
+        key = ("rows", kv8, rows, heads, kv_heads, head_dim, -(-longest // 64), shared)
+        found = self._splits.get(key)
+        if found is None:
+            group, best = heads // kv_heads, (math.inf, 1)
+            pairs, tiles = rows * kv_heads * -(-group // 8), max(1, -(-longest // (128 if kv8 or head_dim <= 64 else 64)))
+            room = lambda s, few=0: int(self.lib.hb_attention_rows_capacity(kv8, few, head_dim, group, s)) * (self.sms if s == 1 else 1)     # noqa: E731
             for s in range(1, min(16, tiles) + 1):
-                room = int(self.lib.hb_attention_rows_capacity(kv8, head_dim, group, s)) * (self.sms if s == 1 else 1)
-                if room > 0:
-                    best = min(best, (-(-pairs // room) * (-(-tiles // s) + 2 + (s > 1)), s, int(pairs > room)))
-            self._splits[key] = best[1:]
-        return self._splits[key]
+                if room(s) > 0:
+                    best = min(best, (-(-pairs // room(s)) * (-(-tiles // s) + 4) + (s > 1) * (4 if shared else 1), s))
+            few = int(longest <= self.FEW_KEYS and best[1] == 1 and pairs > room(1))
+            found = self._splits[key] = best[1], few, int(pairs > room(best[1], few))
+        return found
 
     KV_BUCKET_MIN = 512                       # the smallest number of keys a captured decode launch is planned for
 

@@ -23,16 +23,18 @@ from holon_b200.weights import RandomSource, SafetensorsSource
 def found(held, shared, page=16, pads=0):
     table, count = c8.paged(held, page, len(held), 0, shared)
     table = np.concatenate([table.numpy(), np.full((pads, table.shape[1]), count - 1, dtype=np.int32)])
-    got = SharedPrefix.find(table, np.array(held + [1] * pads, dtype=np.int32), page)
+    slots = np.arange(len(held) + pads)[::-1] + 3
+    got = SharedPrefix.find(table, np.array(held + [1] * pads, dtype=np.int32), page, slots)
     if got is None:
         return None
     n = len(held) + pads
-    assert got["skip"].shape == got["members"].shape == (n,) and got["groups"].shape == (3 * (n // 2),)
+    assert got["skip"].shape == got["members"].shape == (n,) and got["groups"].shape == (4 * (n // 2),)
     assert all(a.dtype == np.int32 for a in (got["skip"], got["members"], got["groups"]))
     out, seen = [], set()
-    for start, count_, tokens in got["groups"].reshape(-1, 3).tolist():
+    for start, count_, tokens, slot in got["groups"].reshape(-1, 4).tolist():
         if count_:
             rows = got["members"][start:start + count_].tolist()
+            assert slot in slots[rows]
             assert count_ > 1 and tokens > 0 and tokens % page == 0 and not seen & set(rows)
             assert all(got["skip"][r] == tokens < held[r] for r in rows)
             assert (table[rows, :tokens // page] == table[rows[0], :tokens // page]).all()
@@ -57,11 +59,11 @@ def test_rows_that_share_more_with_some():
     table, _ = c8.paged([1000] * 6, 16, 6, 0, [(list(range(6)), 4)])
     table = table.numpy()
     table[1, 4:50], table[3, 4:50] = table[0, 4:50], table[2, 4:50]                 # 0 with 1 and 2 with 3 share 46 pages more
-    got = SharedPrefix.find(table, np.full(6, 1000, dtype=np.int32), 16)
-    assert sorted(got["groups"].reshape(-1, 3)[:, 1:].tolist()) == [[0, 0], [2, 800], [2, 800]]
+    got = SharedPrefix.find(table, np.full(6, 1000, dtype=np.int32), 16, np.arange(6))
+    assert sorted(got["groups"].reshape(-1, 4)[:, 1:3].tolist()) == [[0, 0], [2, 800], [2, 800]]
     table[1, 6:], table[3, 6:] = -1, -2                                             # two pages more are not worth a cut
-    got = SharedPrefix.find(table, np.full(6, 1000, dtype=np.int32), 16)
-    assert got["groups"].tolist() == [0, 6, 64] + [0] * 6
+    got = SharedPrefix.find(table, np.full(6, 1000, dtype=np.int32), 16, np.arange(6))
+    assert got["groups"].tolist() == [0, 6, 64, 0] + [0] * 8
 
 
 def test_random_tables():
@@ -159,7 +161,7 @@ def test_generation_with_both(tmp_path):
 
     class Watched(c8.RefKernels8):
         def paged_attention(self, out, q, kv, block_table, rows, scale, window, sinks=None, shared=None):
-            calls.append(None if shared is None else (rows.n_decode, shared.rows, shared.groups.tolist()))
+            calls.append(None if shared is None else (rows.n_decode, shared.rows, shared.groups[:3].tolist()))
             super().paged_attention(out, q, kv, block_table, rows, scale, window, sinks)
 
     for option in (True, False):
@@ -176,7 +178,7 @@ def test_generation_with_both(tmp_path):
         assert len({tuple(got["a", i]) for i in range(1, 5)}) == 1
         hits = [c for c in calls if c is not None]
         assert bool(hits) == option
-        assert not option or (6, 6, [0, 5, 144, 0, 0, 0, 0, 0, 0]) in hits
+        assert not option or (6, 6, [0, 5, 144]) in hits
         calls.clear()
 
 
@@ -187,7 +189,7 @@ class Noted(CudaKernels):
     def __init__(self):
         self.device, self.called, self._pending, self._splits, self.sms = torch.device("cpu"), [], [], {}, 148
         self.prefill_attention, self.prefill_tile, self.attention_bf16 = "tcgen05", None, "fast"
-        self.lib = types.SimpleNamespace(hb_attention_prefix_plan=self.plan, hb_attention_rows_capacity=lambda kv8, dim, group, s: 3 if s == 1 else 400 // s)
+        self.lib = types.SimpleNamespace(hb_attention_prefix_plan=self.plan, hb_attention_rows_capacity=lambda kv8, few, dim, group, s: 3 if s == 1 else 400 // s)
 
     def plan(self, dim, page, group, part_rows, tile_rows):
         part_rows._obj.value, tile_rows._obj.value = 64, 64 // group
@@ -217,7 +219,7 @@ def test_which_kernels_run():
     assert attend([100, 200], [1, 50]) == ["hb_attention_rows", "hb_kv_read_rows", "hb_attention_prefill_tcgen05"]
     assert attend([100, 200], [9, 50], dim=64) == ["hb_kv_read_rows", "hb_attention_prefill_bf16"]
     assert attend([100, 200, 300], [9, 50, 300], dim=64, READ_BACK_TOKENS=400) == ["hb_kv_read_rows", "hb_attention_prefill_bf16"] * 3
-    shared = SharedPrefix(*(torch.zeros(n, dtype=torch.int32) for n in (2, 2, 3)), 2, 50)
+    shared = SharedPrefix(*(torch.zeros(n, dtype=torch.int32) for n in (2, 2, 4)), 2, 50)
     assert attend([300, 400], [1, 1], shared=shared) == ["hb_attention_prefix", "hb_attention_rows"]
     assert attend([300, 400], [1, 1], kv8=False, shared=shared) == ["hb_attention_prefix", "hb_attention_rows"]
     assert attend([300, 400], [1, 1], heads=130, shared=shared) == ["hb_attention_rows"]

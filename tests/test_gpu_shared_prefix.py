@@ -47,7 +47,7 @@ def case(groups, alone, heads, kvh, dim, page, fp8, seed=0, portion=None):
     else:
         kv = torch.randn(count, 2, kvh, page, dim, generator=torch.Generator().manual_seed(seed)).to(BF16)
     q = (1.5 * torch.randn(rows.n_tokens, heads, dim, generator=torch.Generator().manual_seed(seed + 1))).to(BF16)
-    found = SharedPrefix.of(table[rows.row_slot[:rows.n_decode].long()].numpy(), rows.host_kv_len[:rows.n_decode], page, DEV)
+    found = SharedPrefix.of(table[rows.row_slot[:rows.n_decode].long()].numpy(), rows.host_kv_len[:rows.n_decode], page, DEV, rows.row_slot.numpy())
     return q, kv, table, rows, found
 
 
@@ -142,7 +142,7 @@ def test_graph(K, fp8):
         kv = torch.zeros(pages, *cases[0][1].shape[1:], dtype=cases[0][1].dtype, device=DEV)
         from holon_b200.engine.batch import Rows
         rows = Rows(i32(6), torch.arange(7, dtype=torch.int32, device=DEV), i32(6), 6, 6, 6, 1, 2048)
-        return q, kv, i32(7, width), rows, SharedPrefix(i32(6), i32(6), i32(9), 6, 512), torch.zeros_like(q)
+        return q, kv, i32(7, width), rows, SharedPrefix(i32(6), i32(6), i32(12), 6, 512), torch.zeros_like(q)
     def fill(b, c):
         q, kv, table, rows, shared = c
         b[0].copy_(q), b[1][:kv.shape[0]].copy_(kv), b[2].fill_(0)
