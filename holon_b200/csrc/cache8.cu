@@ -6,6 +6,7 @@
 // Read: a page's codes times their scales, as bfloat16 or 32-bit, either for a list of pages or for the pages that rows of
 // several tokens attend over, which then hold zeros behind a row's last key.
 #include "cache8.cuh"
+#include "tcgen05.cuh"
 
 template <typename TW> __device__ __forceinline__ float2 load_w2(const TW* w);
 template <> __device__ __forceinline__ float2 load_w2<float>(const float* w) { return make_float2(w[0], w[1]); }
@@ -112,6 +113,25 @@ template <> __device__ __forceinline__ void load8<float>(const float* w, float (
     f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
 }
 
+// Two numbers in one 64-bit register: an instruction of sm_100 does both (tcgen05.cuh has the names).
+struct Eight {
+    uint64_t v[4];
+    __device__ __forceinline__ Eight() {}
+    __device__ __forceinline__ explicit Eight(const float (&f)[8]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = pack2(f[2 * i], f[2 * i + 1]);
+    }
+    __device__ __forceinline__ void to(float (&f)[8]) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) unpack2(v[i], f[2 * i], f[2 * i + 1]);
+    }
+};
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
 template <typename TW, int LANES>
 __global__ void __launch_bounds__(256, 3) qk_norm_rope_kv_write8_lanes_kernel(
         bf16* __restrict__ q_out, const bf16* __restrict__ qkv, const int32_t* __restrict__ positions,
@@ -147,7 +167,7 @@ __global__ void __launch_bounds__(256, 3) qk_norm_rope_kv_write8_lanes_kernel(
         const bool is_q = head < heads, is_v = head >= heads + kv_heads, turns = !is_v && pairs;
         bool live = inside && u < units;
         int pos = n_pos;
-        float a[8], b[8], wa[8], wb[8], cs[8], sn[8];
+        float a[8], b[8], cs[8], sn[8];
         const TW* weight = is_q ? q_weight : is_v ? nullptr : k_weight;
         if (live && turns) {
             pos = pos < 0 ? 0 : (pos >= max_positions ? max_positions - 1 : pos);
@@ -155,7 +175,6 @@ __global__ void __launch_bounds__(256, 3) qk_norm_rope_kv_write8_lanes_kernel(
             load8<float>(row, cs);
             load8<float>(row + (rotary_dim >> 1), sn);
         }
-        if (live && weight) { load8<TW>(weight + c0, wa); load8<TW>(weight + c1, wb); }
         t += step_t;
         item += step_item;
         if (item >= items) { item -= items; ++t; }
@@ -169,40 +188,61 @@ __global__ void __launch_bounds__(256, 3) qk_norm_rope_kv_write8_lanes_kernel(
 #pragma unroll
             for (int i = 0; i < 8; ++i) { a[i] += x[i]; b[i] += y[i]; }
         }
-        float ss = 0.f;
+        Eight pa(a), pb(b);
+        if (__any_sync(0xffffffffu, weight != nullptr)) {
+            uint64_t sums = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) ss += a[i] * a[i] + b[i] * b[i];
-        if (!inside) ss = 0.f;                                       // (lanes behind the head's end take part with zeros)
+            for (int i = 0; i < 4; ++i) sums = fma2(pa.v[i], pa.v[i], fma2(pb.v[i], pb.v[i], sums));
+            float s0, s1;
+            unpack2(sums, s0, s1);
+            float ss = inside ? s0 + s1 : 0.f;                       // (lanes behind the head's end take part with zeros)
 #pragma unroll
-        for (int o = 1; o < LANES; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        if (weight && live) {
-            const float rstd = rsqrtf(ss / (float)head_dim + eps);
+            for (int o = 1; o < LANES; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            if (weight && live) {
+                const float rstd = rsqrtf(ss / (float)head_dim + eps);
+                const uint64_t r2 = pack2(rstd, rstd), o2 = pack2(offset * rstd, offset * rstd);
+                float wa[8], wb[8];
+                load8<TW>(weight + c0, wa);                          // (few lines, which every unit reads: they are near)
+                load8<TW>(weight + c1, wb);
+                const Eight ga(wa), gb(wb);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) { a[i] *= rstd * (wa[i] + offset); b[i] *= rstd * (wb[i] + offset); }
-        }
-        if (live && turns) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float x = a[i] * cs[i] - b[i] * sn[i];
-                b[i] = b[i] * cs[i] + a[i] * sn[i];
-                a[i] = x;
+                for (int i = 0; i < 4; ++i) {
+                    pa.v[i] = mul2(pa.v[i], fma2(ga.v[i], r2, o2));
+                    pb.v[i] = mul2(pb.v[i], fma2(gb.v[i], r2, o2));
+                }
             }
         }
+        if (live && turns) {
+            const Eight c(cs), n(sn);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint64_t x = mul2(pb.v[i], n.v[i]), y = mul2(pa.v[i], n.v[i]);
+                pa.v[i] = fma2(pa.v[i], c.v[i], x ^ 0x8000000080000000ull);      // a cos - b sin
+                pb.v[i] = fma2(pb.v[i], c.v[i], y);
+            }
+        }
+        pa.to(a);
+        pb.to(b);
         if (live && is_q) {
             bf16* dst = q_out + ((size_t)token * heads + head) * head_dim;
             *(uint4*)(dst + c0) = pack8(a);
             *(uint4*)(dst + c1) = pack8(b);
         }
         if (!__any_sync(0xffffffffu, live && !is_q)) continue;
-        // The largest magnitude by its bits: they order as the numbers do, and what is not finite lies above all that is.
-        uint32_t bits = 0;
-        if (inside)
+        float largest = 0.f, any = 0.f;                              // (a sum is finite unless a number is not, or the numbers nearly are not)
+        if (inside) {
+            uint64_t sums = 0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) bits = max(bits, max(__float_as_uint(a[i]) & 0x7fffffffu, __float_as_uint(b[i]) & 0x7fffffffu));
+            for (int i = 0; i < 4; ++i) sums = add2(sums, add2(pa.v[i], pb.v[i]));
 #pragma unroll
-        for (int o = 1; o < LANES; o <<= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
-        float largest = __uint_as_float(bits);
-        if (__any_sync(0xffffffffu, bits >= 0x7f800000u)) {           // (rows with infinities or NaN: the largest finite one, and NaN for the others)
+            for (int i = 0; i < 8; ++i) largest = fmaxf(largest, fmaxf(fabsf(a[i]), fabsf(b[i])));
+            float s0, s1;
+            unpack2(sums, s0, s1);
+            any = s0 + s1;
+        }
+#pragma unroll
+        for (int o = 1; o < LANES; o <<= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+        if (__any_sync(0xffffffffu, !(fabsf(any) < INFINITY))) {      // (rows with infinities or NaN: the largest finite one, and NaN for the others)
             largest = 0.f;
             if (inside)
 #pragma unroll
@@ -219,9 +259,12 @@ __global__ void __launch_bounds__(256, 3) qk_norm_rope_kv_write8_lanes_kernel(
             if (page < pages) {
                 unsigned char* base = kv + (((size_t)page * 2 + is_v) * kv_heads + (head - heads - (is_v ? kv_heads : 0))) * ((size_t)page_size * (head_dim + 1));
                 const int e = c8_exponent(largest);
-                const float inv = c8_power(-e);
+                const uint64_t inv = pack2(c8_power(-e), c8_power(-e));
+                Eight qa(a), qb(b);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) { a[i] *= inv; b[i] *= inv; }
+                for (int i = 0; i < 4; ++i) { qa.v[i] = mul2(qa.v[i], inv); qb.v[i] = mul2(qb.v[i], inv); }
+                qa.to(a);
+                qb.to(b);
                 unsigned char* row = base + (size_t)off * head_dim;
                 *(uint2*)(row + c0) = make_uint2(c8_pack4_finite(a[0], a[1], a[2], a[3]), c8_pack4_finite(a[4], a[5], a[6], a[7]));
                 *(uint2*)(row + c1) = make_uint2(c8_pack4_finite(b[0], b[1], b[2], b[3]), c8_pack4_finite(b[4], b[5], b[6], b[7]));

@@ -548,7 +548,7 @@ class CudaKernels:
         if shared is not None and (window > 0 or q.dtype != torch.bfloat16 or shared.rows != rows.n_decode):
             raise KernelError("paged_attention: shared beginnings go with bfloat16, without a window, and are those of the step's one-token rows")
         if kv.dtype == torch.uint8:
-            return self._attention8(out, q, kv, block_table, rows, scale, int(window), sinks, shared)
+            return self._attention8(out, q, heads, head_dim, kv, block_table, rows, scale, int(window), sinks, shared)
         if out.shape != q.shape or kv.dtype != q.dtype or out.dtype != q.dtype or kv.shape[4] != head_dim:
             raise KernelError("paged_attention: out and q [tokens, heads, head_dim], kv [pages, 2, kv_heads, page_size, "
                               "head_dim], one dtype")
@@ -569,8 +569,8 @@ class CudaKernels:
                     else rows.n_tokens // 64 + rows.n_rows
             return self._call("hb_attention_f32", self._p(out), self._p(q), self._p(kv), *common, rows.n_decode,
                               rows.n_rows, tiles, *sizes, self._p(sinks))
-        if shared is not None and rows.n_decode and self._shares(heads, kv_heads, head_dim, kv, q, out):
-            self._attention_rows(out, q, kv, block_table, rows, scale, 0, sinks, shared)
+        if shared is not None and rows.n_decode and self._shares(heads // kv_heads, head_dim, kv.shape[3], kv, q, out):
+            self._attention_rows(out, q, kv, 0, (heads, kv_heads, head_dim, kv.shape[0], kv.shape[3]), block_table, rows, scale, 0, sinks, shared)
         elif rows.n_decode:
             splits = self.decode_splits(rows.n_decode, heads, kv_heads, rows.max_kv)
             mode = self._decode_mode_of(rows)
@@ -615,16 +615,15 @@ class CudaKernels:
     # ---- 8-bit pages, shared beginnings
     READ_BACK_TOKENS = 65536                  # tokens of scratch that rows of several tokens read an 8-bit cache back into at once
 
-    def _attention8(self, out, q, kv, block_table, rows, scale, window: int, sinks, shared) -> None:
-        heads, head_dim = q.shape[1:]
+    def _attention8(self, out, q, heads: int, head_dim: int, kv, block_table, rows, scale, window: int, sinks, shared) -> None:
         kv_heads = kv.shape[2] if kv.dim() == 5 else 0
         pages, page_size = self._pages8(kv, kv_heads, head_dim)
         if q.dtype != torch.bfloat16 or out.dtype != torch.bfloat16 or out.shape != q.shape or heads % kv_heads or head_dim > 256:
             raise KernelError("paged_attention: an 8-bit cache takes bfloat16 q and out [tokens, heads, head_dim] with head sizes up to 256")
         if rows.n_decode:
-            if shared is not None and not self._shares(heads, kv_heads, head_dim, kv, q, out):
+            if shared is not None and not self._shares(heads // kv_heads, head_dim, page_size, kv, q, out):
                 shared = None
-            self._attention_rows(out, q, kv, block_table, rows, scale, window, sinks, shared)
+            self._attention_rows(out, q, kv, 1, (heads, kv_heads, head_dim, pages, page_size), block_table, rows, scale, window, sinks, shared)
         if rows.n_rows == rows.n_decode:
             return
         common = (self._i32(block_table, "block_table"), block_table.shape[1], self._i32(rows.row_slot, "row_slot"),
@@ -667,9 +666,9 @@ class CudaKernels:
         whole = -(-longest // page_size) * page_size
         return max(whole, min(rows * whole, self.READ_BACK_TOKENS)) * 2 * kv_heads * head_dim * 2
 
-    def _shares(self, heads: int, kv_heads: int, head_dim: int, kv, q, out) -> bool:
+    def _shares(self, group: int, head_dim: int, page_size: int, kv, q, out) -> bool:
         """Whether the kernels for shared beginnings take these sizes (other sizes attend row by row)."""
-        return kv.shape[3] % 16 == 0 and self._prefix_plan(heads // kv_heads, head_dim, kv.shape[3])[0] > 0 \
+        return page_size % 16 == 0 and self._prefix_plan(group, head_dim, page_size)[0] > 0 \
             and not (kv.data_ptr() | q.data_ptr()) % 16 and out.data_ptr() % 8 == 0
 
     def _prefix_plan(self, group: int, head_dim: int, page_size: int) -> tuple[int, int, int]:
@@ -682,37 +681,44 @@ class CudaKernels:
             self._splits[key] = (per_sm * self.sms, part.value, tile.value)
         return self._splits[key]
 
-    def _attention_rows(self, out, q, kv, block_table, rows, scale, window: int, sinks, shared) -> None:
-        """The step's one-token rows over 8-bit pages, or over either kind with the beginnings that some of them share."""
-        heads, head_dim = q.shape[1:]
-        pages, _, kv_heads, page_size, _ = kv.shape
-        n, kv8 = rows.n_decode, int(kv.dtype == torch.uint8)
-        if not (block_table.dtype == rows.row_slot.dtype == rows.query_start.dtype == rows.kv_len.dtype == torch.int32):
+    def _attention_rows(self, out, q, kv, kv8: int, sizes, block_table, rows, scale, window: int, sinks, shared) -> None:
+        """The step's one-token rows over 8-bit pages (`kv8`), or over either kind with the beginnings that some of them share.
+        `sizes`: heads, kv heads, head size, pages, page size."""
+        n, row_slot, query_start, kv_len, i32 = rows.n_decode, rows.row_slot, rows.query_start, rows.kv_len, torch.int32
+        if block_table.dtype != i32 or row_slot.dtype != i32 or query_start.dtype != i32 or kv_len.dtype != i32:
             raise KernelError("paged_attention: the block table and the rows' numbers must be int32")
-        q_at, kv_at, table, slots, stride = q.data_ptr(), kv.data_ptr(), block_table.data_ptr(), rows.row_slot.data_ptr(), block_table.shape[1]
-        part, longest = (None, None, None, None, 0), rows.max_kv
-        if shared is not None:
-            self._check(shared.skip, shared.members, shared.groups)
-            if not (shared.skip.dtype == shared.members.dtype == shared.groups.dtype == torch.int32) or shared.skip.shape != (n,) \
-                    or shared.members.shape != (n,) or shared.groups.dim() != 1 or shared.groups.shape[0] < 4 or shared.groups.shape[0] % 4:
-                raise KernelError("paged_attention: shared beginnings are int32: skip [rows], members [rows], groups [4 times as many as there may be]")
-            key = ("shared", n, heads, kv_heads, head_dim, page_size)
-            plan = self._splits.get(key)
-            if plan is None:
-                ctas, part_rows, _ = self._prefix_plan(heads // kv_heads, head_dim, page_size)
-                plan = self._splits[key] = ctas, part_rows, self._prefix_units(n, heads, kv_heads, head_dim, page_size) * part_rows
-            ctas, part_rows, rows_left = plan
-            scratch = torch.empty(rows_left * (head_dim + 2) + 4 * n, dtype=torch.float32, device=self.device)
-            part_o = scratch.data_ptr()
-            part_ml = part_o + 4 * rows_left * head_dim
-            part_at = part_ml + 8 * rows_left
-            self._call("hb_attention_prefix", part_o, part_ml, part_at, q_at, kv_at, kv8, table, stride, shared.members.data_ptr(),
-                       shared.groups.data_ptr(), shared.groups.shape[0] // 4, heads, kv_heads, head_dim, pages, page_size, scale, ctas)
-            part, longest = (shared.skip.data_ptr(), part_o, part_ml, part_at, part_rows), shared.longest_own
-        splits, few, by_length = self._row_splits(kv8, n, heads, kv_heads, head_dim, longest, window, shared is not None)
-        self._call("hb_attention_rows", out.data_ptr(), q_at, kv_at, kv8, table, stride, slots, rows.query_start.data_ptr(),
-                   rows.kv_len.data_ptr(), n, heads, kv_heads, head_dim, pages, page_size, scale, window, splits, few, by_length,
-                   sinks.data_ptr() if sinks is not None else None, *part)
+        q_at, kv_at, table, stride = q.data_ptr(), kv.data_ptr(), block_table.data_ptr(), block_table.shape[1]
+        if shared is None:
+            splits, few, by_length = self._row_splits(kv8, n, *sizes[:3], rows.max_kv, window, False)
+            return self._call("hb_attention_rows", out.data_ptr(), q_at, kv_at, kv8, table, stride, row_slot.data_ptr(), query_start.data_ptr(),
+                              kv_len.data_ptr(), n, *sizes, scale, window, splits, few, by_length,
+                              sinks.data_ptr() if sinks is not None else None, None, None, None, None, 0)
+        skip, members, groups = shared.skip, shared.members, shared.groups
+        self._check(skip, members, groups)
+        at_most = groups.shape[0] // 4 if groups.dim() == 1 else 0
+        if skip.dtype != i32 or members.dtype != i32 or groups.dtype != i32 or skip.shape != (n,) or members.shape != (n,) \
+                or at_most < 1 or groups.shape[0] % 4:
+            raise KernelError("paged_attention: shared beginnings are int32: skip [rows], members [rows], groups [4 times as many as there may be]")
+        ctas, part_rows, rows_left = self._prefix_room(n, *sizes)
+        scratch = torch.empty(rows_left * (sizes[2] + 2) + 4 * n, dtype=torch.float32, device=self.device)
+        part_o = scratch.data_ptr()
+        part_ml = part_o + 4 * rows_left * sizes[2]
+        part_at = part_ml + 8 * rows_left
+        self._call("hb_attention_prefix", part_o, part_ml, part_at, q_at, kv_at, kv8, table, stride, members.data_ptr(), groups.data_ptr(),
+                   at_most, *sizes, scale, ctas)
+        splits, few, by_length = self._row_splits(kv8, n, *sizes[:3], shared.longest_own, 0, True)
+        self._call("hb_attention_rows", out.data_ptr(), q_at, kv_at, kv8, table, stride, row_slot.data_ptr(), query_start.data_ptr(),
+                   kv_len.data_ptr(), n, *sizes, scale, 0, splits, few, by_length, sinks.data_ptr() if sinks is not None else None,
+                   skip.data_ptr(), part_o, part_ml, part_at, part_rows)
+
+    def _prefix_room(self, rows: int, heads: int, kv_heads: int, head_dim: int, pages: int, page_size: int) -> tuple[int, int, int]:
+        """(CTAs, query rows a piece of work leaves results for, such rows in all) of the kernel for shared keys."""
+        key = ("prefix room", rows, heads, kv_heads, head_dim, page_size)
+        room = self._splits.get(key)
+        if room is None:
+            ctas, part_rows, _ = self._prefix_plan(heads // kv_heads, head_dim, page_size)
+            room = self._splits[key] = ctas, part_rows, self._prefix_units(rows, heads, kv_heads, head_dim, page_size) * part_rows
+        return room
 
     def _prefix_units(self, rows: int, heads: int, kv_heads: int, head_dim: int, page_size: int) -> int:
         """Partial results that `rows` one-token rows may leave at most for what they share, whatever their groups are: a tile for
