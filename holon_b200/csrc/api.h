@@ -63,11 +63,12 @@ int hb_qk_norm_rope_kv_write8(void* q_out, const void* qkv, const int32_t* posit
 // index that names no page gives zeros.
 int hb_kv_read(void* out, int dtype, const void* kv, const int32_t* index, int count, int pages, int kv_heads, int page_size,
                int head_dim, hb_stream stream);
-// The pages that the new tokens of rows row0 .. rows - 1 see, in bfloat16 for an attention kernel: page i of row b to page
-// (b - row0) * stride + i of out, rows behind a row's last key as zeros, pages before its window not at all. Also makes the
-// tables that go with it: table [rows - row0, stride], slots [rows] (from row0 on). stride: at least the pages of the longest row.
+// The keys and values that the new tokens of rows row0 .. rows - 1 see, in bfloat16 and in a row: out [rows - row0, 2, kv_heads, length,
+// head_dim], with zeros before them from the last multiple of 64 on and behind them up to the next (attention kernels read whole
+// tiles). Also makes the tables with which those find row b's keys as one page of `length` tokens, b - row0: table [rows - row0],
+// slots [rows] (from row0 on). length: at least the longest row's tokens, a multiple of 64.
 int hb_kv_read_rows(void* out, int32_t* table, int32_t* slots, const void* kv, const int32_t* block_table, int table_stride,
-                    const int32_t* row_slot, const int32_t* query_start, const int32_t* kv_len, int row0, int rows, int stride,
+                    const int32_t* row_slot, const int32_t* query_start, const int32_t* kv_len, int row0, int rows, int length,
                     int pages, int kv_heads, int page_size, int head_dim, int window, hb_stream stream);
 
 // Attention of the step's new rows over the paged cache, any sizes, on CUDA cores with 32-bit arithmetic.

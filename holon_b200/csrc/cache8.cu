@@ -341,23 +341,22 @@ template <> __device__ __forceinline__ void store16<float>(float* dst, const uin
     store32(dst + 8, make_uint4(f[8], f[9], f[10], f[11]), make_uint4(f[12], f[13], f[14], f[15]));
 }
 
-// One (part, kv head) block of a page, blockIdx.y's, 16 codes a thread and turn, four turns' loads at once; rows [0, keep) as they are,
-// the others as zeros. per_row: chunks of 16 codes a row, shift its log2 or -1.
+// One (part, kv head) block of a page, blockIdx.y's, to `out`, 16 codes a thread and turn, four turns' loads at once; rows [skip, keep) as
+// they are, the others as zeros, none from `upto` on. shift: log2 of the chunks of 16 codes a row, or -1.
 #define RD_THREADS 128
 #define RD_TURNS 4
 template <typename T>
-__device__ __forceinline__ void read_block(T* __restrict__ out, const unsigned char* __restrict__ kv, bool valid, int keep, int page_size, int head_dim, int shift) {
-    const int per_row = head_dim >> 4, chunks = page_size * per_row;
+__device__ __forceinline__ void read_block(T* __restrict__ out, const unsigned char* __restrict__ kv, bool valid, int skip, int keep, int upto, int page_size, int head_dim, int shift) {
+    const int per_row = head_dim >> 4, chunks = min(page_size, upto) * per_row;
     const size_t blk = blockIdx.y, codes_of = (size_t)page_size * head_dim;
     const unsigned char* b = kv + blk * (codes_of + page_size);
-    out += blk * codes_of;
     for (int i0 = threadIdx.x; i0 < chunks; i0 += RD_THREADS * RD_TURNS) {
         uint4 codes[RD_TURNS];
         float scale[RD_TURNS];
 #pragma unroll
         for (int k = 0; k < RD_TURNS; ++k) {
             const int i = i0 + k * RD_THREADS, r = shift >= 0 ? i >> shift : i / per_row;
-            const bool take = valid && i < chunks && r < keep;
+            const bool take = valid && i < chunks && r >= skip && r < keep;
             codes[k] = take ? *(const uint4*)(b + (size_t)i * 16) : make_uint4(0, 0, 0, 0);
             scale[k] = take ? c8_power((int)b[codes_of + r] - 127) : 0.f;
         }
@@ -373,31 +372,28 @@ __global__ void __launch_bounds__(RD_THREADS) kv_read_kernel(T* __restrict__ out
     const int page = index[blockIdx.x];
     const bool valid = page >= 0 && page < pages;
     const size_t rows = (size_t)gridDim.y * page_size;
-    read_block<T>(out + (size_t)blockIdx.x * rows * head_dim, kv + (valid ? (size_t)page * rows * (head_dim + 1) : 0), valid, page_size, page_size,
-                  head_dim, shift);
+    read_block<T>(out + ((size_t)blockIdx.x * rows + (size_t)blockIdx.y * page_size) * head_dim, kv + (valid ? (size_t)page * rows * (head_dim + 1) : 0),
+                  valid, 0, page_size, page_size, page_size, head_dim, shift);
 }
 
-// Rows row0 .. rows - 1: the pages that hold keys which one of a row's new tokens sees go to out, page i of row b at
-// (b - row0) * stride + i, and the tables with which an attention kernel finds them there are made: table [rows - row0, stride]
-// and slots [rows] (slots[b] = b - row0).
+// Rows row0 .. rows - 1: the keys and values that one of a row's new tokens sees, in a row: out [rows - row0, 2, kv_heads, length,
+// head_dim]. Zeros stand before them from the last multiple of 64 on and behind them up to the next (attention kernels read whole
+// tiles). The tables with which an attention kernel finds row b's keys as one page b - row0 are made, too: table [rows - row0], slots [rows].
 __global__ void __launch_bounds__(RD_THREADS) kv_read_rows_kernel(bf16* __restrict__ out, int32_t* __restrict__ table, int32_t* __restrict__ slots,
                                                                   const unsigned char* __restrict__ kv, const int32_t* __restrict__ block_table,
                                                                   int table_stride, const int32_t* __restrict__ row_slot,
                                                                   const int32_t* __restrict__ query_start, const int32_t* __restrict__ kv_len, int row0,
-                                                                  int stride, int pages, int page_size, int head_dim, int window, int shift) {
+                                                                  int length, int pages, int page_size, int head_dim, int window, int shift) {
     const int r = blockIdx.z, i = blockIdx.x, b = row0 + r;
-    if (threadIdx.x == 0 && blockIdx.y == 0) {
-        table[(size_t)r * stride + i] = r * stride + i;
-        if (i == 0) slots[b] = r;
-    }
+    if (threadIdx.x == 0 && blockIdx.y == 0 && i == 0) { table[r] = r; slots[b] = r; }
     const int n = kv_len[b], first = n - (query_start[b + 1] - query_start[b]);
-    const int lo = window > 0 ? max(0, first - window + 1) : 0;
-    if (i * page_size >= n || (i + 1) * page_size <= lo) return;
-    const int page = block_table[(size_t)row_slot[b] * table_stride + i];
+    const int lo = window > 0 ? max(0, first - window + 1) : 0, at = i * page_size;
+    if (at >= ((n + 63) & ~63) || at + page_size <= (lo & ~63)) return;
+    const int page = at < n && at + page_size > lo ? block_table[(size_t)row_slot[b] * table_stride + i] : -1;
     const bool valid = page >= 0 && page < pages;
     const size_t rows = (size_t)gridDim.y * page_size;
-    read_block<bf16>(out + ((size_t)r * stride + i) * rows * head_dim, kv + (valid ? (size_t)page * rows * (head_dim + 1) : 0), valid,
-                     n - i * page_size, page_size, head_dim, shift);
+    read_block<bf16>(out + (((size_t)r * gridDim.y + blockIdx.y) * length + at) * head_dim, kv + (valid ? (size_t)page * rows * (head_dim + 1) : 0),
+                     valid, lo - at, n - at, length - at, page_size, head_dim, shift);
 }
 
 static int check_pages(const char* who, const void* out, const void* kv, int kv_heads, int page_size, int head_dim) {
@@ -430,14 +426,14 @@ extern "C" int hb_kv_read(void* out, int dtype, const void* kv, const int32_t* i
 }
 
 extern "C" int hb_kv_read_rows(void* out, int32_t* table, int32_t* slots, const void* kv, const int32_t* block_table, int table_stride,
-                               const int32_t* row_slot, const int32_t* query_start, const int32_t* kv_len, int row0, int rows, int stride,
+                               const int32_t* row_slot, const int32_t* query_start, const int32_t* kv_len, int row0, int rows, int length,
                                int pages, int kv_heads, int page_size, int head_dim, int window, hb_stream stream) {
-    if (rows <= row0 || stride < 1) return 0;
+    if (rows <= row0 || length < 1) return 0;
     if (int rc = check_pages("kv_read_rows", out, kv, kv_heads, page_size, head_dim)) return rc;
-    if (stride > table_stride) HB_REFUSE("kv_read_rows: %d pages a row, the block table has %d", stride, table_stride);
+    if (length % 64) HB_REFUSE("kv_read_rows: %d tokens a row are no multiple of 64", length);
     if (rows - row0 > 65535) HB_REFUSE("kv_read_rows: %d rows", rows - row0);
-    kv_read_rows_kernel<<<dim3(stride, 2 * kv_heads, rows - row0), RD_THREADS, 0, (cudaStream_t)stream>>>(
-        (bf16*)out, table, slots, (const unsigned char*)kv, block_table, table_stride, row_slot, query_start, kv_len, row0, stride, pages,
+    kv_read_rows_kernel<<<dim3((length + page_size - 1) / page_size, 2 * kv_heads, rows - row0), RD_THREADS, 0, (cudaStream_t)stream>>>(
+        (bf16*)out, table, slots, (const unsigned char*)kv, block_table, table_stride, row_slot, query_start, kv_len, row0, length, pages,
         page_size, head_dim, window, chunk_shift(head_dim));
     HB_LAUNCH_CHECK("kv_read_rows");
     return 0;

@@ -601,8 +601,8 @@ class CudaKernels:
     def _attention_prompts(self, out, q, kv, common, rows, first: int, last: int, sizes, sinks) -> None:
         """Rows `first` .. `last` - 1, which bring several tokens each, over bfloat16 pages. `common`, `sizes`: the arguments that
         the kernels share."""
-        heads, head_dim = sizes[0], sizes[2]
-        if self.prefill_attention == "tcgen05" and head_dim == 128 and kv.shape[3] % 64 == 0:
+        heads, head_dim, page_size = sizes[0], sizes[2], sizes[4]
+        if self.prefill_attention == "tcgen05" and head_dim == 128 and page_size % 64 == 0:
             tile_q, tiles = 256, self._query_tiles(rows, 256, first, last)
             if self.prefill_tile == 128 or (self.prefill_tile is None and 4 * heads * tiles < 3 * self.sms):              # tiles of 256 queries would leave SMs idle: one group of
                 tile_q, tiles = 128, self._query_tiles(rows, 128, first, last)   # 128 a CTA, twice the CTAs
@@ -628,42 +628,42 @@ class CudaKernels:
             return
         common = (self._i32(block_table, "block_table"), block_table.shape[1], self._i32(rows.row_slot, "row_slot"),
                   self._i32(rows.query_start, "query_start"), self._i32(rows.kv_len, "kv_len"))
-        for first, last, stride in self._read_back_portions(rows, page_size, block_table.shape[1]):
+        for first, last, length in self._read_back_portions(rows, block_table.shape[1] * page_size):
             count = last - first
-            back = torch.empty((count * stride, 2, kv_heads, page_size, head_dim), dtype=torch.bfloat16, device=self.device)
-            tables = torch.empty(count * stride + last, dtype=torch.int32, device=self.device)
-            table, slots = tables[:count * stride], tables[count * stride:]
-            self._call("hb_kv_read_rows", self._p(back), self._p(table), self._p(slots), self._p(kv), *common, first, last, stride, pages,
+            back = torch.empty((count, 2, kv_heads, length, head_dim), dtype=torch.bfloat16, device=self.device)
+            tables = torch.empty(count + last, dtype=torch.int32, device=self.device)
+            table, slots = tables[:count], tables[count:]
+            self._call("hb_kv_read_rows", self._p(back), self._p(table), self._p(slots), self._p(kv), *common, first, last, length, pages,
                        kv_heads, page_size, head_dim, window)
-            self._attention_prompts(out, q, back, (self._p(table), stride, self._p(slots), *common[3:]), rows, first, last,
-                                    (heads, kv_heads, head_dim, count * stride, page_size, ctypes.c_float(scale), window), sinks)
+            common_ = (self._p(table), 1, self._p(slots), *common[3:])       # (a row's keys are one page)
+            self._attention_prompts(out, q, back, common_, rows, first, last, (heads, kv_heads, head_dim, count, length, ctypes.c_float(scale), window), sinks)
 
-    def _read_back_portions(self, rows, page_size: int, most: int):
-        """The rows of several tokens in runs (first, last, pages a row) whose keys are read back at once: as many rows as
-        READ_BACK_TOKENS of scratch hold at the length of the longest, one at least. Where the rows' lengths are not known on the
-        host, or are not those that the launch will meet (a captured step), all at once at the longest there may be."""
+    def _read_back_portions(self, rows, most: int):
+        """The rows of several tokens in runs (first, last, tokens a row, a multiple of 64) whose keys are read back at once: as many
+        rows as READ_BACK_TOKENS of scratch hold at the length of the longest, one at least. Where the rows' lengths are not known on the
+        host, or are not those that the launch will meet (a captured step), all at once at the longest there may be (at most `most`)."""
         if rows.n_rows <= rows.n_decode:
             return
-        pages_of = lambda tokens: min(most, max(1, -(-int(tokens) // page_size)))             # noqa: E731
+        whole = lambda tokens: -(-min(most, max(1, int(tokens))) // 64) * 64                  # noqa: E731
         if rows.host_kv_len is None or "any cut" in rows.plan:
-            yield rows.n_decode, rows.n_rows, pages_of(rows.max_kv)
+            yield rows.n_decode, rows.n_rows, whole(rows.max_kv)
             return
-        first, stride = rows.n_decode, 0
+        first, length = rows.n_decode, 0
         for b in range(rows.n_decode, rows.n_rows):
-            mine = max(stride, pages_of(rows.host_kv_len[b]))
-            if b > first and (b + 1 - first) * mine * page_size > self.READ_BACK_TOKENS:
-                yield first, b, stride
-                first, mine = b, pages_of(rows.host_kv_len[b])
-            stride = mine
-        yield first, rows.n_rows, stride
+            mine = max(length, whole(rows.host_kv_len[b]))
+            if b > first and (b + 1 - first) * mine > self.READ_BACK_TOKENS:
+                yield first, b, length
+                first, mine = b, whole(rows.host_kv_len[b])
+            length = mine
+        yield first, rows.n_rows, length
 
-    def read_back_scratch(self, tokens: int, rows: int, longest: int, kv_heads: int, head_dim: int, page_size: int) -> int:
+    def read_back_scratch(self, tokens: int, rows: int, longest: int, kv_heads: int, head_dim: int) -> int:
         """Bytes of scratch that rows of several tokens take at most for reading an 8-bit cache back (`rows` such rows of up to
         `longest` tokens in a step of `tokens`)."""
         rows = min(rows, tokens // 2)
         if rows < 1:
             return 0
-        whole = -(-longest // page_size) * page_size
+        whole = -(-longest // 64) * 64
         return max(whole, min(rows * whole, self.READ_BACK_TOKENS)) * 2 * kv_heads * head_dim * 2
 
     def _shares(self, group: int, head_dim: int, page_size: int, kv, q, out) -> bool:

@@ -14,6 +14,9 @@ plain copy as the value); `sink` (one learned number per head, stored as `sink`:
 denominator, without key or value and without the score scale); `names` (the stored names of the q, k, v and output
 weights, where they are not `q_proj.weight` and so on); `biases` (q, k and v carry biases, stored under the weights'
 names with `.b` behind the stem, added before norm and rotation; the output projection has none).
+
+With the engine's `cache_dtype` "fp8" the pages hold 8-bit codes with a scale per token and kv head (`PagedKV.fp8`), quantised as they are
+written; with `shared_prefix` one-token rows that hold the same first pages attend to those together (`GroupStep.shared`).
 """
 from __future__ import annotations
 
@@ -94,12 +97,12 @@ class GQA(Part):
 
     def context_scratch(self, tokens: int, rows: int, longest: int) -> int:
         scratch = getattr(self.ctx.kernels, "read_back_scratch", None) if self.fp8 else None
-        return scratch(tokens, rows, longest, self.kv_heads, self.head_dim, self.ctx.page_size) if scratch is not None else 0
+        return scratch(tokens, rows, longest, self.kv_heads, self.head_dim) if scratch is not None else 0
 
     def graph_scratch(self, rows: int, portions: int, longest: int, page_size: int) -> int:
         k, bytes_ = self.ctx.kernels, 0
         if self.fp8:                                                 # (a captured step reads all its portions back at once)
-            bytes_ += portions * -(-longest // page_size) * page_size * 4 * self.kv_heads * self.head_dim
+            bytes_ += portions * -(-longest // 64) * 64 * 4 * self.kv_heads * self.head_dim
         if self.ctx.shared_prefix and hasattr(k, "shared_scratch"):
             bytes_ += 4 * k.shared_scratch(rows, self.heads, self.kv_heads, self.head_dim, page_size)
         return bytes_

@@ -217,6 +217,7 @@ def attend(held, new, dim=128, heads=8, kvh=2, page=64, kv8=True, shared=None, *
 def test_which_kernels_run():
     assert attend([100, 200], [1, 1]) == ["hb_attention_rows"]
     assert attend([100, 200], [1, 50]) == ["hb_attention_rows", "hb_kv_read_rows", "hb_attention_prefill_tcgen05"]
+    assert attend([100, 200], [9, 50], prefill_attention="mma") == ["hb_kv_read_rows", "hb_attention_prefill_bf16"]
     assert attend([100, 200], [9, 50], dim=64) == ["hb_kv_read_rows", "hb_attention_prefill_bf16"]
     assert attend([100, 200, 300], [9, 50, 300], dim=64, READ_BACK_TOKENS=400) == ["hb_kv_read_rows", "hb_attention_prefill_bf16"] * 3
     shared = SharedPrefix(*(torch.zeros(n, dtype=torch.int32) for n in (2, 2, 4)), 2, 50)
@@ -230,13 +231,14 @@ def test_which_kernels_run():
 def test_portions_that_are_read_back_at_once():
     k, rows = Noted(), c8.rows_of([1, 500, 100, 90, 700], [1, 3, 4, 5, 6])
     k.READ_BACK_TOKENS = 1024
-    got = list(k._read_back_portions(rows, 64, 100))
-    assert got == [(1, 3, 8), (3, 4, 2), (4, 5, 11)]
-    assert all((b - a) * s * 64 <= 1024 or b - a == 1 for a, b, s in got)
-    assert max((b - a) * s * 64 for a, b, s in got) * 2 * 2 * 128 * 2 <= k.read_back_scratch(18, 5, 704, 2, 128, 64)
+    got = list(k._read_back_portions(rows, 6400))
+    assert got == [(1, 3, 512), (3, 4, 128), (4, 5, 704)]
+    assert all((b - a) * n <= 1024 or b - a == 1 for a, b, n in got)
+    assert max((b - a) * n for a, b, n in got) * 2 * 2 * 128 * 2 <= k.read_back_scratch(18, 5, 704, 2, 128)
     rows.plan["any cut"], rows.max_kv = True, 1000
-    assert list(k._read_back_portions(rows, 64, 100)) == [(1, 5, 16)] and list(k._read_back_portions(rows, 64, 12)) == [(1, 5, 12)]
-    assert list(k._read_back_portions(c8.rows_of([4, 5], [1, 1]), 64, 9)) == []
+    assert list(k._read_back_portions(rows, 6400)) == [(1, 5, 1024)] and list(k._read_back_portions(rows, 768)) == [(1, 5, 768)]
+    assert list(k._read_back_portions(c8.rows_of([4, 5], [1, 1]), 576)) == []
+    assert k.read_back_scratch(1, 5, 704, 2, 128) == 0
 
 
 def test_a_captured_step_is_planned_for_a_bucket_of_own_keys():

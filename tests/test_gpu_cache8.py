@@ -268,10 +268,11 @@ def test_rows_without_keys_and_pages_that_are_not_there(K):
 
 
 PROMPTS = [([300, 90], [300, 17], 8, 2, 128, 64), ([33, 900, 40], [2, 300, 40], 6, 2, 96, 16), ([1, 700, 64, 650, 400], [1, 1, 2, 650, 64], 4, 4, 128, 128),
-           ([130, 257], [130, 129], 2, 1, 256, 32), ([50, 40], [3, 40], 5, 5, 16, 48)]
+           ([130, 257], [130, 129], 2, 1, 256, 32), ([50, 40], [3, 40], 5, 5, 16, 48), ([130, 300, 700, 2], [129, 256, 5, 2], 8, 8, 128, 16),
+           ([1000, 128], [600, 128], 4, 1, 128, 48), ([2000], [257], 2, 2, 128, 64), ([40, 900], [1, 899], 16, 2, 128, 32)]
 
 
-@pytest.mark.parametrize("window", [0, 37])
+@pytest.mark.parametrize("window", [0, 37, 300])
 @pytest.mark.parametrize("held,new,heads,kvh,dim,page", PROMPTS)
 def test_portions(K, held, new, heads, kvh, dim, page, window, monkeypatch):
     q, kv, table, rows = case(held, new, heads, kvh, dim, page, seed=dim)
@@ -280,19 +281,24 @@ def test_portions(K, held, new, heads, kvh, dim, page, window, monkeypatch):
     whole = run(K, q, kv, table, rows, dim ** -0.5, window, sinks)
     within(whole, want, mass, halves=False)
     monkeypatch.setattr(K, "READ_BACK_TOKENS", 256, raising=False)                      # (a few rows, or one, at a time)
-    assert len(list(K._read_back_portions(rows, page, table.shape[1]))) > 1 or sum(n > 1 for n in new) < 2 or sum(held) < 256
+    assert len(list(K._read_back_portions(rows, table.shape[1] * page))) > 1 or sum(n > 1 for n in new) < 2 or sum(held) < 256
     assert torch.equal(run(K, q, kv, table, rows, dim ** -0.5, window, sinks), whole)
 
 
 def test_portions_behind_what_is_masked(K):
     """Rows of several tokens beside NaN bytes in the tail of their last page."""
-    for dim, page in ((128, 64), (64, 16)):
-        q, kv, table, rows = case([70, 33], [40, 5], 4, 2, dim, page, seed=2)
-        want, mass = c8.attend(q, kv, table, rows, 0.1)
+    for dim, page, window in ((128, 64, 0), (64, 16, 0), (128, 16, 0), (128, 16, 20), (64, 16, 20)):
+        held = [270, 133]
+        q, kv, table, rows = case(held, [40, 5], 4, 2, dim, page, seed=2)
+        want, mass = c8.attend(q, kv, table, rows, 0.1, window)
         flat = kv.view(kv.shape[0], 2, 2, -1)
-        for s, n in zip(rows.row_slot.tolist(), [70, 33]):
+        for s, n, new in zip(rows.row_slot.tolist(), held, (40, 5)):
             flat[table[s, (n - 1) // page], :, :, ((n - 1) % page + 1) * dim:page * dim] = 127
-        within(run(K, q, kv, table, rows, 0.1), want, mass, halves=False)
+            before = n - new - window + 1 if window else 0           # what lies before the first new token's window, too
+            for j in range(before):
+                flat[table[s, j // page], :, :, j % page * dim:(j % page + 1) * dim] = 127
+                flat[table[s, j // page], :, :, page * dim + j % page] = 255
+        within(run(K, q, kv, table, rows, 0.1, window), want, mass, halves=False)
 
 
 def test_attention_refusals(K):

@@ -136,7 +136,7 @@ def test_memory_of_the_largest_steps():
     assert 1.9 < fixed["fp8"] / fixed["auto"] < 2.0
     e = engine(memory_fraction=0.05, cache_dtype="fp8", shared_prefix=True)
     k, m = e.built.ctx.kernels, e.built.memory
-    assert m.activations >= k.read_back_scratch(512, 8, 4096, 2, 128, 64) > 0
+    assert m.activations >= k.read_back_scratch(512, 8, 4096, 2, 128) > 0
     assert m.graphs >= 2 * 4096 * 4 * 2 * 128 + 4 * k.shared_scratch(8, 8, 2, 128, 64)
     with torch.inference_mode():
         out = e.generate([random_prompt(331, 3000, i) for i in range(3)], SamplingParams(temperature=0.0, max_tokens=4, ignore_eos=True))
