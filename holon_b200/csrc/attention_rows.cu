@@ -30,10 +30,8 @@
 #define AR_HEADS 8
 #define AR_BIAS 14.f
 #define AR_BY_LENGTH 1024             // rows up to which a launch may take the longest first
-#ifndef AR_NK
 #define AR_NK(D_PAD, KV8) ((KV8) || (D_PAD) <= 64 ? 2 : 1)
 #define AR_STAGES(BYTES) ((BYTES) <= 16384 ? 4 : (BYTES) <= 32768 ? 3 : 2)
-#endif
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"

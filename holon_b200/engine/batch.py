@@ -49,18 +49,19 @@ class SharedPrefix:
     A group is two or more rows and the tokens that all of them share (whole pages, and fewer than any of them holds); a
     row is in one group at most. Device, int32: `skip` [rows] (tokens that the row shares, 0 outside the groups), `members`
     [rows] (the groups' rows, one group after the other; what follows is not read) and `groups` [4 · (rows // 2)] ((start in `members`,
-    rows, tokens, the block-table row of one of them) a group, zeros behind the last). Host: `rows`, and `longest_own`, the most tokens any row has beside those it shares."""
+    rows, tokens, the block-table row of one of them) a group, zeros behind the last). Host: `rows`; `longest_own`, the most tokens any row
+    has beside those it shares; `saved`, the tokens that are read once in place of again (None: whatever they are, share)."""
 
-    __slots__ = ("skip", "members", "groups", "rows", "longest_own")
+    __slots__ = ("skip", "members", "groups", "rows", "longest_own", "saved")
 
-    LEAST = 256                # tokens that are read once in place of again (over a group's rows but one) from which a group pays
+    LEAST = 256                # tokens that are read once in place of again (over a group's rows but one) from which a group is one
 
-    def __init__(self, skip, members, groups, rows: int, longest_own: int) -> None:
-        self.skip, self.members, self.groups, self.rows, self.longest_own = skip, members, groups, rows, longest_own
+    def __init__(self, skip, members, groups, rows: int, longest_own: int, saved: int | None = None) -> None:
+        self.skip, self.members, self.groups, self.rows, self.longest_own, self.saved = skip, members, groups, rows, longest_own, saved
 
     @classmethod
     def find(cls, table: np.ndarray, kv_len: np.ndarray, page_size: int, row_slot: np.ndarray) -> dict | None:
-        """The arrays (host) and `longest_own` for rows that hold `kv_len` tokens in the pages `table` [rows, pages], the rows
+        """The arrays (host), `longest_own` and `saved` for rows that hold `kv_len` tokens in the pages `table` [rows, pages], the rows
         `row_slot` of the block table; None where no group is worth it. Rows that share more with some than with others go with the cut that saves most."""
         n = len(kv_len)
         limit = np.maximum((np.asarray(kv_len, dtype=np.int64) - 1) // page_size, 0)      # (a row's last token stays its own)
@@ -79,7 +80,8 @@ class SharedPrefix:
             members[at:at + len(rows)] = rows
             groups[4 * i:4 * i + 4] = at, len(rows), pages * page_size, row_slot[rows[0]]
             at += len(rows)
-        return {"skip": skip, "members": members, "groups": groups, "longest_own": int((np.asarray(kv_len) - skip).max())}
+        return {"skip": skip, "members": members, "groups": groups, "longest_own": int((np.asarray(kv_len) - skip).max()),
+                "saved": sum((len(rows) - 1) * pages * page_size for rows, pages in found)}
 
     @staticmethod
     def _alike(rows, table, limit, page: int) -> list[list[int]]:
@@ -110,7 +112,7 @@ class SharedPrefix:
         if found is None:
             return None
         on = [torch.from_numpy(found[name]).to(device) for name in ("skip", "members", "groups")]
-        return cls(*on, len(kv_len), found["longest_own"])
+        return cls(*on, len(kv_len), found["longest_own"], found["saved"])
 
 
 class GroupStep:

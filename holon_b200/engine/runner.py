@@ -53,8 +53,10 @@ class Runner:
         self.device, self.max_step_tokens = build_ctx.device, max_step_tokens
         s, t, g = cache.max_seqs + 1, max_step_tokens, len(cache.groups)
         tables = sum(s * (group.max_pages + 1) + 8 for group in cache.groups)     # every block-table row changed at once
-        self._sharing = [group.index for group in cache.groups if build_ctx.shared_prefix and isinstance(group.decl, PagedKV)
-                         and group.decl.window <= 0]              # groups whose rows are looked over for pages that they share
+        # Groups whose rows are looked over for pages that they share, with the tokens that sharing has to save.
+        least = getattr(build_ctx.kernels, "shared_least", lambda decl: 0)
+        self._sharing = {group.index: least(group.decl) for group in cache.groups if build_ctx.shared_prefix
+                         and isinstance(group.decl, PagedKV) and group.decl.window <= 0}
         self.uploader = Uploader(t * (3 + g) + 16 * s + 64 + tables + len(self._sharing) * (5 * s + 16), self.device)
         self.vocab = model.spec.vocab
         self._reads = None                                        # what recorded steps read (None: not looked at)
@@ -142,7 +144,7 @@ class Runner:
         sharing = {}
         for i in self._sharing if n_decode > 1 else ():
             found = SharedPrefix.find(c.groups[i].table[row_slot[:one]], kv_len[:one], c.groups[i].page_size, row_slot)
-            if found is not None:
+            if found is not None and found["saved"] >= self._sharing[i]:
                 sharing[i] = found
                 for name in ("skip", "members", "groups"):
                     up.put(f"shared.{name}.{i}", found[name])
@@ -162,7 +164,7 @@ class Runner:
                      max(counts), int(kv_len.max()), query_start, kv_len)
         if bucket:
             rows_.plan["any cut"] = True              # (a graph's launches serve every cut of its tokens into its rows)
-        shared = {i: SharedPrefix(*(dev[f"shared.{name}.{i}"] for name in ("skip", "members", "groups")), one, found["longest_own"])
+        shared = {i: SharedPrefix(*(dev[f"shared.{name}.{i}"] for name in ("skip", "members", "groups")), one, found["longest_own"], found["saved"])
                   for i, found in sharing.items()}
         groups = [GroupStep(g.table_device, dev[f"write_index.{g.index}"], g.page_size, g.decl, shared.get(g.index)) for g in c.groups]
         step = StepContext(dev["token_ids"], dev["positions"], dev["logits_index"], rows_, groups, c)

@@ -558,10 +558,15 @@ class CudaKernels:
             and rows.n_decode <= 65535 and heads <= 65535 and not (q.data_ptr() | out.data_ptr() | kv.data_ptr()) % 16
         if not fast and not wide:
             return self._attention_generic(out, q, kv, block_table, rows, scale, window, sinks)
-        kv_heads = kv.shape[2]
+        pages, _, kv_heads, page_size, _ = kv.shape
+        together = fast and shared is not None and rows.n_decode > 0 and self._shares(shared, heads, page_size, kv_heads, head_dim, kv, q, out)
+        if together:
+            self._attention_rows(out, q, kv, 0, (heads, kv_heads, head_dim, pages, page_size), block_table, rows, scale, 0, sinks, shared)
+            if rows.n_rows == rows.n_decode:
+                return
         common = (self._i32(block_table, "block_table"), block_table.shape[1], self._i32(rows.row_slot, "row_slot"),
                   self._i32(rows.query_start, "query_start"), self._i32(rows.kv_len, "kv_len"))
-        sizes = (heads, kv_heads, head_dim, kv.shape[0], kv.shape[3], ctypes.c_float(scale), int(window))
+        sizes = (heads, kv_heads, head_dim, pages, page_size, ctypes.c_float(scale), int(window))
         if wide:
             tiles = 0
             if rows.n_rows > rows.n_decode:              # (without the host's row starts: the most that there can be)
@@ -569,9 +574,7 @@ class CudaKernels:
                     else rows.n_tokens // 64 + rows.n_rows
             return self._call("hb_attention_f32", self._p(out), self._p(q), self._p(kv), *common, rows.n_decode,
                               rows.n_rows, tiles, *sizes, self._p(sinks))
-        if shared is not None and rows.n_decode and self._shares(heads // kv_heads, head_dim, kv.shape[3], kv, q, out):
-            self._attention_rows(out, q, kv, 0, (heads, kv_heads, head_dim, kv.shape[0], kv.shape[3]), block_table, rows, scale, 0, sinks, shared)
-        elif rows.n_decode:
+        if rows.n_decode and not together:
             splits = self.decode_splits(rows.n_decode, heads, kv_heads, rows.max_kv)
             mode = self._decode_mode_of(rows)
             if sinks is None and splits > 1 and mode == "balanced" and rows.n_decode <= self.BALANCED_ROWS:
@@ -621,7 +624,7 @@ class CudaKernels:
         if q.dtype != torch.bfloat16 or out.dtype != torch.bfloat16 or out.shape != q.shape or heads % kv_heads or head_dim > 256:
             raise KernelError("paged_attention: an 8-bit cache takes bfloat16 q and out [tokens, heads, head_dim] with head sizes up to 256")
         if rows.n_decode:
-            if shared is not None and not self._shares(heads // kv_heads, head_dim, page_size, kv, q, out):
+            if shared is not None and not self._shares(shared, heads, page_size, kv_heads, head_dim, kv, q, out):
                 shared = None
             self._attention_rows(out, q, kv, 1, (heads, kv_heads, head_dim, pages, page_size), block_table, rows, scale, window, sinks, shared)
         if rows.n_rows == rows.n_decode:
@@ -666,9 +669,24 @@ class CudaKernels:
         whole = -(-longest // 64) * 64
         return max(whole, min(rows * whole, self.READ_BACK_TOKENS)) * 2 * kv_heads * head_dim * 2
 
-    def _shares(self, group: int, head_dim: int, page_size: int, kv, q, out) -> bool:
-        """Whether the kernels for shared beginnings take these sizes (other sizes attend row by row)."""
-        return page_size % 16 == 0 and self._prefix_plan(group, head_dim, page_size)[0] > 0 \
+    # Bytes of keys and values a layer that have to be spared for shared beginnings to pay: what a second launch, its partial results
+    # and their weighing cost. Of 252 shapes (2 to 64 rows on 512 to 16,384 tokens, heads of 32 to 256, both kinds of pages) sharing always
+    # takes 24% more than the better way in the mean, with this rule 1.6%. Heads of 128 over 8-bit pages: 4 rows on 1,024 tokens
+    # (6 MB spared) 14.0 us together and 8.9 apart; 8 on 8,192 (118 MB) 23.8 and 24.5; 64 on 4,096 (533 MB) 27.8 and 76.4. Tests: 0.
+    SHARED_BYTES = 40_000_000
+
+    def shared_least(self, decl) -> int:
+        """Tokens that a step's rows have to save by what they share, over the pages of `decl` (parts.base.PagedKV)."""
+        return self._shared_least(decl.kv_heads, 2 * (decl.head_dim + 1 if decl.fp8 else 2 * decl.head_dim))
+
+    def _shared_least(self, kv_heads: int, bytes_: int) -> int:
+        return -(-self.SHARED_BYTES // (kv_heads * bytes_))
+
+    def _shares(self, shared, heads: int, page_size: int, kv_heads: int, head_dim: int, kv, q, out) -> bool:
+        """Whether the one-token rows attend to what they share together: where that pays and the kernels take the sizes."""
+        if shared.saved is not None and shared.saved < self._shared_least(kv_heads, 2 * (head_dim + 1 if kv.dtype == torch.uint8 else 2 * head_dim)):
+            return False
+        return page_size % 16 == 0 and self._prefix_plan(heads // kv_heads, head_dim, page_size)[0] > 0 \
             and not (kv.data_ptr() | q.data_ptr()) % 16 and out.data_ptr() % 8 == 0
 
     def _prefix_plan(self, group: int, head_dim: int, page_size: int) -> tuple[int, int, int]:

@@ -41,6 +41,7 @@ def found(held, shared, page=16, pads=0):
             seen |= set(rows)
             out.append((sorted(rows), tokens))
     assert all(got["skip"][r] == 0 for r in range(n) if r not in seen)
+    assert got["saved"] == sum((len(rows) - 1) * tokens for rows, tokens in out)
     assert got["longest_own"] == max(h - int(s) for h, s in zip(held + [1] * pads, got["skip"]))
     return sorted(out)
 
@@ -164,9 +165,13 @@ def test_generation_with_both(tmp_path):
             calls.append(None if shared is None else (rows.n_decode, shared.rows, shared.groups[:3].tolist()))
             super().paged_attention(out, q, kv, block_table, rows, scale, window, sinks)
 
-    for option in (True, False):
+    class Dear(Watched):
+        def shared_least(self, decl):
+            return 5 * 144 + 1                                                       # (the siblings save 4 x 144)
+
+    for option, table in ((True, Watched), (False, Watched), (True, Dear)):
         engine = Engine(EngineConfig(model=str(folder), device="cpu", cache_dtype="fp8", shared_prefix=option, page_size=16, max_seqs=6,
-                                     max_model_len=256, max_step_tokens=256, state_memory=4 << 20), kernels=Watched())
+                                     max_model_len=256, max_step_tokens=256, state_memory=4 << 20), kernels=table())
         engine.add(random_prompt(384, 150, 7), SamplingParams(temperature=0.0, max_tokens=6, n=5, ignore_eos=True), rid="a")
         engine.add(random_prompt(384, 20, 8), SamplingParams(temperature=0.0, max_tokens=6, ignore_eos=True), rid="b")
         got: dict = {}
@@ -177,11 +182,9 @@ def test_generation_with_both(tmp_path):
         assert len(got) == 6 and all(len(t) == 6 for t in got.values())
         assert len({tuple(got["a", i]) for i in range(1, 5)}) == 1
         hits = [c for c in calls if c is not None]
-        assert bool(hits) == option
-        assert not option or (6, 6, [0, 5, 144]) in hits
+        assert bool(hits) == (option and table is Watched)
+        assert not hits or (6, 6, [0, 5, 144]) in hits
         calls.clear()
-
-
 
 
 # ---------------------------------------------------------------- the kernel table's decisions
@@ -226,6 +229,17 @@ def test_which_kernels_run():
     assert attend([300, 400], [1, 1], heads=130, shared=shared) == ["hb_attention_rows"]
     with pytest.raises(KernelError, match="shared beginnings"):
         attend([300, 400, 500], [1, 1, 1], shared=shared)
+
+
+@pytest.mark.parametrize("kv8", [True, False])
+def test_sharing_that_does_not_pay(kv8):
+    least = -(-CudaKernels.SHARED_BYTES // (2 * (258 if kv8 else 512)))
+    decl = types.SimpleNamespace(kv_heads=2, head_dim=128, fp8=kv8)
+    assert Noted().shared_least(decl) == least
+    for saved, both in ((None, True), (least, True), (least - 1, False)):
+        shared = SharedPrefix(*(torch.zeros(n, dtype=torch.int32) for n in (2, 2, 4)), 2, 50, saved)
+        called = attend([200, 200], [1, 1], kv8=kv8, shared=shared, decode_splits=lambda *a: 1, _decode_mode_of=lambda rows: "equal")
+        assert ("hb_attention_prefix" in called) == both and len(called) == 1 + both
 
 
 def test_portions_that_are_read_back_at_once():

@@ -20,6 +20,12 @@ CONFIGS = {"48": SMALL, "128": WIDE}
 NEAR = 5e-2
 
 
+@pytest.fixture(autouse=True)
+def small_groups_share(monkeypatch):
+    from holon_b200.kernels.cuda import CudaKernels
+    monkeypatch.setattr(CudaKernels, "SHARED_BYTES", 0)
+
+
 def made(config, device="cuda:0", **kw):
     args = dict(dtype="bfloat16", page_size=16, max_seqs=8, max_model_len=1024, max_step_tokens=1024, pages=200)
     args.update(kw)

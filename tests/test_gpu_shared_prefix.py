@@ -18,7 +18,10 @@ BF16 = torch.bfloat16
 @pytest.fixture(scope="module")
 def K():
     from holon_b200.kernels import load_kernels
-    return load_kernels(DEV)
+    table = load_kernels(DEV)
+    table.SHARED_BYTES = 0                    # (small groups share, too)
+    yield table
+    del table.SHARED_BYTES
 
 
 def within(got, want, mass):
