@@ -4,7 +4,7 @@ fixed size per request.
 A group is a set of cache entries whose mixers asked for the same thing (`PagedKV`: heads, head size, window; or
 `PagedLatent`: one latent row per token that all heads read). One
 page number of a group names the same page in each of its entries, so a request has one block-table row per group.
-Groups have pools of their own, sized to hold the same number of tokens
+Groups have pools of their own (bytes where a declaration keeps 8-bit codes, else the engine's dtype), sized to hold the same number of tokens
 (core/holon/core/memory.py:327-330; core/holon/core/assembly.py:140-189). A page goes back to its pool when its
 request ends, or, in a group with a window, when every position in it lies before the window of the next token
 (core/holon/core/state.py:398-418, 499-517) and is none of the first ones that the group keeps (`keep_first`: a request's

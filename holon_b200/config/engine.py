@@ -1,6 +1,7 @@
 """Engine settings. Field names and meanings follow the reference's `EngineConfig`
 (core/holon/core/engine.py:61-100), one command-line flag per field; fields of features this engine does not have
-(drafts, kernel pins and preferences, memory tiers, plugin options) are absent."""
+(drafts, kernel pins and preferences, memory tiers, plugin options) are absent, and `cache_dtype` and `shared_prefix` are this
+engine's own."""
 from __future__ import annotations
 
 import dataclasses
