@@ -6,9 +6,11 @@ import pytest
 import torch
 
 import cache8_tools as c8
+import kasovik_tools as kt
+import vobosun_tools as vt
 from helpers import random_prompt
 from holon_b200.engine import Engine, EngineConfig, SamplingParams, StepEntry, build
-from holon_b200.weights import RandomSource
+from holon_b200.weights import RandomSource, SafetensorsSource
 
 pytestmark = pytest.mark.gpu
 SMALL = dict(architectures=["Qwen3ForCausalLM"], num_hidden_layers=2, hidden_size=128, num_attention_heads=6, num_key_value_heads=2, head_dim=48,
@@ -77,6 +79,21 @@ def test_steps_against_the_plain_table(name, page):
     assert gpu.cache.groups[0].kv.dtype == torch.uint8
     for a, b in zip(trace(gpu, [150, 33, 1], 5), trace(cpu, [150, 33, 1], 5)):
         assert off(a, b) <= NEAR
+
+
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("tools,config", [(kt, kt.KA), (kt, kt.KD), (vt, vt.V_ATT)], ids=["kasovik", "kasovik 128", "vobosun"])
+def test_other_models(tmp_path, tools, config, page):
+    """Windows with sinks and values that are the keys before norm; biases and a stretched partial rotation."""
+    folder = tools.make_folder(tmp_path, "x", seed=3, config=config)
+    args = dict(dtype="bfloat16", page_size=page, max_seqs=8, max_model_len=512, max_step_tokens=512, pages=100)
+    with torch.inference_mode():
+        gpu = build(SafetensorsSource(folder), device="cuda:0", cache_dtype="fp8", **args)
+        cpu = build(SafetensorsSource(folder), device="cpu", kernels=c8.RefKernels8(), cache_dtype="fp8", **args)
+    assert gpu.cache.groups[0].kv.dtype == torch.uint8
+    for a, b in zip(trace(gpu, [150, 33, 1], 5), trace(cpu, [150, 33, 1], 5)):
+        assert off(a, b) <= NEAR
+    gpu.cache.check()
 
 
 @pytest.mark.parametrize("fp8", [True, False])
