@@ -284,7 +284,7 @@ extern "C" int hb_qk_norm_rope_kv_write8(void* q_out, const void* qkv, const int
     if (kv && (page_size < 16 || page_size % 16)) HB_REFUSE("qk_norm_rope_kv_write8: page size %d is no multiple of 16", page_size);
     if (rotary_dim < 0 || rotary_dim > head_dim || (rotary_dim & 1))
         HB_REFUSE("qk_norm_rope_kv_write8: rotary_dim %d must be even and at most head_dim %d", rotary_dim, head_dim);
-    if (rotary_dim && !table) HB_REFUSE("qk_norm_rope_kv_write8: a rotation needs its table");
+    if (rotary_dim && (!table || max_positions < 1)) HB_REFUSE("qk_norm_rope_kv_write8: a rotation needs its table");
     if ((q_weight == nullptr) != (k_weight == nullptr)) HB_REFUSE("qk_norm_rope_kv_write8: give both norm weights or none");
     if (kv && !write_index) HB_REFUSE("qk_norm_rope_kv_write8: writing the cache needs write_index");
     if (kv_heads < 1 || heads < 1) HB_REFUSE("qk_norm_rope_kv_write8: %d heads, %d kv heads", heads, kv_heads);

@@ -50,14 +50,16 @@ class SharedPrefix:
     row is in one group at most. Device, int32: `skip` [rows] (tokens that the row shares, 0 outside the groups), `members`
     [rows] (the groups' rows, one group after the other; what follows is not read) and `groups` [4 · (rows // 2)] ((start in `members`,
     rows, tokens, the block-table row of one of them) a group, zeros behind the last). Host: `rows`; `longest_own`, the most tokens any row
-    has beside those it shares; `saved`, the tokens that are read once in place of again (None: whatever they are, share)."""
+    has beside those it shares; `saved`, the tokens that are read once in place of again (None: whatever they are, share);
+    `page_size`, of the pages that the tokens are whole numbers of (0: not known)."""
 
-    __slots__ = ("skip", "members", "groups", "rows", "longest_own", "saved")
+    __slots__ = ("skip", "members", "groups", "rows", "longest_own", "saved", "page_size")
 
     LEAST = 256                # tokens that are read once in place of again (over a group's rows but one) from which a group is one
 
-    def __init__(self, skip, members, groups, rows: int, longest_own: int, saved: int | None = None) -> None:
-        self.skip, self.members, self.groups, self.rows, self.longest_own, self.saved = skip, members, groups, rows, longest_own, saved
+    def __init__(self, skip, members, groups, rows: int, longest_own: int, saved: int | None = None, page_size: int = 0) -> None:
+        self.skip, self.members, self.groups, self.rows = skip, members, groups, rows
+        self.longest_own, self.saved, self.page_size = longest_own, saved, page_size
 
     @classmethod
     def find(cls, table: np.ndarray, kv_len: np.ndarray, page_size: int, row_slot: np.ndarray) -> dict | None:
@@ -112,7 +114,7 @@ class SharedPrefix:
         if found is None:
             return None
         on = [torch.from_numpy(found[name]).to(device) for name in ("skip", "members", "groups")]
-        return cls(*on, len(kv_len), found["longest_own"], found["saved"])
+        return cls(*on, len(kv_len), found["longest_own"], found["saved"], page_size)
 
 
 class GroupStep:

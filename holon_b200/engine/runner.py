@@ -164,7 +164,8 @@ class Runner:
                      max(counts), int(kv_len.max()), query_start, kv_len)
         if bucket:
             rows_.plan["any cut"] = True              # (a graph's launches serve every cut of its tokens into its rows)
-        shared = {i: SharedPrefix(*(dev[f"shared.{name}.{i}"] for name in ("skip", "members", "groups")), one, found["longest_own"], found["saved"])
+        shared = {i: SharedPrefix(*(dev[f"shared.{name}.{i}"] for name in ("skip", "members", "groups")), one, found["longest_own"], found["saved"],
+                                  c.groups[i].page_size)
                   for i, found in sharing.items()}
         groups = [GroupStep(g.table_device, dev[f"write_index.{g.index}"], g.page_size, g.decl, shared.get(g.index)) for g in c.groups]
         step = StepContext(dev["token_ids"], dev["positions"], dev["logits_index"], rows_, groups, c)

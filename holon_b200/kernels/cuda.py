@@ -438,7 +438,7 @@ class CudaKernels:
                               "[tokens, heads, head_dim]")
         if bias is not None and (bias.shape != (width,) or bias.dtype != qkv.dtype):
             raise KernelError("qk_norm_rope_kv_write: bias must be one row of qkv's width and dtype")
-        if table is not None and (table.dtype != torch.float32 or table.dim() != 2 or table.shape[1] != rotary_dim):
+        if table is not None and (table.dtype != torch.float32 or table.dim() != 2 or table.shape[1] != rotary_dim or not len(table)):
             raise KernelError("qk_norm_rope_kv_write: the rotation table must be float32 [positions, rotary_dim]")
         if write_index is None or positions.shape != (t,) or write_index.shape != (t,) \
                 or positions.dtype != torch.int32 or write_index.dtype != torch.int32:
@@ -545,8 +545,10 @@ class CudaKernels:
         t, heads, head_dim = q.shape
         if sinks is not None and (sinks.dtype != torch.float32 or sinks.shape != (heads,)):
             raise KernelError("paged_attention: sinks must be float32 [heads]")
-        if shared is not None and (window > 0 or q.dtype != torch.bfloat16 or shared.rows != rows.n_decode):
-            raise KernelError("paged_attention: shared beginnings go with bfloat16, without a window, and are those of the step's one-token rows")
+        if shared is not None and (window > 0 or q.dtype != torch.bfloat16 or shared.rows != rows.n_decode
+                                   or shared.page_size not in (0, kv.shape[3])):
+            raise KernelError("paged_attention: shared beginnings go with bfloat16, without a window, and are those of the step's one-token rows "
+                              "in pages of the cache's size")
         if kv.dtype == torch.uint8:
             return self._attention8(out, q, heads, head_dim, kv, block_table, rows, scale, int(window), sinks, shared)
         if out.shape != q.shape or kv.dtype != q.dtype or out.dtype != q.dtype or kv.shape[4] != head_dim:

@@ -2,6 +2,7 @@
 engine on the plain kernel table."""
 from __future__ import annotations
 
+import contextlib
 import random
 import types
 
@@ -229,6 +230,19 @@ def test_which_kernels_run():
     assert attend([300, 400], [1, 1], heads=130, shared=shared) == ["hb_attention_rows"]
     with pytest.raises(KernelError, match="shared beginnings"):
         attend([300, 400, 500], [1, 1, 1], shared=shared)
+    shared.page_size = 32                                                            # (whole pages of 32 tokens are none of 64)
+    with pytest.raises(KernelError, match="shared beginnings"):
+        attend([300, 400], [1, 1], shared=shared)
+    assert attend([300, 400], [1, 1], page=32, shared=shared) == ["hb_attention_prefix", "hb_attention_rows"]
+
+
+def test_a_rotation_table_without_rows():
+    k, i32 = Noted(), lambda n: torch.zeros(n, dtype=torch.int32)
+    q, qkv, kv = torch.zeros(1, 2, 32, dtype=torch.bfloat16), torch.zeros(1, 128, dtype=torch.bfloat16), torch.zeros(1, 2, 1, 16, 33, dtype=torch.uint8)
+    for rows in (1, 0):
+        with pytest.raises(KernelError, match="rotation table") if not rows else contextlib.nullcontext():
+            k.qk_norm_rope_kv_write(q, qkv, i32(1), torch.zeros(rows, 32), 32, None, None, 1e-6, 0.0, kv, i32(1), 2, 1, 32)
+    assert k.called == ["hb_qk_norm_rope_kv_write8"]
 
 
 @pytest.mark.parametrize("kv8", [True, False])
