@@ -30,7 +30,7 @@ __device__ __forceinline__ void load_shared_tile(uint32_t k_s, uint32_t v_s, con
     if (ch * W >= a.head_dim) return;
     const int row_bytes = KV8 ? a.head_dim : 2 * a.head_dim;
     const size_t block = (size_t)a.page_size * (KV8 ? a.head_dim + 1 : 2 * a.head_dim), part = (size_t)a.kv_heads * block;
-#pragma unroll
+#pragma unroll 1
     for (int r = threadIdx.x / CPR; r < TILE_N; r += STEP) {
         const int j = j0 + r;
         bool valid = j < hi;
@@ -94,23 +94,23 @@ __global__ void __launch_bounds__(PX_THREADS) prefix_kernel(const PrefixArgs a) 
         cp_async_commit();
         const int32_t* table = a.block_table + (size_t)u.slot * a.table_stride;
         const int first = u.split * all.chunk, last = min((u.tokens + 63) / 64, first + all.chunk);
-        load_shared_tile<D_PAD, KV8>(kv_s, kv_s + TILE_BYTES, a, table, u.hk, first * TILE_N, u.tokens);
-        cp_async_commit();
         uint32_t qf[Q_IN_REGS ? D_PAD / 16 : 1][4];
         float o[D_PAD / 8][4];
 #pragma unroll
         for (int i = 0; i < D_PAD / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
         float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-        for (int tile = first; tile < last; ++tile) {
+        for (int tile = first - 1; tile < last; ++tile) {           // (the turn before the first tile only asks for it: one place loads)
             const uint32_t k_s = kv_s + ((tile - first) & 1) * 2 * TILE_BYTES, v_s = k_s + TILE_BYTES;
-            cp_async_wait<0>();
-            __syncthreads();
+            if (tile >= first) {
+                cp_async_wait<0>();
+                __syncthreads();
+            }
             if (tile + 1 < last) {
                 const uint32_t next = kv_s + ((tile + 1 - first) & 1) * 2 * TILE_BYTES;
                 load_shared_tile<D_PAD, KV8>(next, next + TILE_BYTES, a, table, u.hk, (tile + 1) * TILE_N, u.tokens);
             }
             cp_async_commit();
-            if (warp * 16 >= mrows) continue;                       // (uniform per warp; the barrier is above)
+            if (tile < first || warp * 16 >= mrows) continue;       // (uniform per warp; the barrier is above)
             if (Q_IN_REGS && tile == first) {
 #pragma unroll
                 for (int ks = 0; ks < D_PAD / 16; ++ks)
