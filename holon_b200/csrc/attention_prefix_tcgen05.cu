@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(Shape<KV8>::THREADS, 1) prefix_tcgen05_kernel(
                 const int ch = (part >> 1) * 4 + (sub & 3), v = part & 1;
                 const unsigned char* scales = smem + H::RAWS + s * PT_RAW_STAGE + 2 * PT_RAW_BYTES + v * PT_BN;
                 const uint32_t to0 = dst + v * PT_KV_BYTES + (part >> 1) * (PT_KV_BYTES / 2);
-#pragma unroll 2
+#pragma unroll 1
                 for (int i = 0; i < 8; ++i) {
                     const int row = i * 8 + ((lane >> 3) ^ (sub >> 2) * 5);
                     const uint4 c = ld_shared16(raw + v * PT_RAW_BYTES + row * 128 + ((ch ^ (row & 7)) << 4));

@@ -397,7 +397,7 @@ __global__ void __launch_bounds__(AR_THREADS, D_PAD > 128 ? 1 : FEW ? 4 : 3) row
     using T = Tile<D_PAD, KV8, FEW>;
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     unsigned char* smem = smem_raw + (base - smem_u32(smem_raw));
-    const bool cluster = a.splits > 1;
+    const bool cluster = !FEW && a.splits > 1;                      // (few keys: never cut, so no code for it)
     if (cluster) asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");   // (this CTA runs: waited for before anybody writes here)
     if (threadIdx.x == 0) {
         asm volatile("prefetch.tensormap [%0];\n" ::"l"(&map) : "memory");
@@ -409,7 +409,7 @@ __global__ void __launch_bounds__(AR_THREADS, D_PAD > 128 ? 1 : FEW ? 4 : 3) row
     }
     const int group = a.heads / a.kv_heads, m_tiles = (group + AR_HEADS - 1) / AR_HEADS;
     const int hk = blockIdx.x / m_tiles, g0 = blockIdx.x % m_tiles * AR_HEADS, g = min(AR_HEADS, group - g0);
-    const int split = blockIdx.z, splits = a.splits;
+    const int split = FEW ? 0 : blockIdx.z, splits = FEW ? 1 : a.splits;
     const int b = a.by_length ? row_by_length(smem, a, blockIdx.y) : (int)blockIdx.y;
     const int n = a.kv_len[b], t = a.query_start[b], row_slot = a.row_slot[b];
     const int shared = a.skip ? a.skip[b] : 0;
@@ -582,6 +582,7 @@ extern "C" int hb_attention_rows(void* out, const void* q, const void* kv, int k
     if (kv_heads < 1 || heads < 1 || heads % kv_heads) HB_REFUSE("attention_rows: %d heads, %d kv heads", heads, kv_heads);
     if (page_size < 16 || page_size % 16) HB_REFUSE("attention_rows: page size %d is no multiple of 16", page_size);
     if (splits < 1 || splits > 16) HB_REFUSE("attention_rows: %d splits (1 to 16, a cluster's size)", splits);
+    if (few && splits > 1) HB_REFUSE("attention_rows: the form for few keys does not cut them (%d splits)", splits);
     if (!(scale > 0.f)) HB_REFUSE("attention_rows: the score scale must be positive");
     const int group = heads / kv_heads;
     if (rows > 65535) HB_REFUSE("attention_rows: %d rows", rows);

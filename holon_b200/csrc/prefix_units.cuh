@@ -19,6 +19,14 @@ struct PrefixUnit {
     int start, count, tokens, slot;   // the tile's rows in `members`, the tokens they share, the block table's row where those lie
 };
 
+// a / b for 0 <= a < 2^24, b > 0: an approximate quotient, off by one at most where it is below 2^22, and put right. (Seven
+// divisions stand before a CTA's first load; what they cost is the code that has to come.)
+__device__ __forceinline__ int pu_div(int a, int b) {
+    const int q = (int)__fdividef((float)a, (float)b), rest = a - q * b;
+    return q + (rest >= b ? 1 : rest < 0 ? -1 : 0);
+}
+__device__ __forceinline__ int pu_ceil(int a, int b) { return pu_div(a + b - 1, b); }
+
 // What a lane holds of up to 32 groups, g0 + lane: the first ones are read once (few steps have more).
 struct PrefixGroups {
     const int4* groups;               // [n_groups]: start, count (0: none), tokens, the block table's row of one of them
@@ -28,7 +36,7 @@ struct PrefixGroups {
         const int4 x = g < n_groups ? groups[g] : make_int4(0, 0, 0, 0);
         start = x.x; count = x.y; tokens = x.z; slot = x.w;
         blocks = (tokens + 63) >> 6;
-        tiles = (int)((unsigned)(count + rows_per_tile - 1) / (unsigned)rows_per_tile);
+        tiles = pu_ceil(count, rows_per_tile);
     }
     __device__ __forceinline__ PrefixGroups(const int32_t* groups_, int n, int rows) : groups((const int4*)groups_), n_groups(n), rows_per_tile(rows) {
         read(threadIdx.x & 31);
@@ -56,7 +64,7 @@ __device__ __forceinline__ PrefixUnits prefix_units(const PrefixGroups& all, int
         int units = 0;
         for (int g0 = 0; g0 < all.n_groups; g0 += 32) {
             const PrefixGroups x = all.from(g0);
-            units += x.tiles * (int)((unsigned)(x.blocks + u.chunk - 1) / (unsigned)u.chunk);
+            units += x.tiles * pu_ceil(x.blocks, u.chunk);
         }
         u.units = __reduce_add_sync(0xffffffffu, units) * kv_heads;
         if (u.chunk >= most || u.units <= slots) return u;
@@ -71,7 +79,7 @@ __device__ __forceinline__ PrefixUnit prefix_unit(const PrefixGroups& all, int k
     int before = 0;
     for (int g0 = 0; g0 < all.n_groups; g0 += 32) {
         const PrefixGroups x = all.from(g0);
-        const int splits = (int)((unsigned)(x.blocks + chunk - 1) / (unsigned)chunk), mine = x.tiles * splits * kv_heads;
+        const int splits = pu_ceil(x.blocks, chunk), mine = x.tiles * splits * kv_heads;
         int upto = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -87,10 +95,10 @@ __device__ __forceinline__ PrefixUnit prefix_unit(const PrefixGroups& all, int k
             u.tokens = __shfl_sync(0xffffffffu, x.tokens, src);
             u.slot = __shfl_sync(0xffffffffu, x.slot, src);
             const int in_group = __shfl_sync(0xffffffffu, x.count, src), first_row = __shfl_sync(0xffffffffu, x.start, src);
-            const unsigned rest = want - at, pair = rest / (unsigned)u.splits;    // the unit's (tile, kv head)
-            u.split = (int)(rest - pair * u.splits);
-            u.tile = (int)(pair / (unsigned)kv_heads);
-            u.hk = (int)pair - u.tile * kv_heads;
+            const int rest = want - at, pair = pu_div(rest, u.splits);            // the unit's (tile, kv head)
+            u.split = rest - pair * u.splits;
+            u.tile = pu_div(pair, kv_heads);
+            u.hk = pair - u.tile * kv_heads;
             u.first = at + u.tile * kv_heads * u.splits;
             u.start = first_row + u.tile * all.rows_per_tile;
             u.count = min(all.rows_per_tile, in_group - u.tile * all.rows_per_tile);

@@ -202,15 +202,21 @@ def test_one_token_rows(K, held, heads, kvh, dim, page, window):
     assert torch.equal(got, run(K, q, kv, table, rows, dim ** -0.5, window, sinks))    # (the same bits again)
 
 
-@pytest.mark.parametrize("few", [0, 1])
-@pytest.mark.parametrize("splits", [1, 2, 3, 5, 8, 11, 16])
+@pytest.mark.parametrize("splits,few", [(1, 0), (2, 0), (3, 0), (5, 0), (8, 0), (11, 0), (16, 0), (1, 1)])
 def test_cuts_of_a_row(K, splits, few, monkeypatch):
-    """Any number of CTAs a row, more than it has tiles too, in both forms."""
+    """Any number of CTAs a row, more than it has tiles too; the form for few keys, which is not cut."""
     for held, heads, kvh, dim, page in (([700, 64, 1, 130], 8, 2, 128, 64), ([300, 9], 34, 2, 48, 16), ([2000], 3, 1, 256, 32)):
         q, kv, table, rows = case(held, [1] * len(held), heads, kvh, dim, page, seed=splits)
         monkeypatch.setattr(K, "_row_splits", lambda *a: (splits, few, splits & 1), raising=False)
         want, mass = c8.attend(q, kv, table, rows, dim ** -0.5)
         within(run(K, q, kv, table, rows, dim ** -0.5), want, mass, halves=True)
+
+
+def test_the_form_for_few_keys_refuses_cuts(K, monkeypatch):
+    q, kv, table, rows = case([700], [1], 8, 2, 128, 64, seed=1)
+    monkeypatch.setattr(K, "_row_splits", lambda *a: (2, 1, 0), raising=False)
+    with pytest.raises(KernelError, match="few keys"):
+        run(K, q, kv, table, rows, 1.0)
 
 
 def test_scales_far_apart(K):
