@@ -671,22 +671,23 @@ class CudaKernels:
         whole = -(-longest // 64) * 64
         return max(whole, min(rows * whole, self.READ_BACK_TOKENS)) * 2 * kv_heads * head_dim * 2
 
-    # Bytes of keys and values a layer that have to be spared for shared beginnings to pay: what a second launch, its partial results
-    # and their weighing cost. Of 252 shapes (2 to 64 rows on 512 to 16,384 tokens, heads of 32 to 256, both kinds of pages) sharing always
-    # takes 24% more than the better way in the mean, with this rule 1.6%. Heads of 128 over 8-bit pages: 4 rows on 1,024 tokens
-    # (6 MB spared) 14.0 us together and 8.9 apart; 8 on 8,192 (118 MB) 23.8 and 24.5; 64 on 4,096 (533 MB) 27.8 and 76.4. Tests: 0.
-    SHARED_BYTES = 40_000_000
+    # Bytes of keys and values a layer that have to be spared for shared beginnings to pay (bfloat16 pages, 8-bit ones): what a second
+    # launch, its partial results and their weighing cost. Of 306 shapes (2 to 64 rows on 512 to 16,384 tokens, heads of 32 to 256,
+    # both kinds of pages; other kernels in between, as in a model) sharing always takes 32% more than the better way in the mean, with
+    # this rule 1.9%. 32 heads over 8 kv heads of 128: bfloat16, 8 rows on 2,048 tokens (59 MB spared) 16.9 us together and 16.3 apart, 64
+    # on 512 (132 MB) 23.8 and 33.0; 8-bit, 32 rows on 1,024 (66 MB) 21.7 and 14.8, 64 on 1,024 (133 MB) 25.3 and 29.3. Tests: 0, 0.
+    SHARED_BYTES = 40_000_000, 80_000_000
 
     def shared_least(self, decl) -> int:
         """Tokens that a step's rows have to save by what they share, over the pages of `decl` (parts.base.PagedKV)."""
-        return self._shared_least(decl.kv_heads, 2 * (decl.head_dim + 1 if decl.fp8 else 2 * decl.head_dim))
+        return self._shared_least(decl.kv_heads, decl.head_dim, decl.fp8)
 
-    def _shared_least(self, kv_heads: int, bytes_: int) -> int:
-        return -(-self.SHARED_BYTES // (kv_heads * bytes_))
+    def _shared_least(self, kv_heads: int, head_dim: int, kv8: bool) -> int:
+        return -(-self.SHARED_BYTES[kv8] // (kv_heads * 2 * (head_dim + 1 if kv8 else 2 * head_dim)))
 
     def _shares(self, shared, heads: int, page_size: int, kv_heads: int, head_dim: int, kv, q, out) -> bool:
         """Whether the one-token rows attend to what they share together: where that pays and the kernels take the sizes."""
-        if shared.saved is not None and shared.saved < self._shared_least(kv_heads, 2 * (head_dim + 1 if kv.dtype == torch.uint8 else 2 * head_dim)):
+        if shared.saved is not None and shared.saved < self._shared_least(kv_heads, head_dim, kv.dtype == torch.uint8):
             return False
         return page_size % 16 == 0 and self._prefix_plan(heads // kv_heads, head_dim, page_size)[0] > 0 \
             and not (kv.data_ptr() | q.data_ptr()) % 16 and out.data_ptr() % 8 == 0

@@ -247,7 +247,7 @@ def test_a_rotation_table_without_rows():
 
 @pytest.mark.parametrize("kv8", [True, False])
 def test_sharing_that_does_not_pay(kv8):
-    least = -(-CudaKernels.SHARED_BYTES // (2 * (258 if kv8 else 512)))
+    least = -(-CudaKernels.SHARED_BYTES[kv8] // (2 * (258 if kv8 else 512)))
     decl = types.SimpleNamespace(kv_heads=2, head_dim=128, fp8=kv8)
     assert Noted().shared_least(decl) == least
     for saved, both in ((None, True), (least, True), (least - 1, False)):

@@ -25,7 +25,7 @@ NEAR = 5e-2
 @pytest.fixture(autouse=True)
 def small_groups_share(monkeypatch):
     from holon_b200.kernels.cuda import CudaKernels
-    monkeypatch.setattr(CudaKernels, "SHARED_BYTES", 0)
+    monkeypatch.setattr(CudaKernels, "SHARED_BYTES", (0, 0))
 
 
 def made(config, device="cuda:0", **kw):

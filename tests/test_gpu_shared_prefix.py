@@ -19,7 +19,7 @@ BF16 = torch.bfloat16
 def K():
     from holon_b200.kernels import load_kernels
     table = load_kernels(DEV)
-    table.SHARED_BYTES = 0                    # (small groups share, too)
+    table.SHARED_BYTES = 0, 0                 # (small groups share, too)
     yield table
     del table.SHARED_BYTES
 
