@@ -30,7 +30,7 @@ __device__ __forceinline__ void load_shared_tile(uint32_t k_s, uint32_t v_s, con
     if (ch * W >= a.head_dim) return;
     const int row_bytes = KV8 ? a.head_dim : 2 * a.head_dim;
     const size_t block = (size_t)a.page_size * (KV8 ? a.head_dim + 1 : 2 * a.head_dim), part = (size_t)a.kv_heads * block;
-#pragma unroll 1
+#pragma unroll 4
     for (int r = threadIdx.x / CPR; r < TILE_N; r += STEP) {
         const int j = j0 + r;
         bool valid = j < hi;
