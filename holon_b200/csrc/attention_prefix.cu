@@ -4,7 +4,9 @@
 // Any head size that is a multiple of 16 up to 256, any page size that the caches take; mma.sync m16n8k16 on bfloat16, codes turned
 // into bfloat16 (exactly) as a tile is loaded. A persistent CTA of four warps takes 64 query rows against a unit's blocks of 64 keys.
 // Bound by mma.sync and the loads that feed it (nothing overlaps a CTA's copies but the other CTAs of its SM): with the rows' own keys behind
-// it 64 rows on 8,192 tokens take 87 us over 8-bit pages of 16 tokens (row by row 230), 32 rows on 16,384 70 us over bfloat16 ones (346).
+// it 64 rows on 8,192 tokens take 71 us over 8-bit pages of 16 tokens (row by row 230), 32 rows on 16,384 71 us over bfloat16 ones (346).
+// Tiles are loaded at one place in the code, four rows a thread at a time: all of a thread's rows at two places was code that took
+// up to 15 us to come from memory (heads of 256, between other kernels), one row at a time 126 us in place of 71.
 #include "attention_mma.cuh"
 #include "cache8.cuh"
 #include "prefix_units.cuh"

@@ -12,11 +12,12 @@
 // 128 query rows, and registers that it does not have).
 // Barriers keep their phases from unit to unit; every role counts the tiles that it has seen.
 //
-// Measured, with 32 heads over 8 kv heads and with the rows' own keys behind it: 64 rows on 8,192 tokens of 8-bit pages 38.2 us (in the mma.sync
-// kernel 110, row by row 139), 32 rows on 16,384 of bfloat16 37.1 us (86; 246). Of the first one's 37,000 cycles here, 6,000 go by before a
-// unit is known and 2,400 before its first keys are there, 8 tiles take 2,400 each (24 products, 100 cycles apiece: more than their
+// Measured, with 32 heads over 8 kv heads and with the rows' own keys behind it: 64 rows on 8,192 tokens of 8-bit pages 35.3 us (in the mma.sync
+// kernel 71, row by row 139), 32 rows on 16,384 of bfloat16 35.3 us (71; 246). Of the first one's 35,000 cycles here about 6,000 go by before
+// a unit is known and 2,400 before its first keys are there, 8 tiles take 2,400 each (24 products, 100 cycles apiece: more than their
 // arithmetic, whatever their shape), and 3,800 the results (19 MB of all CTAs). bfloat16 tiles come every 1,650, HBM's rate.
-// Looking the unit up in one warp only and with cheaper divisions made the launch 0.8 us slower: cold code and constants are the time.
+// Between other kernels it takes 2 to 4 us more: its code comes from memory anew, so loops that can do without are not unrolled.
+// Looking the unit up in one warp for all (the look-up twice in the code) made the launch 0.8 us slower.
 #include "cache8.cuh"
 #include "prefix_units.cuh"
 #include "tcgen05.cuh"

@@ -20,11 +20,11 @@
 // 2 c + 1, 2 c + 8, 2 c + 9, so queries are laid out in that order; of values it gets two neighbouring codes of two keys, one byte
 // permutation pairs the keys, and the even numbers of the head are the product's rows 0 - 7, the odd ones its rows 8 - 15.
 //
-// Measured with 32 heads over 8 kv heads of 128, 8-bit pages of 64: 64 rows of 600 to 4,096 tokens 55.3 us (312 MB, 5.6 TB/s, 87% of
-// what a copy reaches), 8 rows of 8,192 27.9 us (135 MB, 4.9 TB/s): bound by HBM and, below some 30 us, by a CTA's start (three loads that
+// Measured with 32 heads over 8 kv heads of 128, 8-bit pages of 64: 64 rows of 600 to 4,096 tokens 55.5 us (312 MB, 5.6 TB/s, 87% of
+// what a copy reaches), 8 rows of 8,192 28.3 us (135 MB, 4.8 TB/s): bound by HBM and, below some 30 us, by a CTA's start (three loads that
 // wait for one another, 1.8 us) and end. One row of 400 tokens 6.6 us: only start and end. Heads as columns and tiles by TMA in place of
 // heads as padded rows and cp.async: 8 rows of 8,192 tokens 52.0 -> 28.8 us, 64 rows 144.5 -> 67.8; longest rows first 67.0 -> 54.8.
-// Behind a shared beginning of 8,192 tokens (64 rows with up to 256 keys of their own) about 14 us, of which 3 weigh 19 MB of partial results.
+// Behind a shared beginning of 8,192 tokens (64 rows with up to 256 keys of their own) about 12 us, of which 3 weigh 19 MB of partial results.
 #include <cuda_fp16.h>
 
 #include "attention_mma.cuh"
