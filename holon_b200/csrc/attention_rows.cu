@@ -29,11 +29,13 @@
 
 #include "attention_mma.cuh"
 #include "cache8.cuh"
+#include "prefix_units.cuh"
 #include "tcgen05.cuh"
 
 #define AR_WARPS 4                    // that compute; one more loads
 #define AR_THREADS (32 * AR_WARPS + 32)
 #define AR_HEADS 8
+#define AR_CLUSTER 16                 // splits at most
 #define AR_BIAS 14.f
 #define AR_BY_LENGTH 1024             // rows up to which a launch may take the longest first
 #define AR_NK(D_PAD, KV8) ((KV8) || (D_PAD) <= 64 ? 2 : 1)
@@ -395,6 +397,7 @@ template <int D_PAD, bool KV8, bool FEW>
 __global__ void __launch_bounds__(AR_THREADS, D_PAD > 128 ? 1 : FEW ? 4 : 3) rows_kernel(const __grid_constant__ CUtensorMap map, const RowsArgs a) {
     extern __shared__ unsigned char smem_raw[];
     using T = Tile<D_PAD, KV8, FEW>;
+    static_assert(T::SUMS + 4 * AR_HEADS * ((FEW ? AR_WARPS : AR_CLUSTER) + PU_MOST_PARTS) <= T::BODY, "the join's weights lie between the sums and `whole`");
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     unsigned char* smem = smem_raw + (base - smem_u32(smem_raw));
     const bool cluster = !FEW && a.splits > 1;                      // (few keys: never cut, so no code for it)
@@ -428,7 +431,7 @@ __global__ void __launch_bounds__(AR_THREADS, D_PAD > 128 ? 1 : FEW ? 4 : 3) row
     // the numbers of all splits. The shared keys' partial results join the last step, and the sink.
     const float* wo = (const float*)smem;                           // [warp][8][D_PAD], then [warp][g][2]
     const float* wml = wo + AR_WARPS * AR_HEADS * D_PAD;
-    float* weights = (float*)(smem + T::SUMS);
+    float* weights = (float*)(smem + T::SUMS);                      // [g][pieces + parts]: room for PU_MOST_PARTS, which bounds the shared keys' units
     float* whole = (float*)(smem + T::BODY);                        // [8][2], over the scales, which are done
     float* recv_o = (float*)(smem + T::RECV);                       // [splits][share], then [splits][g][2]: what the others send
     const int total = g * a.head_dim, share = ((total + splits - 1) / splits + 3) & ~3;
@@ -509,7 +512,7 @@ static int launch_rows(RowsArgs* a, int rows, int splits, int group, int head_di
     int device = 0;
     HB_CUDA(cudaGetDevice(&device));
     if (device >= 64 || !(prepared >> device & 1)) {
-        HB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)rows_smem<D_PAD, KV8, FEW>(16, AR_HEADS, D_PAD)));
+        HB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)rows_smem<D_PAD, KV8, FEW>(AR_CLUSTER, AR_HEADS, D_PAD)));
         HB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
         if (device < 64) prepared |= 1ull << device;
     }
@@ -564,7 +567,7 @@ static int forms(int kv8, int few, RowsArgs* a, int rows, int splits, int group,
 // Clusters of `splits` CTAs that run at once (splits 1: CTAs an SM); -1 where the sizes are refused.
 extern "C" int hb_attention_rows_capacity(int kv8, int few, int head_dim, int group, int splits) {
     int n = 0;
-    if (head_dim < 16 || head_dim > 256 || head_dim % 16 || group < 1 || splits < 1 || splits > 16) return -1;
+    if (head_dim < 16 || head_dim > 256 || head_dim % 16 || group < 1 || splits < 1 || splits > AR_CLUSTER) return -1;
     if (forms(kv8, few, nullptr, 1, splits, group, head_dim, &n, 0) != 0) {
         (void)cudaGetLastError();
         return 0;
@@ -581,7 +584,7 @@ extern "C" int hb_attention_rows(void* out, const void* q, const void* kv, int k
     if (head_dim % 16 || head_dim > 256 || head_dim < 16) HB_REFUSE("attention_rows: head_dim %d is no multiple of 16 up to 256", head_dim);
     if (kv_heads < 1 || heads < 1 || heads % kv_heads) HB_REFUSE("attention_rows: %d heads, %d kv heads", heads, kv_heads);
     if (page_size < 16 || page_size % 16) HB_REFUSE("attention_rows: page size %d is no multiple of 16", page_size);
-    if (splits < 1 || splits > 16) HB_REFUSE("attention_rows: %d splits (1 to 16, a cluster's size)", splits);
+    if (splits < 1 || splits > AR_CLUSTER) HB_REFUSE("attention_rows: %d splits (1 to 16, a cluster's size)", splits);
     if (few && splits > 1) HB_REFUSE("attention_rows: the form for few keys does not cut them (%d splits)", splits);
     if (!(scale > 0.f)) HB_REFUSE("attention_rows: the score scale must be positive");
     const int group = heads / kv_heads;

@@ -5,10 +5,12 @@
 // (tile, kv head) into units of `chunk` blocks of 64 keys. chunk is the least for which all units are at most as many as the
 // launch's slots (sum over tiles of ceil(blocks / chunk) <= sum(blocks) / chunk + tiles: a few tries tell), or all of them where there
 // are more tiles than that. Units are numbered tile by tile, kv head by kv head; a partial result goes to the slot of its unit's number.
+// No (tile, kv head) is cut into more than PU_MOST_PARTS units: attention_rows.cu weighs them in shared memory that holds so many.
 #pragma once
 #include "common.cuh"
 
 #define PU_MIN_CHUNK 2                // blocks of 64 keys a unit has at least
+#define PU_MOST_PARTS 240             // units of a (tile, kv head) at most; reached with one kv head off tcgen05 alone (296 slots)
 
 struct PrefixUnits {
     int units, chunk;                 // of all tiles and kv heads; blocks of 64 keys a unit
@@ -48,6 +50,25 @@ struct PrefixGroups {
     }
 };
 
+// The numbers of blocks a unit that are tried, from `least` to `most`, for `tiles` tiles of `blocks` blocks together, the longest of `longest`
+// blocks, and `each` slots a kv head.
+struct PrefixChunks {
+    int least, most;
+    __host__ __device__ __forceinline__ PrefixChunks(int tiles, int blocks, int longest, int each) {
+        const int budget = each - tiles;                             // units a kv head; those beyond one a tile
+        const int in_parts = (longest + PU_MOST_PARTS - 1) / PU_MOST_PARTS, floor = in_parts > PU_MIN_CHUNK ? in_parts : PU_MIN_CHUNK;
+        most = longest;
+        if (budget > 0 && (blocks + budget - 1) / budget < longest) most = (blocks + budget - 1) / budget;      // surely enough
+        if (most < floor) most = floor;
+        least = most;
+        if (budget > 0) {
+            least = (blocks + each - 1) / each;                      // at least this
+            if (least < floor) least = floor;
+            if (least > most) least = most;
+        }
+    }
+};
+
 // By a whole warp.
 __device__ __forceinline__ PrefixUnits prefix_units(const PrefixGroups& all, int kv_heads, int slots) {
     int tiles = 0, blocks = 0, longest = 0;
@@ -56,10 +77,9 @@ __device__ __forceinline__ PrefixUnits prefix_units(const PrefixGroups& all, int
         tiles += x.tiles; blocks += x.tiles * x.blocks; longest = max(longest, x.tiles > 0 ? x.blocks : 0);
     }
     tiles = __reduce_add_sync(0xffffffffu, tiles); blocks = __reduce_add_sync(0xffffffffu, blocks); longest = __reduce_max_sync(0xffffffffu, longest);
-    const int each = slots / kv_heads, budget = each - tiles;        // units a kv head; those beyond one a tile
-    const int most = max(PU_MIN_CHUNK, budget > 0 ? min(longest, (blocks + budget - 1) / budget) : longest);   // surely enough
+    const PrefixChunks tried(tiles, blocks, longest, slots / kv_heads);
     PrefixUnits u;
-    u.chunk = budget > 0 ? min(most, max(PU_MIN_CHUNK, (blocks + each - 1) / each)) : most;                     // at least this
+    u.chunk = tried.least;
     while (true) {
         int units = 0;
         for (int g0 = 0; g0 < all.n_groups; g0 += 32) {
@@ -67,7 +87,7 @@ __device__ __forceinline__ PrefixUnits prefix_units(const PrefixGroups& all, int
             units += x.tiles * pu_ceil(x.blocks, u.chunk);
         }
         u.units = __reduce_add_sync(0xffffffffu, units) * kv_heads;
-        if (u.chunk >= most || u.units <= slots) return u;
+        if (u.chunk >= tried.most || u.units <= slots) return u;
         ++u.chunk;
     }
 }

@@ -1,0 +1,25 @@
+"""The join of shared beginnings that are cut into as many units as there may be, in every form of the kernel that weighs them."""
+import pytest
+import torch
+
+import cache8_tools as c8
+from test_gpu_shared_prefix import K, case, run, within  # noqa: F401  (K: the fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("fp8", [True, False])
+@pytest.mark.parametrize("pages", [480, 492, 592])                    # 30,720 tokens: 240 units of two blocks of keys; 31,488 and 37,888: fewer, larger ones
+def test_the_most_units_a_tile(K, pages, fp8, monkeypatch):           # noqa: F811
+    """One kv head of 64 with eight query heads off tcgen05: eight rows are one tile, and two CTAs an SM would cut it into 296 units."""
+    q, kv, table, rows, shared = case([(pages, [1, 70, 33, 500, 64, 2, 129, 8])], [1 + 31 * i % 400 for i in range(470)], 8, 1, 64, 64, fp8)
+    assert K._prefix_plan(8, 64, 64)[0] == 2 * K.sms and K._prefix_plan(8, 64, 64)[2] == 8
+    sinks = torch.linspace(-2, 2, 8)
+    want, mass = c8.attend(q, kv, table, rows, 0.125, 0, sinks)
+    assert K._row_splits(int(fp8), rows.n_decode, 8, 1, 64, shared.longest_own, 0, True)[1] == 1       # the form for few keys
+    within(run(K, q, kv, table, rows, 0.125, sinks, shared), want, mass)
+    for form in ((1, 0, 0), (1, 1, 1), (4, 0, 0), (16, 0, 1)):
+        monkeypatch.setattr(K, "_row_splits", lambda *a: form, raising=False)
+        got = run(K, q, kv, table, rows, 0.125, sinks, shared)
+        within(got, want, mass)
+        assert torch.equal(got, run(K, q, kv, table, rows, 0.125, sinks, shared))
