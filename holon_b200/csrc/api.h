@@ -110,15 +110,16 @@ int hb_attention_decode_bf16_cluster(void* out, const void* q, const void* kv, c
 
 // One-token rows 0 .. rows - 1 over a cache of 8-bit codes (`kv8`) or of bfloat16, pages of a multiple of 16 tokens, 1 to 16 splits that
 // merge inside the kernel as a cluster (csrc/attention_rows.cu). `skip` (or null): tokens at a row's start that it shares with other
-// rows; it attends to those behind them, and the partial results of hb_attention_prefix (part_o, part_ml, part_at, and part_rows of its
-// plan) are joined with that; the call then follows that one on its stream. `few`: the form for rows of
+// rows; it attends to those behind them, and the partial results of hb_attention_prefix (part_o, part_ml, part_at, part_rows of its
+// plan, and the `part_units` units that there is room for) are joined with that; the call then follows that one on its stream. An entry of
+// part_at that names no such results counts as a wait that gave up (hb_status_word). `few`: the form for rows of
 // few keys each (64 a tile, less memory a CTA). `by_length`: the rows with most keys first. hb_attention_rows_capacity: clusters of that many CTAs that run at once (splits 1: CTAs an SM), -1
 // for sizes that are refused.
 int hb_attention_rows_capacity(int kv8, int few, int head_dim, int group, int splits);
 int hb_attention_rows(void* out, const void* q, const void* kv, int kv8, const int32_t* block_table, int table_stride,
                       const int32_t* row_slot, const int32_t* query_start, const int32_t* kv_len, int rows, int heads, int kv_heads,
                       int head_dim, int pages, int page_size, float scale, int window, int splits, int few, int by_length, const float* sinks,
-                      const int32_t* skip, const float* part_o, const float* part_ml, const int32_t* part_at, int part_rows,
+                      const int32_t* skip, const float* part_o, const float* part_ml, const int32_t* part_at, int part_rows, int part_units,
                       hb_stream stream);
 // Groups of one-token rows that hold the same first tokens in the same pages, over the keys of those (csrc/attention_prefix.cu;
 // head_dim 128 and pages of a multiple of 64 tokens: csrc/attention_prefix_tcgen05.cu): groups [n_groups][4] = (start in `members`,

@@ -81,7 +81,7 @@ struct RowsArgs {
     const int32_t* skip;           // tokens a row shares (their partial results are in part_*), or null
     const float *part_o, *part_ml; // [units, part_rows, head_dim] and [units, part_rows, 2]
     const int4* part_at;           // per row: the first unit of kv head 0, units a kv head, where the row's heads start among a unit's part_rows
-    int part_rows, table_stride, rows, heads, kv_heads, head_dim, pages, page_size, page_shift, box, window, splits, by_length;
+    int part_rows, part_units, table_stride, rows, heads, kv_heads, head_dim, pages, page_size, page_shift, box, window, splits, by_length;
     float scale_log2;
 };
 
@@ -439,7 +439,14 @@ __global__ void __launch_bounds__(AR_THREADS, D_PAD > 128 ? 1 : FEW ? 4 : 3) row
     bf16* out = a.out + ((size_t)t * a.heads + hk * group + g0) * a.head_dim;
     int4 at = make_int4(0, 0, 0, 0);
     if (a.skip) asm volatile("griddepcontrol.wait;\n" ::: "memory");   // (this launch may have begun before the one that leaves them ended)
-    if (shared > 0) at = a.part_at[b];
+    if (shared > 0) {
+        at = a.part_at[b];
+        // Where a wait of that launch gave up, rows whose turn did not come have no entry, and what is there names anything.
+        if (at.y < 1 || at.y > PU_MOST_PARTS || at.x < 0 || at.x > a.part_units - a.kv_heads * at.y || at.z < 0 || at.z > a.part_rows - group) {
+            at = make_int4(0, 0, 0, 0);
+            if (threadIdx.x == 0) tc_give_up(12);
+        }
+    }
     const size_t slot = (size_t)(at.x + hk * at.y) * a.part_rows + at.z + g0;
     const float* part_ml = shared > 0 ? a.part_ml + slot * 2 : nullptr;
     const float* part_o = shared > 0 ? a.part_o + slot * a.head_dim : nullptr;
@@ -578,7 +585,7 @@ extern "C" int hb_attention_rows_capacity(int kv8, int few, int head_dim, int gr
 extern "C" int hb_attention_rows(void* out, const void* q, const void* kv, int kv8, const int32_t* block_table, int table_stride,
                                  const int32_t* row_slot, const int32_t* query_start, const int32_t* kv_len, int rows, int heads, int kv_heads,
                                  int head_dim, int pages, int page_size, float scale, int window, int splits, int few, int by_length, const float* sinks,
-                                 const int32_t* skip, const float* part_o, const float* part_ml, const int32_t* part_at, int part_rows,
+                                 const int32_t* skip, const float* part_o, const float* part_ml, const int32_t* part_at, int part_rows, int part_units,
                                  hb_stream stream) {
     if (rows == 0) return 0;
     if (head_dim % 16 || head_dim > 256 || head_dim < 16) HB_REFUSE("attention_rows: head_dim %d is no multiple of 16 up to 256", head_dim);
@@ -591,9 +598,9 @@ extern "C" int hb_attention_rows(void* out, const void* q, const void* kv, int k
     if (rows > 65535) HB_REFUSE("attention_rows: %d rows", rows);
     if (pages < 1 || (long)pages * 2 * kv_heads > 0x7ffffffel) HB_REFUSE("attention_rows: %d pages of %d kv heads", pages, kv_heads);
     if (((uintptr_t)kv % 16) || (((uintptr_t)q | (uintptr_t)out) % 8)) HB_REFUSE("attention_rows: the cache must start on 16 bytes, q and out on 8");
-    if (skip && (!part_o || !part_ml || !part_at || window > 0)) HB_REFUSE("attention_rows: shared keys need their partial results, and no window");
+    if (skip && (!part_o || !part_ml || !part_at || part_rows < group || part_units < 1 || window > 0)) HB_REFUSE("attention_rows: shared keys need their partial results, and no window");
     RowsArgs a = {(bf16*)out, (const bf16*)q, (const unsigned char*)kv, block_table, row_slot, query_start, kv_len, sinks, skip, part_o,
-                  part_ml, (const int4*)part_at, part_rows, table_stride, rows, heads, kv_heads, head_dim, pages, page_size,
+                  part_ml, (const int4*)part_at, part_rows, part_units, table_stride, rows, heads, kv_heads, head_dim, pages, page_size,
                   log2_exact(page_size), 0, window, splits, by_length && rows <= AR_BY_LENGTH, scale * 1.4426950408889634f};
     return forms(kv8, few, &a, rows, splits, group, head_dim, nullptr, (cudaStream_t)stream);
 }

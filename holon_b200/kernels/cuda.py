@@ -236,7 +236,7 @@ class CudaKernels:
     ARGUMENTS = {"hb_qk_norm_rope_kv_write8": "pppp" "ii" "pp" "i" "ff" "pp" "iiiiii" "p",
                  "hb_kv_read": "pi" "pp" "iiiii",
                  "hb_attention_prefix": "ppp" "ppi" "pi" "pp" "iiiiii" "f" "i",
-                 "hb_attention_rows": "ppp" "i" "pi" "ppp" "iiiiii" "f" "iiii" "p" "pppp" "i"}
+                 "hb_attention_rows": "ppp" "i" "pi" "ppp" "iiiiii" "f" "iiii" "p" "pppp" "ii"}
 
     def _call_in(self, lib, cache: dict, name: str, *args) -> None:
         """`_call` for a function of another library (an extension's)."""
@@ -713,7 +713,7 @@ class CudaKernels:
             splits, few, by_length = self._row_splits(kv8, n, *sizes[:3], rows.max_kv, window, False)
             return self._call("hb_attention_rows", out.data_ptr(), q_at, kv_at, kv8, table, stride, row_slot.data_ptr(), query_start.data_ptr(),
                               kv_len.data_ptr(), n, *sizes, scale, window, splits, few, by_length,
-                              sinks.data_ptr() if sinks is not None else None, None, None, None, None, 0)
+                              sinks.data_ptr() if sinks is not None else None, None, None, None, None, 0, 0)
         skip, members, groups = shared.skip, shared.members, shared.groups
         self._check(skip, members, groups)
         at_most = groups.shape[0] // 4 if groups.dim() == 1 else 0
@@ -730,7 +730,7 @@ class CudaKernels:
         splits, few, by_length = self._row_splits(kv8, n, *sizes[:3], shared.longest_own, 0, True)
         self._call("hb_attention_rows", out.data_ptr(), q_at, kv_at, kv8, table, stride, row_slot.data_ptr(), query_start.data_ptr(),
                    kv_len.data_ptr(), n, *sizes, scale, 0, splits, few, by_length, sinks.data_ptr() if sinks is not None else None,
-                   skip.data_ptr(), part_o, part_ml, part_at, part_rows)
+                   skip.data_ptr(), part_o, part_ml, part_at, part_rows, rows_left // part_rows)
 
     def _prefix_room(self, rows: int, heads: int, kv_heads: int, head_dim: int, pages: int, page_size: int) -> tuple[int, int, int]:
         """(CTAs, query rows a piece of work leaves results for, such rows in all) of the kernel for shared keys."""

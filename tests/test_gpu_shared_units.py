@@ -23,3 +23,25 @@ def test_the_most_units_a_tile(K, pages, fp8, monkeypatch):           # noqa: F8
         got = run(K, q, kv, table, rows, 0.125, sinks, shared)
         within(got, want, mass)
         assert torch.equal(got, run(K, q, kv, table, rows, 0.125, sinks, shared))
+
+
+@pytest.mark.parametrize("fp8", [True, False])
+@pytest.mark.parametrize("left", [float("nan"), 0.0, -1.0, 1e-40])    # as numbers of four bytes: large ones, zeros, negative ones, 71,362
+def test_partial_results_that_were_not_left(K, fp8, left, monkeypatch):   # noqa: F811
+    """A launch for the shared keys that gave up leaves rows without an entry: the join reports that and reads nothing by what it finds there."""
+    q, kv, table, rows, shared = case([(16, [1, 130, 64, 3])], [60, 7], 8, 2, 128, 64, fp8)
+    clean = run(K, q, kv, table, rows, 0.125, None, shared)
+    call, empty = type(K)._call, torch.empty
+    monkeypatch.setattr(K, "_call", lambda name, *a: None if name == "hb_attention_prefix" else call(K, name, *a), raising=False)
+    monkeypatch.setattr(torch, "empty", lambda *a, **kw: empty(*a, **kw).fill_(left))
+    assert K.status() == 0
+    try:
+        got = run(K, q, kv, table, rows, 0.125, None, shared)
+        torch.cuda.synchronize()
+        assert K.status() >> 28 == 12
+    finally:
+        K.clear_status()
+    alone = [b for b in range(6) if int(shared.skip[b]) == 0]
+    assert len(alone) == 2 and all(torch.equal(got[b], clean[b]) for b in alone)
+    monkeypatch.undo()
+    assert torch.equal(run(K, q, kv, table, rows, 0.125, None, shared), clean) and K.status() == 0
