@@ -131,8 +131,10 @@ int hb_attention_rows(void* out, const void* q, const void* kv, int kv8, const i
 int hb_attention_prefix_plan(int head_dim, int page_size, int group, int* part_rows, int* tile_rows);
 int hb_attention_prefix(float* part_o, float* part_ml, int32_t* part_at, const void* q, const void* kv, int kv8,
                         const int32_t* block_table, int table_stride, const int32_t* members, const int32_t* groups, int n_groups,
-                         int heads, int kv_heads, int head_dim, int pages, int page_size, float scale, int ctas,
+                        int heads, int kv_heads, int head_dim, int pages, int page_size, float scale, int ctas,
                         hb_stream stream);
+int hb_attention_rows_status(unsigned int* status);   // as hb_attention_tcgen05_status
+int hb_attention_prefix_status(unsigned int* status);
 
 // The same rows with the keys of all of them shared out evenly over `ctas` CTAs (one wave that fills the GPU): each
 // takes the same number of 64-key tiles, across rows and heads where its stretch crosses them, so rows of any lengths

@@ -364,6 +364,13 @@ __global__ void __launch_bounds__(Shape<KV8>::THREADS, 1) prefix_tcgen05_kernel(
 }
 
 HB_DEFINE_STATUS_MIRROR(hb_attention_prefix_status_mirror)
+extern "C" int hb_attention_prefix_status(unsigned int* status) {
+    HB_CUDA(cudaDeviceSynchronize());
+    HB_CUDA(cudaMemcpyFromSymbol(status, g_tc_status, sizeof(unsigned int)));
+    const unsigned int zero = 0;
+    HB_CUDA(cudaMemcpyToSymbol(g_tc_status, &zero, sizeof(unsigned int)));
+    return 0;
+}
 
 template <bool KV8> static int launch(const PrefixTcArgs& a, int ctas, cudaStream_t s) {
     using H = Shape<KV8>;

@@ -565,6 +565,13 @@ template <bool KV8, bool FEW> static int any_rows(RowsArgs* a, int rows, int spl
 }
 
 HB_DEFINE_STATUS_MIRROR(hb_attention_rows_status_mirror)
+extern "C" int hb_attention_rows_status(unsigned int* status) {
+    HB_CUDA(cudaDeviceSynchronize());
+    HB_CUDA(cudaMemcpyFromSymbol(status, g_tc_status, sizeof(unsigned int)));
+    const unsigned int zero = 0;
+    HB_CUDA(cudaMemcpyToSymbol(g_tc_status, &zero, sizeof(unsigned int)));
+    return 0;
+}
 
 static int forms(int kv8, int few, RowsArgs* a, int rows, int splits, int group, int head_dim, int* capacity, cudaStream_t s) {
     if (kv8) return few ? any_rows<true, true>(a, rows, splits, group, head_dim, capacity, s) : any_rows<true, false>(a, rows, splits, group, head_dim, capacity, s);
