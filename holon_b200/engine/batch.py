@@ -138,6 +138,7 @@ class StepContext:
         self.link = None             # parts.base.Link: a block's offer to the product that ends its mixer or feed-forward
         self.from_last = None        # int32 [rows]: 1 where the row's token is fed from the device
         self.offset_of: dict = {}    # host: entry index -> offset of its first token among the step's tokens
+        self.layout: tuple = ()      # host: what decides where the step's arrays lie beside its counts (the cache groups whose rows share)
 
     def entry_slots(self, entry: int) -> dict:
         """The fixed-size per-request tensors kept under cache entry `entry`, by name."""
