@@ -350,7 +350,7 @@ class Engine:
         step = runner.context(entries, pad_rows=pad, extra=padded)
         kernels = self.built.ctx.kernels
         # what the mixers' kernels pin for a captured step is part of the key: a graph per plan
-        key = (bucket, len(portions), step.rows.n_tokens - bucket, runner.plan(step, self.config.max_model_len))
+        key = (bucket, len(portions), step.rows.n_tokens - bucket, *runner.plan(step, self.config.max_model_len))
         if key not in self._graphs:
             # The first step of a shape runs eagerly (which also warms up what the capture must not do for the first
             # time) and is then recorded for the steps to come. Its results are the eager run's: replaying the new

@@ -179,7 +179,7 @@ class Runner:
         """What a step that is to run as a CUDA graph has in common with those that its graph may be replayed for, beside its counts: the
         mixers' plans (`Model.capture_plan`, for requests of up to `longest` tokens), and which groups' shared beginnings were uploaded.
         Those lie before the arrays of `extra`, whose places a graph holds, whether or not a mixer reads them."""
-        return step.layout, self.model.capture_plan(step, longest)
+        return self.model.capture_plan(step, longest), step.layout
 
     # ------------------------------------------------------------------ the step
     def step(self, entries: Sequence[StepEntry]) -> torch.Tensor | None:
@@ -231,7 +231,7 @@ class Runner:
         kernels do for their first launch must not be captured. Both run with the plan that serves every step of the kind, so a
         step's logits do not depend on how it was run."""
         step = self.context(entries, pad_rows=0)
-        kind = (len(entries), self.plan(step, self.ctx.max_positions),
+        kind = (len(entries), *self.plan(step, self.ctx.max_positions),
                 torch.backends.cuda.matmul.allow_bf16_reduced_precision_reduction)
         key = (self._generation, *kind)
         found = self._recorded.get(key)
