@@ -19,19 +19,20 @@ class EngineConfig:
     model: str = dataclasses.field(metadata={"help": "model folder: config.json and *.safetensors"})
     device: str = _setting("cuda:0", "CUDA device to run on")
     dtype: str = _setting("bfloat16", "bfloat16: the serving kernels; float32: every product and sum in true 32-bit")
-    cache_dtype: str = _setting("auto", "keys and values of grouped-query attention: auto (the dtype) or fp8 (8-bit floats, a scale per token and head)")
     page_size: int = _setting(64, "tokens per page of the key/value cache")
     max_seqs: int = _setting(64, "sequences served at once")
     max_model_len: int = _setting(8192, "prompt + generated tokens per request; the cache always holds one")
     max_step_tokens: int = _setting(4096, "tokens one step computes at most")
     chunk_with_decode: int = _setting(0, "prefill tokens a step with decode rows may also carry (0: none)")
     prefix_cache: bool = _setting(True, "share whole cache pages of equal prompt prefixes between requests")
-    shared_prefix: bool = _setting(False, "decode rows that share pages read the keys there once for all of them")
     memory_fraction: float = _setting(0.9, "of the memory left after the weights, for the cache and activations")
     state_memory: int | None = _setting(None, "bytes for the cache pools; default: from memory_fraction")
     overlap: bool = _setting(True, "schedule step N while step N-1 runs (depth 1); off: depth 0")
     cuda_graphs: bool = _setting(True, "replay decode steps from CUDA graphs, per batch-size bucket")
     seed: int | None = _setting(None, "base seed for requests that bring none; default: drawn at start")
+    # (fields that come later stand behind: settings may be given by position)
+    cache_dtype: str = _setting("auto", "keys and values of grouped-query attention: auto (the dtype) or fp8 (8-bit floats, a scale per token and head)")
+    shared_prefix: bool = _setting(False, "decode rows that share pages read the keys there once for all of them")
 
     def __post_init__(self) -> None:
         for name in ("page_size", "max_seqs", "max_model_len", "max_step_tokens"):
