@@ -97,15 +97,19 @@ class GQA(Part):
 
     def context_scratch(self, tokens: int, rows: int, longest: int) -> int:
         scratch = getattr(self.ctx.kernels, "read_back_scratch", None) if self.fp8 else None
-        return scratch(tokens, rows, longest, self.kv_heads, self.head_dim) if scratch is not None else 0
+        back = scratch(tokens, rows, longest, self.kv_heads, self.head_dim) if scratch is not None else 0
+        return back + self._shared_scratch(rows, self.ctx.page_size)
 
     def graph_scratch(self, rows: int, portions: int, longest: int, page_size: int) -> int:
-        k, bytes_ = self.ctx.kernels, 0
+        bytes_ = self._shared_scratch(rows, page_size)
         if self.fp8:                                                 # (a captured step reads all its portions back at once)
             bytes_ += portions * -(-longest // 64) * 64 * 4 * self.kv_heads * self.head_dim
-        if self.ctx.shared_prefix and hasattr(k, "shared_scratch"):
-            bytes_ += 4 * k.shared_scratch(rows, self.heads, self.kv_heads, self.head_dim, page_size)
         return bytes_
+
+    def _shared_scratch(self, rows: int, page_size: int) -> int:
+        """Bytes for what `rows` one-token rows share: steps that are measured share nothing."""
+        scratch = getattr(self.ctx.kernels, "shared_scratch", None) if self.ctx.shared_prefix and self.window <= 0 else None
+        return 4 * scratch(rows, self.heads, self.kv_heads, self.head_dim, page_size) if scratch is not None else 0
 
     @property
     def plan_group(self):
