@@ -17,6 +17,8 @@ def test_memory_without_graphs(cache_dtype):
         k, m = e.built.ctx.kernels, e.built.memory
         e.close()
         return k.shared_scratch(64, 8, 2, 128, 64), m
+    account()                                                         # (what the matrix library keeps from its first call on is not counted twice)
     (scratch, apart), (_, together) = account(), account(shared_prefix=True)
-    assert apart.graphs == together.graphs == 0
-    assert together.activations >= 4 * scratch > 0 and together.activations >= apart.activations
+    assert apart.graphs == together.graphs == 0 and scratch > 0
+    # the measured steps are alike, up to the 2 MB in which the allocator takes memory from the device
+    assert together.activations >= apart.activations + 4 * scratch - (2 << 20)
