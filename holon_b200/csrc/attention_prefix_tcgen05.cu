@@ -142,6 +142,7 @@ __global__ void __launch_bounds__(Shape<KV8>::THREADS, 1) prefix_tcgen05_kernel(
 
         if (warp == 0) {
             const int32_t* table = a.block_table + (size_t)u.slot * a.table_stride;
+            int asked = 0;                                            // tiles whose copies are on their way or there
             for (int t0 = 0; t0 < tiles && ok; t0 += 32) {
                 const int key = (first + t0 + lane) * PT_BN, pi = key / a.page_size, in = key - pi * a.page_size;     // this lane's tile
                 int page = t0 + lane < tiles ? table[pi] : 0;
@@ -154,6 +155,7 @@ __global__ void __launch_bounds__(Shape<KV8>::THREADS, 1) prefix_tcgen05_kernel(
                     const int n = seen + t0 + i, s = n % (KV8 ? H::RAW : H::STAGES), round = n / (KV8 ? H::RAW : H::STAGES);
                     ok = __all_sync(0xffffffffu, mbar_wait((KV8 ? raw_empty0 : kv_empty0) + 8 * s, (round & 1) ^ 1, 1));
                     if (!ok) break;
+                    asked = t0 + i + 1;
                     if (lane != i) continue;
                     if (KV8) {
                         const uint32_t full = raw_full0 + 8 * s, dst = base + H::RAWS + s * PT_RAW_STAGE;
@@ -172,6 +174,11 @@ __global__ void __launch_bounds__(Shape<KV8>::THREADS, 1) prefix_tcgen05_kernel(
                     }
                 }
             }
+            // No copy may come after the CTA's end, whoever gave up before (else others wait for them, too).
+            constexpr int RING = KV8 ? H::RAW : H::STAGES;
+#pragma unroll 1
+            for (int n = seen + max(0, asked - RING); n < seen + asked; ++n) ok &= mbar_wait((KV8 ? raw_full0 : kv_full0) + 8 * (n % RING), (n / RING) & 1, 13);
+            ok = __all_sync(0xffffffffu, ok);
         } else if (KV8 && warp >= 12) {
             const int part = warp - 12, sub = lane & 7;
             for (int j = 0; j < tiles && ok; ++j) {

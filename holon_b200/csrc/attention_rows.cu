@@ -115,7 +115,9 @@ __device__ __forceinline__ void load_tiles(const CUtensorMap* map, const RowsArg
     const uint32_t full = base + T::BARS, empty = full + 8 * T::STAGES;
     const uint32_t bytes = T::STAGE + (KV8 ? 2 * T::KEYS : 0);
     const size_t block = (size_t)a.page_size * (a.head_dim + 1);
-    for (int t0 = first; t0 < last; t0 += batch) {
+    int asked = 0;                                                   // tiles whose copies are on their way or there
+    bool ok = true;
+    for (int t0 = first; t0 < last && ok; t0 += batch) {
         const int key = t0 * T::KEYS + lane * a.box, pi = a.page_shift >= 0 ? key >> a.page_shift : key / a.page_size, in = key - pi * a.page_size;   // this lane's box
         const int page = lane < batch * boxes && key < n ? table[pi] : -1;
         const bool there = page >= 0 && page < a.pages;
@@ -124,7 +126,9 @@ __device__ __forceinline__ void load_tiles(const CUtensorMap* map, const RowsArg
         const unsigned char* v_scale = k_scale + (size_t)a.kv_heads * block;
         for (int i = 0; i < batch && t0 + i < last; ++i) {
             const int j = t0 + i - first, s = j % T::STAGES;
-            if (!__all_sync(0xffffffffu, mbar_wait(empty + 8 * s, ((j / T::STAGES) & 1) ^ 1, 1))) return;
+            ok = __all_sync(0xffffffffu, mbar_wait(empty + 8 * s, ((j / T::STAGES) & 1) ^ 1, 1));
+            if (!ok) break;
+            asked = j + 1;
             if (lane == 0) mbar_expect_tx(full + 8 * s, bytes);
             __syncwarp();
             if (lane / boxes != i) continue;
@@ -141,6 +145,9 @@ __device__ __forceinline__ void load_tiles(const CUtensorMap* map, const RowsArg
             }
         }
     }
+    // No copy may come after the CTA's end, whoever gave up before (else the computing warps wait for them, too).
+#pragma unroll 1
+    for (int j = max(0, asked - T::STAGES); j < asked; ++j) mbar_wait(full + 8 * (j % T::STAGES), (j / T::STAGES) & 1, 3);
 }
 
 // The B fragments of up to eight heads' queries at `q` (head_dim apart), head lane / 4; for codes as halves, each head divided by a
