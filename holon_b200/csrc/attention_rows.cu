@@ -85,8 +85,9 @@ struct RowsArgs {
     float scale_log2;
 };
 
-// A stage's tile of KEYS keys (FEW: 64, two stages: for rows of a few hundred keys, whose time is a CTA's start and end; four such
-// CTAs fit an SM): keys, then values, each as column blocks [KEYS rows][SUB bytes] that TMA swizzles over SUB bytes.
+// A stage's tile of KEYS keys (FEW: 64, two stages: for rows of a few hundred keys, whose time is a CTA's start and end; an SM holds four
+// such CTAs where it holds two of the others, bfloat16 heads of 128 three, 8-bit heads of 64 four in place of three, above 128 8-bit ones
+// two in place of one and bfloat16 ones no more): keys, then values, each as column blocks [KEYS rows][SUB bytes] that TMA swizzles over SUB bytes.
 template <int D_PAD, bool KV8, bool FEW> struct Tile {
     static constexpr int ROW = KV8 ? D_PAD : 2 * D_PAD;              // bytes of a key
     static constexpr int NK = FEW ? 1 : AR_NK(D_PAD, KV8), KEYS = 16 * AR_WARPS * NK;   // a warp takes NK times 16 keys of a tile
@@ -97,6 +98,8 @@ template <int D_PAD, bool KV8, bool FEW> struct Tile {
     static constexpr int BODY = STAGES * STAGE > SUMS ? STAGES * STAGE : SUMS;
     static constexpr int BARS = BODY + STAGES * 2 * KEYS;            // behind the tiles: a stage's scale bytes, then the barriers
     static constexpr int RECV = BARS + 16 * STAGES;                  // then what the other CTAs of a cluster send
+    // CTAs an SM that its 228 KB hold (1 KB of each is the system's, 1 KB goes to the boundary): registers are not cut for more of them.
+    static constexpr int FIT = (228 * 1024) / (RECV + 2048), CTAS = D_PAD > 128 ? 1 : FIT < (FEW ? 4 : 3) ? FIT : FEW ? 4 : 3;
 };
 // Byte offset of (row, 16-byte chunk) in a part of a tile: eight rows at one chunk lie in eight bank groups.
 template <int D_PAD, bool KV8, bool FEW> __device__ __forceinline__ uint32_t tile_at(int row, int chunk) {
@@ -401,7 +404,7 @@ __device__ __forceinline__ int row_by_length(unsigned char* smem, const RowsArgs
 
 // grid (kv_heads * ceil(group / 8), rows, splits), a cluster along z.
 template <int D_PAD, bool KV8, bool FEW>
-__global__ void __launch_bounds__(AR_THREADS, D_PAD > 128 ? 1 : FEW ? 4 : 3) rows_kernel(const __grid_constant__ CUtensorMap map, const RowsArgs a) {
+__global__ void __launch_bounds__(AR_THREADS, (Tile<D_PAD, KV8, FEW>::CTAS)) rows_kernel(const __grid_constant__ CUtensorMap map, const RowsArgs a) {
     extern __shared__ unsigned char smem_raw[];
     using T = Tile<D_PAD, KV8, FEW>;
     static_assert(T::SUMS + 4 * AR_HEADS * ((FEW ? AR_WARPS : AR_CLUSTER) + PU_MOST_PARTS) <= T::BODY, "the join's weights lie between the sums and `whole`");

@@ -759,9 +759,9 @@ class CudaKernels:
         + 4 for its start), and what a cluster costs: 1 tile's time, 4 where every CTA of it also joins shared keys' results. A
         tile is 128 keys, 64 of bfloat16 heads above 64. Measured: one row of 400 keys of 16 / 8 heads 7.2 us in one CTA, 6.3 in four; 8
         rows of 8,192 keys 53.5 / 31.0 / 29.7 / 27.4 / 40.9 us in 1 to 5 (the fifth is a second wave); 4 rows with 65 own keys behind
-        1,024 shared ones 12.5 / 13.7 us in 1 and 2. Second: whether they run in the form for few keys, four of whose CTAs an SM
-        holds in place of two: 64 rows with up to 256 own keys 43.2 us with it off, 38.0 on; 64 rows of up to 4,096 keys
-        55 and 69. Third: whether there are more CTAs than run at once, so that the longest rows should start first (64 rows of up
+        1,024 shared ones 12.5 / 13.7 us in 1 and 2. Second: whether they run in the form for few keys, where an SM holds
+        more of its CTAs (four in place of two for 8-bit heads of 128): 64 rows with up to 256 own keys behind 8,192 shared ones 41.2 us with it
+        off, 35.6 on, bfloat16 42.6 and 40.0 (three in place of two), heads of 64 48.9 and 43.5; 64 rows of up to 4,096 keys 55 and 69. Third: whether there are more CTAs than run at once, so that the longest rows should start first (64 rows of up
         to 4,096 keys 54.8 us, in any order 67.0)."""
         if 0 < window < longest:
             longest = window + 127                                   # (a window may begin within a tile)
@@ -774,7 +774,7 @@ class CudaKernels:
             for s in range(1, min(16, tiles) + 1):
                 if room(s) > 0:
                     best = min(best, (-(-pairs // room(s)) * (-(-tiles // s) + 4) + (s > 1) * (4 if shared else 1), s))
-            few = int(longest <= self.FEW_KEYS and best[1] == 1 and pairs > room(1))
+            few = int(longest <= self.FEW_KEYS and best[1] == 1 and pairs > room(1) and room(1, 1) > room(1))
             found = self._splits[key] = best[1], few, int(pairs > room(best[1], few))
         return found
 
