@@ -201,7 +201,7 @@ extern "C" int hb_attention_prefix_plan(int head_dim, int page_size, int group, 
     }
     *part_rows = PX_ROWS;
     *tile_rows = PX_ROWS / group;
-    return group <= PX_ROWS ? 2 : 0;
+    return group > PX_ROWS ? 0 : head_dim > 128 ? 1 : 2;            // (above 128 a CTA's tiles take 160 KB)
 }
 
 extern "C" int hb_attention_prefix(float* part_o, float* part_ml, int32_t* part_at, const void* q, const void* kv, int kv8,

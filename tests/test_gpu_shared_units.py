@@ -46,3 +46,9 @@ def test_partial_results_that_were_not_left(K, fp8, left, monkeypatch):   # noqa
     assert len(alone) == 2 and all(torch.equal(got[b], clean[b]) for b in alone)
     monkeypatch.undo()
     assert torch.equal(run(K, q, kv, table, rows, 0.125, None, shared), clean) and K.status() == 0
+
+
+def test_as_many_ctas_as_an_sm_holds(K):                              # noqa: F811
+    """Off tcgen05 two CTAs of the kernel for shared keys fit an SM, above heads of 128 one (160 KB of tiles)."""
+    assert [K._prefix_plan(4, dim, 64)[0] // K.sms for dim in (64, 80, 144, 192, 256)] == [2, 2, 1, 1, 1]
+    assert K._prefix_plan(4, 128, 16)[0] == 2 * K.sms and K._prefix_plan(4, 128, 64)[0] == K.sms
