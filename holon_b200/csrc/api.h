@@ -113,7 +113,7 @@ int hb_attention_decode_bf16_cluster(void* out, const void* q, const void* kv, c
 // rows; it attends to those behind them, and the partial results of hb_attention_prefix (part_o, part_ml, part_at, part_rows of its
 // plan, and the `part_units` units that there is room for) are joined with that; the call then follows that one on its stream. An entry of
 // part_at that names no such results counts as a wait that gave up (hb_status_word). `few`: the form for rows of
-// few keys each (64 a tile, less memory a CTA). `by_length`: the rows with most keys first. hb_attention_rows_capacity: clusters of that many CTAs that run at once (splits 1: CTAs an SM), -1
+// few keys each (64 a tile, less memory a CTA). `by_length`: the rows with most keys first (up to 1,024 rows). hb_attention_rows_capacity: clusters of that many CTAs that run at once (splits 1: CTAs an SM), -1
 // for sizes that are refused.
 int hb_attention_rows_capacity(int kv8, int few, int head_dim, int group, int splits);
 int hb_attention_rows(void* out, const void* q, const void* kv, int kv8, const int32_t* block_table, int table_stride,

@@ -37,7 +37,7 @@
 #define AR_HEADS 8
 #define AR_CLUSTER 16                 // splits at most
 #define AR_BIAS 14.f
-#define AR_BY_LENGTH 1024             // rows up to which a launch may take the longest first
+#define AR_BY_LENGTH 1024             // rows whose lengths a CTA has room to rank (what pays is the caller's to say)
 #define AR_NK(D_PAD, KV8) ((KV8) || (D_PAD) <= 64 ? 2 : 1)
 #define AR_STAGES(BYTES) ((BYTES) <= 16384 ? 4 : (BYTES) <= 32768 ? 3 : 2)
 

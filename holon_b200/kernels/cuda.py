@@ -754,6 +754,12 @@ class CudaKernels:
 
     FEW_KEYS = 512                            # keys a row up to which the form for few keys pays, where CTAs are more than run at once
 
+    # Rows up to which the longest start first. Every CTA ranks the rows by itself, rows^2 / 160 steps, before its first load. 8-bit pages, 32
+    # heads over 8 kv heads of 128, any order and longest first: 40 rows of up to 1,000 keys 19.2 and 16.1 us, 64 rows of up to 4,096 66.5 and
+    # 55.1, 72 rows 73.1 and 61.8, but 80 rows 83.3 and 92.1, 128 rows 124.7 and 138.5, 256 rows of up to 1,000 73.7 and 116.9, 1,024 rows of up to
+    # 300 114 and 1,893. One long row among 64 short ones 37.3 and 30.8, among 80 41.1 and 46.5; rows alike lose 2% up to 72.
+    BY_LENGTH_ROWS = 72
+
     def _row_splits(self, kv8: int, rows: int, heads: int, kv_heads: int, head_dim: int, longest: int, window: int, shared: bool) -> tuple[int, int, int]:
         """Into how many CTAs (a cluster) the keys of a one-token row are cut: the number with the least waves x (tiles a CTA walks
         + 4 for its start), and what a cluster costs: 1 tile's time, 4 where every CTA of it also joins shared keys' results. A
@@ -761,8 +767,8 @@ class CudaKernels:
         rows of 8,192 keys 53.5 / 31.0 / 29.7 / 27.4 / 40.9 us in 1 to 5 (the fifth is a second wave); 4 rows with 65 own keys behind
         1,024 shared ones 12.5 / 13.7 us in 1 and 2. Second: whether they run in the form for few keys, where an SM holds
         more of its CTAs (four in place of two for 8-bit heads of 128): 64 rows with up to 256 own keys behind 8,192 shared ones 41.2 us with it
-        off, 35.6 on, bfloat16 42.6 and 40.0 (three in place of two), heads of 64 48.9 and 43.5; 64 rows of up to 4,096 keys 55 and 69. Third: whether there are more CTAs than run at once, so that the longest rows should start first (64 rows of up
-        to 4,096 keys 54.8 us, in any order 67.0)."""
+        off, 35.6 on, bfloat16 42.6 and 40.0 (three in place of two), heads of 64 48.9 and 43.5; 64 rows of up to 4,096 keys
+        55 and 69. Third: whether the longest rows start first, where there are more CTAs than run at once and up to BY_LENGTH_ROWS rows."""
         if 0 < window < longest:
             longest = window + 127                                   # (a window may begin within a tile)
         key = ("rows", kv8, rows, heads, kv_heads, head_dim, -(-longest // 64), shared)
@@ -775,7 +781,7 @@ class CudaKernels:
                 if room(s) > 0:
                     best = min(best, (-(-pairs // room(s)) * (-(-tiles // s) + 4) + (s > 1) * (4 if shared else 1), s))
             few = int(longest <= self.FEW_KEYS and best[1] == 1 and pairs > room(1) and room(1, 1) > room(1))
-            found = self._splits[key] = best[1], few, int(pairs > room(best[1], few))
+            found = self._splits[key] = best[1], few, int(rows <= self.BY_LENGTH_ROWS and pairs > room(best[1], few))
         return found
 
     KV_BUCKET_MIN = 512                       # the smallest number of keys a captured decode launch is planned for
