@@ -98,8 +98,9 @@ template <int D_PAD, bool KV8, bool FEW> struct Tile {
     static constexpr int BODY = STAGES * STAGE > SUMS ? STAGES * STAGE : SUMS;
     static constexpr int BARS = BODY + STAGES * 2 * KEYS;            // behind the tiles: a stage's scale bytes, then the barriers
     static constexpr int RECV = BARS + 16 * STAGES;                  // then what the other CTAs of a cluster send
-    // CTAs an SM that its 228 KB hold (1 KB of each is the system's, 1 KB goes to the boundary): registers are not cut for more of them.
-    static constexpr int FIT = (228 * 1024) / (RECV + 2048), CTAS = D_PAD > 128 ? 1 : FIT < (FEW ? 4 : 3) ? FIT : FEW ? 4 : 3;
+    // CTAs an SM that registers are cut for: of the form for few keys what its 228 KB hold (1 KB of each is the system's, 1 KB goes to the
+    // boundary), up to four; of the other three, of which two or three fit (8 rows of 8,192 keys 28.0 us in 128 registers, 28.5 in the 143 that two would leave).
+    static constexpr int FIT = (228 * 1024) / (RECV + 2048), CTAS = D_PAD > 128 ? 1 : !FEW ? 3 : FIT < 4 ? FIT : 4;
 };
 // Byte offset of (row, 16-byte chunk) in a part of a tile: eight rows at one chunk lie in eight bank groups.
 template <int D_PAD, bool KV8, bool FEW> __device__ __forceinline__ uint32_t tile_at(int row, int chunk) {
