@@ -7,9 +7,8 @@
 // over the S they came from; O += P V (128 x 128 x 16, four products, P from tensor memory). The running maximum may lag by 2^8
 // before O is rescaled. No key is masked: shared pages are whole, and whole numbers of 64 keys.
 // bfloat16 pages: keys and values come by TMA as the products want them. 8-bit pages: TMA brings the codes, and four warps turn them
-// into bfloat16, scale and all (exactly), in the same layout: six instructions for two codes, where halves without the scale would be one
-// and leave the scales to the softmax (a factor and a term a score, a factor a weight: as many instructions once there are
-// 128 query rows, and registers that it does not have).
+// into bfloat16, scale and all (exactly), in the same layout. (Halves without the scale would convert in fewer steps and leave the scales to
+// the softmax: a factor and a term a score, a factor a weight, in threads that have no registers left. Not built.)
 // Barriers keep their phases from unit to unit; every role counts the tiles that it has seen.
 //
 // Measured, with 32 heads over 8 kv heads and with the rows' own keys behind it: 64 rows on 8,192 tokens of 8-bit pages 35.3 us (in the mma.sync

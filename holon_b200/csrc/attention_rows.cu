@@ -10,12 +10,15 @@
 // Both products have the heads as their eight columns: S^T = K Q^T (16 keys a product) and O^T = V^T P^T (16 numbers of the head), so
 // that eight heads fill the shape and a lane's maxima and sums belong to the columns of its outputs; the weights pass from one
 // product's result to the other's operand by a transposition of 8 x 8 blocks.
-// 8-bit pages: codes become halves, which hold every code exactly (mma.sync on codes themselves is the same conversion and more
-// instructions on this GPU: 8 to 12 where the two conversions and the product are 5, counted). With k_j = 2^a_j K_j and
+// 8-bit pages: codes become halves, which hold every code exactly. (mma.sync m16n8k32 on codes themselves: 9 executed instructions by
+// counter, an m16n8k16 on halves 2.5, the conversion of four codes 2.5.) With k_j = 2^a_j K_j and
 // v_j = 2^b_j V_j (K, V codes) and the head's query scaled into the halves' range by a power of two 2^-c,
 //     u_j = (q 2^-c . K_j) 2^(a_j + c) scale log2(e) + b_j,   w_j = 2^(u_j - M),   O = sum w_j V_j,   l = sum w_j 2^-b_j
 // with M the running maximum of u, not of the scores: the weights that meet the codes stay at most 2^14 whatever the values' scales
-// are (14 is taken off M so that small weights are no subnormal halves), and l sums the softmax's own weights in the same units.
+// are (14 is taken off M so that small weights are no subnormal halves), and l sums the softmax's own weights in the same units. Keys whose
+// weights vanish in 32 bits (below 2^-126) would be missing in l: they are less than 2^-25 of it in all, for up to 2^20 keys, while the b of a
+// head lie within 2^80 of one another (a value of zeros has b = -64: values up to 2^24 beside such). Where keys with values of (nearly) zeros
+// take all but 2^-28 of the weight, the others' weights are subnormal halves with fewer bits.
 // ldmatrix moves pairs of codes as it moves bfloat16: of a key a lane gets codes 4 c .. 4 c + 3 where the fragment wants columns 2 c,
 // 2 c + 1, 2 c + 8, 2 c + 9, so queries are laid out in that order; of values it gets two neighbouring codes of two keys, one byte
 // permutation pairs the keys, and the even numbers of the head are the product's rows 0 - 7, the odd ones its rows 8 - 15.
