@@ -23,7 +23,7 @@ __global__ void __launch_bounds__(128) qk_norm_rope_kv_write8_kernel(
         const bf16* __restrict__ bias) {
     extern __shared__ float smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int items = heads + (kv ? 2 * kv_heads : 0);
+    const int items = heads + 2 * kv_heads;
     const long unit = (long)blockIdx.x * (blockDim.x >> 5) + warp;
     if (unit >= units) return;                       // (a whole warp; nothing below waits for another one)
     const long t = unit / items;
@@ -139,7 +139,7 @@ __global__ void __launch_bounds__(256, 3) qk_norm_rope_kv_write8_lanes_kernel(
         const TW* __restrict__ k_weight, float eps, float offset, unsigned char* __restrict__ kv,
         const int32_t* __restrict__ write_index, int pages, int page_size, int page_shift, unsigned units, int heads, int kv_heads, int head_dim,
         const bf16* __restrict__ bias) {
-    const unsigned items = heads + (kv ? 2 * kv_heads : 0), step = gridDim.x * (256 / LANES);
+    const unsigned items = heads + 2 * kv_heads, step = gridDim.x * (256 / LANES);
     const unsigned step_t = step / items, step_item = step - step_t * items;
     const int sub = threadIdx.x & (LANES - 1);
     const bool pairs = sub < rotary_dim >> 4, inside = sub < head_dim >> 4;      // (a value head's chunks are cut alike)
@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(256, 3) qk_norm_rope_kv_write8_lanes_kernel(
         const bf16* src = first + (size_t)t * width + item * head_dim;
         if (inside) { na = *(const uint4*)src; nb = *(const uint4*)(src + apart); }
         if (rotary_dim) n_pos = positions[t];
-        if (kv) n_write = write_index[t];
+        n_write = write_index[t];
     };
     // (every lane of a warp makes as many turns: the shuffles are the whole warp's)
     ask(mine);
@@ -281,16 +281,16 @@ extern "C" int hb_qk_norm_rope_kv_write8(void* q_out, const void* qkv, const int
                                          const void* bias, hb_stream stream) {
     if (tokens == 0) return 0;
     if (head_dim < 16 || head_dim % 16 || head_dim > 1024) HB_REFUSE("qk_norm_rope_kv_write8: head_dim %d is no multiple of 16 up to 1024", head_dim);
-    if (kv && (page_size < 16 || page_size % 16)) HB_REFUSE("qk_norm_rope_kv_write8: page size %d is no multiple of 16", page_size);
+    if (!kv || !write_index) HB_REFUSE("qk_norm_rope_kv_write8: needs a cache and write_index");
+    if (page_size < 16 || page_size % 16) HB_REFUSE("qk_norm_rope_kv_write8: page size %d is no multiple of 16", page_size);
     if (rotary_dim < 0 || rotary_dim > head_dim || (rotary_dim & 1))
         HB_REFUSE("qk_norm_rope_kv_write8: rotary_dim %d must be even and at most head_dim %d", rotary_dim, head_dim);
     if (rotary_dim && (!table || max_positions < 1)) HB_REFUSE("qk_norm_rope_kv_write8: a rotation needs its table");
     if ((q_weight == nullptr) != (k_weight == nullptr)) HB_REFUSE("qk_norm_rope_kv_write8: give both norm weights or none");
-    if (kv && !write_index) HB_REFUSE("qk_norm_rope_kv_write8: writing the cache needs write_index");
     if (kv_heads < 1 || heads < 1) HB_REFUSE("qk_norm_rope_kv_write8: %d heads, %d kv heads", heads, kv_heads);
     if (((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)bias | (uintptr_t)kv) % 4) HB_REFUSE("qk_norm_rope_kv_write8: tensors must start on 4 bytes");
     cudaStream_t s = (cudaStream_t)stream;
-    const long units = (long)tokens * (heads + (kv ? 2 * kv_heads : 0));
+    const long units = (long)tokens * (heads + 2 * kv_heads);
 #define HB_ARGS(TW) (bf16*)q_out, (const bf16*)qkv, positions, table, rotary_dim, max_positions, (const TW*)q_weight, (const TW*)k_weight, \
     eps, offset, (unsigned char*)kv, write_index, pages, page_size, units, heads, kv_heads, head_dim, (const bf16*)bias
     const bool aligned = ((uintptr_t)q_out | (uintptr_t)qkv | (uintptr_t)table | (uintptr_t)q_weight | (uintptr_t)k_weight | (uintptr_t)kv | (uintptr_t)bias) % 16 == 0;
@@ -302,7 +302,7 @@ extern "C" int hb_qk_norm_rope_kv_write8(void* q_out, const void* qkv, const int
     if (sms == 0) HB_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, 0));
 #define HB_LANES(TW, N) qk_norm_rope_kv_write8_lanes_kernel<TW, N><<<(unsigned)min(blocks, 3l * sms), 256, 0, s>>>( \
         (bf16*)q_out, (const bf16*)qkv, positions, table, rotary_dim, max_positions, (const TW*)q_weight, (const TW*)k_weight, eps, offset, \
-        (unsigned char*)kv, write_index, pages, page_size, page_size & (page_size - 1) ? -1 : __builtin_ctz(page_size | (page_size == 0)), (unsigned)units, heads, kv_heads, head_dim, (const bf16*)bias)
+        (unsigned char*)kv, write_index, pages, page_size, page_size & (page_size - 1) ? -1 : __builtin_ctz(page_size), (unsigned)units, heads, kv_heads, head_dim, (const bf16*)bias)
 #define HB_WRITE(TW) do { \
         if (!lanes) qk_norm_rope_kv_write8_kernel<TW><<<(unsigned)blocks, 128, 4 * head_dim * sizeof(float), s>>>(HB_ARGS(TW)); \
         else if (width == 2) HB_LANES(TW, 2); \

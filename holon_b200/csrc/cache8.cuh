@@ -11,7 +11,6 @@
 
 #define C8_LOW -64                    // the least exponent of a scale: rows whose largest magnitude is below 2^-55 lose bits
 #define C8_HIGH 120
-#define C8_MAX 448.f
 
 // The exponent of the scale of a row whose largest finite magnitude is `largest`.
 __device__ __forceinline__ int c8_exponent(float largest) {
