@@ -634,7 +634,7 @@ class CudaKernels:
         common = (self._i32(block_table, "block_table"), block_table.shape[1], self._i32(rows.row_slot, "row_slot"),
                   self._i32(rows.query_start, "query_start"), self._i32(rows.kv_len, "kv_len"))
         for first, last, length in self._read_back_portions(rows, block_table.shape[1] * page_size):
-            count = last - first
+            count, back = last - first, None                         # (the turn before gives its scratch back first)
             back = torch.empty((count, 2, kv_heads, length, head_dim), dtype=torch.bfloat16, device=self.device)
             tables = torch.empty(count + last, dtype=torch.int32, device=self.device)
             table, slots = tables[:count], tables[count:]

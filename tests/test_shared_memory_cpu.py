@@ -24,3 +24,24 @@ def test_scratch_of_steps(cache_dtype, shared):
     back, together = 1000 * 5 * (cache_dtype == "fp8"), 4 * 5 * config["num_attention_heads"] * 32 * shared
     assert b.model.context_scratch(100, 5, 500) == back + together
     assert b.model.graph_scratch(5, 0, 500, 32) == together
+
+
+def test_one_portion_of_scratch_at_a_time(monkeypatch):
+    """Rows of several tokens that are read back in turns hold the scratch of one turn: that is what the account has."""
+    import weakref
+
+    import torch
+
+    from test_cache8_cpu import attend
+    empty, made, most = torch.empty, [], [0]
+
+    def watched(*a, **kw):
+        t = empty(*a, **kw)
+        if t.dim() == 5:
+            made.append(weakref.ref(t))
+            most[0] = max(most[0], sum(r() is not None for r in made))
+        return t
+
+    monkeypatch.setattr(torch, "empty", watched)
+    attend([100, 200, 300], [9, 50, 300], dim=64, READ_BACK_TOKENS=400)
+    assert len(made) == 3 and most[0] == 1
