@@ -62,11 +62,15 @@ class SharedPrefix:
         self.longest_own, self.saved, self.page_size = longest_own, saved, page_size
 
     @classmethod
-    def find(cls, table: np.ndarray, kv_len: np.ndarray, page_size: int, row_slot: np.ndarray) -> dict | None:
+    def find(cls, table: np.ndarray, kv_len: np.ndarray, page_size: int, row_slot: np.ndarray, least: int = 0) -> dict | None:
         """The arrays (host), `longest_own` and `saved` for rows that hold `kv_len` tokens in the pages `table` [rows, pages], the rows
-        `row_slot` of the block table; None where no group is worth it. Rows that share more with some than with others go with the cut that saves most."""
+        `row_slot` of the block table; None where no group is worth it, or where the rows cannot save `least` tokens whatever they share
+        (of each group one row's tokens are read, so at most all but the longest row's are saved). Rows that share more with some than with
+        others go with the cut that saves most."""
         n = len(kv_len)
         limit = np.maximum((np.asarray(kv_len, dtype=np.int64) - 1) // page_size, 0)      # (a row's last token stays its own)
+        if n < 2 or int(limit.sum() - limit.max()) * page_size < least:
+            return None
         first = table[:, 0] if n > 1 and table.shape[1] else np.zeros(0, dtype=np.int32)
         if len(np.unique(first)) == len(first):                       # (no two rows begin alike)
             return None

@@ -143,7 +143,7 @@ class Runner:
         one = n_decode + pad_rows
         sharing = {}
         for i in self._sharing if n_decode > 1 else ():
-            found = SharedPrefix.find(c.groups[i].table[row_slot[:one]], kv_len[:one], c.groups[i].page_size, row_slot)
+            found = SharedPrefix.find(c.groups[i].table[row_slot[:one]], kv_len[:one], c.groups[i].page_size, row_slot, self._sharing[i])
             if found is not None and found["saved"] >= self._sharing[i]:
                 sharing[i] = found
                 for name in ("skip", "members", "groups"):
