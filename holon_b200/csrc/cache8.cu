@@ -88,7 +88,8 @@ __global__ void __launch_bounds__(128) qk_norm_rope_kv_write8_kernel(
 // The same with LANES lanes a (token, head), heads of up to 16 LANES numbers and rotations of a multiple of 16: a lane holds two
 // chunks of 8, where the head turns the two that pair (chunk c of the first half of the turned numbers and c of the second), so
 // that every access is 16 bytes wide, sums and maxima are shuffles and nothing goes through shared memory. 4,096 tokens of 32 + 8
-// heads of 128: 90 us in the kernel above, 27.6 us here (92 MB, 3.3 TB/s), bound by its instructions: 65% of the issue slots are taken.
+// heads of 128: 90 us in the kernel above, 27.6 us here (92 MB, 3.3 TB/s). No unit is at its limit (66% of the issue slots, 22% of DRAM): it waits for
+// its loads with 24 warps an SM, and every one of a token's heads loads the rotation's row and the gains and multiplies them anew.
 __device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
