@@ -47,7 +47,7 @@ def cut(groups, rows_per_tile):
 
 def test_units_are_bounded(chunks):
     rng = random.Random(7)
-    shapes = [([(8, n)], 8, 296) for n in (64, 128, 15360, 30720, 31488, 37888, 88064, 90000, 1 << 20)]      # (one kv head of 64, eight query heads)
+    shapes = [([(8, n)], 8, 296) for n in (64, 128, 15360, 30656, 31488, 37888, 88064, 90000, 1 << 20)]      # (one kv head of 64, eight query heads)
     shapes += [([(2, 40000), (2, 64), (9, 640)], 64 // g, each) for g in (1, 8, 64) for each in (296, 148, 18, 1)]
     for _ in range(3000):
         n = rng.randint(1, 40)
